@@ -15,8 +15,9 @@ DMT_F32, DMT_BF16, DMT_FP8_E4M3 = 0, 1, 2
 DMT_OPT_SGD, DMT_OPT_ADAGRAD, DMT_OPT_ADADELTA, DMT_OPT_RMSPROP, DMT_OPT_FTRL = 1, 2, 3, 4, 5
 DMT_MAX_FEATURES, DMT_MAX_SEQS, DMT_MAX_TABLES = 32, 4, 32
 DMT_SEQ_TARGET = 100
+DMT_KV_BLOCK = 64
 DMT_ERR_UNSUPPORTED = -3
-DMT_ABI_VERSION = 6        # include/dmt_hip.h: the revision this binding was written against (checked by load())
+DMT_ABI_VERSION = 7        # include/dmt_hip.h: the revision this binding was written against (checked by load())
 
 c_i32, c_i64, c_f32, c_vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
@@ -136,6 +137,22 @@ class TableMap(C.Structure):
                 ("elem_off", c_i64 * DMT_MAX_TABLES), ("shard_w", c_i32), ("shard_r", c_i32)]
 
 
+class AttnVarDesc(C.Structure):
+    _fields_ = [("dtype", c_i32), ("B", c_i32), ("Hq", c_i32), ("Hkv", c_i32), ("dh", c_i32), ("max_q", c_i32), ("max_k", c_i32),
+                ("rows_q", c_i64), ("rows_k", c_i64), ("Q", c_vp), ("q_rs", c_i64), ("K", c_vp), ("k_rs", c_i64), ("V", c_vp), ("v_rs", c_i64),
+                ("q_off", c_vp), ("q_lens", c_vp), ("k_off", c_vp), ("k_lens", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32),
+                ("slopes", c_vp), ("prefix", c_vp), ("q_doc", c_vp), ("k_doc", c_vp), ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp),
+                ("dout", c_vp), ("do_rs", c_i64), ("dQ", c_vp), ("dq_rs", c_i64), ("dK", c_vp), ("dk_rs", c_i64),
+                ("dV", c_vp), ("dv_rs", c_i64), ("dslopes", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
+
+
+class KvAttnDesc(C.Structure):
+    _fields_ = [("n", c_i32), ("Hq", c_i32), ("Hkv", c_i32), ("dh", c_i32), ("n_blocks", c_i32), ("max_q", c_i32), ("max_len", c_i32),
+                ("width", c_i32), ("rows", c_i64), ("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("Q", c_vp), ("q_rs", c_i64),
+                ("table", c_vp), ("lens", c_vp), ("row_off", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32), ("slopes", c_vp),
+                ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
+
+
 _SIGS = {
     "dmt_gather_fwd": [C.POINTER(GatherDesc), c_vp],
     "dmt_embgrad_keys": [C.POINTER(EmbGradDesc), c_vp, c_vp, c_vp],
@@ -214,10 +231,18 @@ _SIGS = {
     "dmt_mhsa_image_bytes": [C.POINTER(c_i64)],
     "dmt_mhsa_image_build": [c_vp, c_i64, c_vp, c_vp],
     "dmt_mhsa_block_fwd": [C.POINTER(MhsaDesc), c_vp],
+    "dmt_attn_var_fwd": [C.POINTER(AttnVarDesc), c_vp],
+    "dmt_attn_var_bwd": [C.POINTER(AttnVarDesc), c_vp],
+    "dmt_kv_plan": [c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_uint64, c_vp],
+    "dmt_kv_release": [c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp],
+    "dmt_kv_append": [c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp],
+    "dmt_kv_read": [c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp],
+    "dmt_kv_attn": [C.POINTER(KvAttnDesc), c_vp],
 }
 
 EXPORTED_SYMBOLS = sorted(list(_SIGS.keys()) + ["dmt_last_error", "dmt_version", "dmt_build_arch", "dmt_ln_bwd_partials", "dmt_struct_size", "dmt_chain_supported", "dmt_proj_supported", "dmt_image_job_bytes",
-                                                 "dmt_attn_long_supported", "dmt_mmoe_experts_supported", "dmt_mmoe_experts_ws_bytes", "dmt_heads_supported", "dmt_q1mem_supported", "dmt_reduce_det_ws_bytes", "dmt_wgrad320_det_ws_bytes", "dmt_route_trace", "dmt_route_count", "dmt_route_dump"])
+                                                 "dmt_attn_long_supported", "dmt_mmoe_experts_supported", "dmt_mmoe_experts_ws_bytes", "dmt_heads_supported", "dmt_q1mem_supported", "dmt_reduce_det_ws_bytes", "dmt_wgrad320_det_ws_bytes", "dmt_route_trace", "dmt_route_count", "dmt_route_dump",
+                                                 "dmt_attn_var_supported", "dmt_attn_var_ws_bytes", "dmt_kv_plan_ws_bytes", "dmt_kv_attn_ws_bytes"])
 
 _lib = None
 
@@ -273,6 +298,14 @@ def load():
     lib.dmt_attn_long_supported.argtypes = [c_i32, c_i32, c_i32, c_i32]
     lib.dmt_wgrad320_det_ws_bytes.restype = C.c_uint64
     lib.dmt_wgrad320_det_ws_bytes.argtypes = [c_i64, c_i32]
+    lib.dmt_attn_var_supported.restype = c_i32
+    lib.dmt_attn_var_supported.argtypes = [c_i32] * 4
+    lib.dmt_attn_var_ws_bytes.restype = C.c_uint64
+    lib.dmt_attn_var_ws_bytes.argtypes = [C.POINTER(AttnVarDesc), c_i32]
+    lib.dmt_kv_plan_ws_bytes.restype = C.c_uint64
+    lib.dmt_kv_plan_ws_bytes.argtypes = [c_i32]
+    lib.dmt_kv_attn_ws_bytes.restype = C.c_uint64
+    lib.dmt_kv_attn_ws_bytes.argtypes = [C.POINTER(KvAttnDesc)]
     lib.dmt_route_trace.restype = c_i32
     lib.dmt_route_trace.argtypes = [c_i32]
     lib.dmt_route_count.restype = c_i64

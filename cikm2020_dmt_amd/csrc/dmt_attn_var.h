@@ -1,0 +1,294 @@
+// What the kernels of dmt_attn_var.hip (forward) and dmt_attn_var_bwd.hip share: the arguments, the scores and masks, and the row kernels.
+//
+// Scores are kept in log2 units (z2 = z log2 e), so that a weight is one v_exp_f32: p = 2^(z2 - m2).  tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e)):
+// exact at both ends (the power runs to infinity or zero), absolute error ~2^-23, which is what a score of magnitude `cap` has anyway.
+#pragma once
+#include "dmt_common.h"
+
+namespace attn_var {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int KT = 64;              // keys (dQ and forward) or queries (dK, dV) of one tile
+constexpr int MAX_DH = 128;
+
+struct Args {
+  int B, Hq, Hkv, dh, G;
+  int max_q, max_k;
+  long long rows_q, rows_k;
+  const void* Q; long long q_rs;
+  const void* K; long long k_rs;
+  const void* V; long long v_rs;
+  const int* q_off; const int* q_lens; const int* k_off; const int* k_lens;
+  float scale, cap;
+  int causal;
+  const float* slopes;
+  const int* prefix;
+  const int* q_doc; const int* k_doc;
+  void* out; long long o_rs;
+  float* lse;
+  const void* dout; long long do_rs;
+  void* dQ; long long dq_rs;
+  void* dK; long long dk_rs;
+  void* dV; long long dv_rs;
+  float* dslopes;
+  float* D;                         // [rows_q, Hq]: rowsum(dout * out)
+  float* slope_part;                // [Hq][B * ceil(max_q / 128)]
+  const int2* q_rng; const int2* k_rng;   // (least, largest) document id of every 64-row tile: [B][ceil(max / 64)]
+  int nqt, nkt;                     // 64-row tiles of max_q, max_k
+};
+
+// one example's lengths and what its queries may see
+struct Ex {
+  int ql, kl, off, pre;
+  long long q0, k0;
+};
+// (a length is cut where its rows would leave the matrix, a start outside it leaves nothing: no index of a caller reaches past the operands)
+__device__ __forceinline__ int clip_len(int len, int most, int first, long long rows) {
+  if (first < 0 || len <= 0) return 0;
+  long long m = len < most ? len : most;
+  if (first + m > rows) m = rows - first;
+  return m > 0 ? (int)m : 0;
+}
+__device__ __forceinline__ Ex example(const Args& a, int b) {
+  Ex e;
+  e.q0 = a.q_off[b];
+  e.k0 = a.k_off[b];
+  e.ql = clip_len(a.q_lens[b], a.max_q, (int)e.q0, a.rows_q);
+  e.kl = clip_len(a.k_lens[b], a.max_k, (int)e.k0, a.rows_k);
+  e.off = e.kl - e.ql;
+  const int p = a.prefix ? a.prefix[b] : 0;
+  e.pre = p < 0 ? 0 : (p > e.kl ? e.kl : p);
+  return e;
+}
+
+// constants of one head's scores: z2 = shaped ? ... : c1 s
+struct Shape {
+  float c1;        // scale log2e
+  float cap2;      // cap log2e
+  float ck;        // 2 log2e scale / cap
+  float sl2;       // slope log2e
+  bool cap, slope;
+};
+__device__ __forceinline__ Shape shape_of(const Args& a, int h) {
+  Shape s;
+  s.c1 = a.scale * LOG2E;
+  s.cap = a.cap > 0.f;
+  s.cap2 = a.cap * LOG2E;
+  s.ck = s.cap ? 2.f * LOG2E * a.scale / a.cap : 0.f;
+  s.slope = a.slopes != nullptr;
+  s.sl2 = s.slope ? a.slopes[h] * LOG2E : 0.f;
+  return s;
+}
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
+// 1 / (1 + 2^(ck s)) = (1 - tanh) / 2, from which tanh = 1 - 2 r and its derivative 1 - tanh^2 = 4 r (1 - r) follow
+__device__ __forceinline__ float cap_r(const Shape& s, float x) { return rcp_hw(1.f + exp2_hw(s.ck * x)); }
+__device__ __forceinline__ float z2_of(const Shape& s, float x, float dist) {
+  float y = s.cap ? __builtin_fmaf(-2.f * s.cap2, cap_r(s, x), s.cap2) : s.c1 * x;
+  if (s.slope) y = __builtin_fmaf(-s.sl2, fabsf(dist), y);
+  return y;
+}
+
+template <typename T> __device__ __forceinline__ float dot_rows(const float* __restrict__ q, const T* __restrict__ k, int dh) {
+  float s = 0.f;
+  for (int c = 0; c < dh; ++c) s = __builtin_fmaf(q[c], ldf<T>(k + c), s);
+  return s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- rows, one at a time
+// One wavefront computes one row with plain arithmetic: 64 keys at a time, a lane per key for the scores, a lane per dim for the sums; only
+// what the row may see is ever read into a sum.  It is the form that holds whatever the operands hold: the tile kernels multiply the
+// weight 0 of a masked place into what stands there, so a row that comes out of them not finite is computed again here.
+// lds: [2 * MAX_DH + 2 * 64] floats of the wavefront's own.
+__device__ __forceinline__ void lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+constexpr int ROW_LDS = 2 * MAX_DH + 2 * 64;
+
+__device__ __forceinline__ bool may_see(const Args& a, const Ex& e, int i, int j, int qd) {
+  if (j >= e.kl) return false;
+  if (j < e.pre) return true;
+  if (a.causal && j > i + e.off) return false;
+  return a.q_doc == nullptr || a.k_doc[e.k0 + j] == qd;
+}
+
+template <typename T>
+__device__ void row_fwd(const Args& a, const Ex& e, int h, int i, float* lds, int lane) {
+  float* q = lds;
+  float* pl = lds + 2 * MAX_DH;
+  const int dh = a.dh, hk = h / a.G;
+  const T* Q = (const T*)a.Q + (e.q0 + i) * a.q_rs + (long long)h * dh;
+  const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * dh;
+  const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * dh;
+  for (int c = lane; c < dh; c += 64) q[c] = ldf<T>(Q + c);
+  lds_fence();
+  const Shape s = shape_of(a, h);
+  const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 < e.kl; j0 += 64) {
+    const int j = j0 + lane;
+    const bool ok = may_see(a, e, i, j, qd);
+    const unsigned long long vis = __ballot(ok);
+    if (!vis) continue;
+    float z = -INFINITY;
+    if (ok) z = z2_of(s, dot_rows<T>(q, K + (long long)j * a.k_rs, dh), (float)(i + e.off - j));
+    const float mn = fmaxf(m, wave_max(z));
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float p = ok ? exp2_hw(z - mu) : 0.f;
+    const float f = m == -INFINITY ? 0.f : exp2_hw(m - mu);
+    m = mn;
+    l = l * f + wave_sum(p);
+    o0 *= f;
+    o1 *= f;
+    pl[lane] = p;
+    lds_fence();
+    for (int t = 0; t < 64; ++t) {
+      if (!((vis >> t) & 1)) continue;
+      const float pt = pl[t];
+      const T* v = V + (long long)(j0 + t) * a.v_rs;
+      if (lane < dh) o0 = __builtin_fmaf(pt, ldf<T>(v + lane), o0);
+      if (lane + 64 < dh) o1 = __builtin_fmaf(pt, ldf<T>(v + lane + 64), o1);
+    }
+    lds_fence();
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;            // (nothing seen: 0; NaN stays)
+  const long long row = e.q0 + i;
+  T* O = (T*)a.out + row * a.o_rs + (long long)h * dh;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int c = lane + 64 * u;
+    if (c < dh) {
+      const float o = (u ? o1 : o0) * inv;
+      stf<T>(O + c, o);
+    }
+  }
+  if (a.lse && lane == 0) a.lse[row * a.Hq + h] = (m == -INFINITY && l == 0.f) ? -INFINITY : (m + __log2f(l)) * LN2;
+}
+
+// dq of one row; returns this row's part of dslopes[h] (all lanes):
+//     - sum_j |d_j| P_j (dP_j - D)  =  S0 S2 - S1,   S0 = sum P dP, S1 = sum P dP |d|, S2 = sum P |d|
+// with D = S0 from the same weights, not from the rounded output: the terms cancel, and dslopes is an fp32 result.
+template <typename T>
+__device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, int lane) {
+  float* q = lds;
+  float* g = lds + MAX_DH;
+  float* xl = lds + 2 * MAX_DH;
+  const int dh = a.dh, hk = h / a.G;
+  const long long row = e.q0 + i;
+  const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * dh;
+  const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * dh;
+  for (int c = lane; c < dh; c += 64) {
+    q[c] = ldf<T>((const T*)a.Q + row * a.q_rs + (long long)h * dh + c);
+    g[c] = ldf<T>((const T*)a.dout + row * a.do_rs + (long long)h * dh + c);
+  }
+  lds_fence();
+  const Shape s = shape_of(a, h);
+  const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
+  const float lse2 = a.lse[row * a.Hq + h] * LOG2E, D = a.D[row * a.Hq + h];
+  float o0 = 0.f, o1 = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f;
+  for (int j0 = 0; j0 < e.kl; j0 += 64) {
+    const int j = j0 + lane;
+    const bool ok = may_see(a, e, i, j, qd);
+    const unsigned long long vis = __ballot(ok);
+    if (!vis) continue;
+    float dx = 0.f;
+    if (ok) {
+      const float x = dot_rows<T>(q, K + (long long)j * a.k_rs, dh);
+      const float dist = (float)(i + e.off - j);
+      const float p = exp2_hw(z2_of(s, x, dist) - lse2);
+      const float dp = dot_rows<T>(g, V + (long long)j * a.v_rs, dh), pd = p * dp;
+      s0 += pd;
+      s1 = __builtin_fmaf(pd, fabsf(dist), s1);
+      s2 = __builtin_fmaf(p, fabsf(dist), s2);
+      dx = p * (dp - D);
+      if (s.cap) {
+        const float r = cap_r(s, x);
+        dx *= 4.f * r * (1.f - r);
+      }
+    }
+    xl[lane] = dx;
+    lds_fence();
+    for (int t = 0; t < 64; ++t) {
+      if (!((vis >> t) & 1)) continue;
+      const float xt = xl[t];
+      const T* k = K + (long long)(j0 + t) * a.k_rs;
+      if (lane < dh) o0 = __builtin_fmaf(xt, ldf<T>(k + lane), o0);
+      if (lane + 64 < dh) o1 = __builtin_fmaf(xt, ldf<T>(k + lane + 64), o1);
+    }
+    lds_fence();
+  }
+  T* O = (T*)a.dQ + row * a.dq_rs + (long long)h * dh;
+  if (lane < dh) stf<T>(O + lane, o0 * a.scale);
+  if (lane + 64 < dh) stf<T>(O + lane + 64, o1 * a.scale);
+  s0 = wave_sum(s0);
+  return __builtin_fmaf(s0, wave_sum(s2), -wave_sum(s1));
+}
+
+// dk and dv of one key row: over the query heads of its group, then over the queries
+template <typename T>
+__device__ void row_dkv(const Args& a, const Ex& e, int hk, int j, float* lds, int lane) {
+  float* k = lds;
+  float* v = lds + MAX_DH;
+  float* pl = lds + 2 * MAX_DH;
+  float* xl = pl + 64;
+  const int dh = a.dh;
+  const long long row = e.k0 + j;
+  for (int c = lane; c < dh; c += 64) {
+    k[c] = ldf<T>((const T*)a.K + row * a.k_rs + (long long)hk * dh + c);
+    v[c] = ldf<T>((const T*)a.V + row * a.v_rs + (long long)hk * dh + c);
+  }
+  lds_fence();
+  float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
+  for (int h = hk * a.G; h < hk * a.G + a.G; ++h) {
+    const Shape s = shape_of(a, h);
+    const T* Q = (const T*)a.Q + e.q0 * a.q_rs + (long long)h * dh;
+    const T* O = (const T*)a.dout + e.q0 * a.do_rs + (long long)h * dh;
+    for (int i0 = 0; i0 < e.ql; i0 += 64) {
+      const int i = i0 + lane;
+      const bool ok = i < e.ql && may_see(a, e, i, j, a.q_doc ? a.q_doc[e.q0 + i] : 0);
+      const unsigned long long vis = __ballot(ok);
+      if (!vis) continue;
+      float p = 0.f, dx = 0.f;
+      if (ok) {
+        const long long qr = (e.q0 + i) * a.Hq + h;
+        const float x = dot_rows<T>(k, Q + (long long)i * a.q_rs, dh);
+        p = exp2_hw(z2_of(s, x, (float)(i + e.off - j)) - a.lse[qr] * LOG2E);
+        dx = p * (dot_rows<T>(v, O + (long long)i * a.do_rs, dh) - a.D[qr]);
+        if (s.cap) {
+          const float r = cap_r(s, x);
+          dx *= 4.f * r * (1.f - r);
+        }
+      }
+      pl[lane] = p;
+      xl[lane] = dx;
+      lds_fence();
+      for (int t = 0; t < 64; ++t) {
+        if (!((vis >> t) & 1)) continue;
+        const float pt = pl[t], xt = xl[t];
+        const T* qr = Q + (long long)(i0 + t) * a.q_rs;
+        const T* gr = O + (long long)(i0 + t) * a.do_rs;
+        if (lane < dh) {
+          k0 = __builtin_fmaf(xt, ldf<T>(qr + lane), k0);
+          v0 = __builtin_fmaf(pt, ldf<T>(gr + lane), v0);
+        }
+        if (lane + 64 < dh) {
+          k1 = __builtin_fmaf(xt, ldf<T>(qr + lane + 64), k1);
+          v1 = __builtin_fmaf(pt, ldf<T>(gr + lane + 64), v1);
+        }
+      }
+      lds_fence();
+    }
+  }
+  T* dk = (T*)a.dK + row * a.dk_rs + (long long)hk * dh;
+  T* dv = (T*)a.dV + row * a.dv_rs + (long long)hk * dh;
+  if (lane < dh) { stf<T>(dk + lane, k0 * a.scale); stf<T>(dv + lane, v0); }
+  if (lane + 64 < dh) { stf<T>(dk + lane + 64, k1 * a.scale); stf<T>(dv + lane + 64, v1); }
+}
+
+}  // namespace attn_var
+
+int dmt_attn_var_args(const dmt_attn_var_desc* d, attn_var::Args* a, bool backward, const char* what);
+int dmt_attn_var_doc_ranges(const attn_var::Args& a, void* stream);

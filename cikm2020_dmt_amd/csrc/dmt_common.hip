@@ -80,6 +80,8 @@ extern "C" int dmt_struct_size(int which) {
     case 12: return (int)sizeof(dmt_heads_desc);
     case 13: return (int)sizeof(dmt_q1mem_desc);
     case 14: return (int)sizeof(dmt_mhsa_bwd_desc);
+    case 15: return (int)sizeof(dmt_attn_var_desc);
+    case 16: return (int)sizeof(dmt_kv_attn_desc);
     default: return -1;
   }
 }

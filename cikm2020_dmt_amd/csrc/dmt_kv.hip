@@ -1,0 +1,529 @@
+// K / V cache in 8 bits for served histories: block tables and slots, append, read back, attention (include/dmt_hip.h: dmt_kv_*).
+//
+// Layout of a block (64 tokens of one request) for one key / value head:
+//   K [64 tokens][dh]       the A operand of S^T = K Q^T: a lane's 8 (or 16) contraction values lie side by side;
+//   V [dh][64 places]       the A operand of O^T = V^T P^T.  A 16x16 product leaves lane group b = lane / 16 with the weights of tokens
+//                           16 a + 4 b + r (a = tile, r = register): place 16 b + 4 a + r puts the 16 tokens of a group side by side.
+#include "dmt_common.h"
+
+namespace {
+
+constexpr int BS = DMT_KV_BLOCK;
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr int MAX_DH = 128;
+constexpr float F8_MAX = 448.f;
+
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+__host__ __device__ __forceinline__ int place_of(int t) { return 16 * ((t >> 2) & 3) + 4 * (t >> 4) + (t & 3); }
+__device__ __forceinline__ float f8_to_f32(unsigned byte) { return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0); }
+// nearest e4m3, ties to even; infinities and what is past the largest value -> +-448, NaN stays
+__device__ __forceinline__ float f8_clamp(float x) { return x > F8_MAX ? F8_MAX : (x < -F8_MAX ? -F8_MAX : x); }
+__device__ __forceinline__ unsigned f32_to_f8x2(float a, float b) {
+  return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(f8_clamp(a), f8_clamp(b), 0, false) & 0xffffu;
+}
+// least power of two s >= 2^-100 with a <= 448 s  (448 = 1.75 * 2^8; a finite, >= 0)
+__device__ __forceinline__ int scale_exp(float a) {
+  const unsigned u = __float_as_uint(a);
+  const int e = (int)(u >> 23) - 127;
+  const int s = e - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return s < -100 ? -100 : s;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+// ================================================================================================================ plan
+// The sums run over the requests in chunks of one workgroup (1024): rows, blocks wanted, runs.  What a row needs -- its request, position,
+// block -- it then finds by itself (a binary search over row_off), so the second part is as wide as there are rows; with few rows and
+// requests the first workgroup does it too and there is one launch.
+constexpr int PLAN_NT = 1024;
+constexpr int PLAN_SMALL_ROWS = 4096;
+
+struct PlanArgs {
+  int n, rows, width, max_runs;
+  const int* lens; const int* new_lens; int* table; const int* free_ids; const int* n_free;
+  int* row_off; int* lens_out; int* slots; int* run_row; int* run_len; int* state;
+  int free_cap;
+  int2* req;        // [n]: (index of the request's first new block among the step's new blocks, or -1 when refused; first run)
+  int* totals;      // {runs}
+};
+__device__ __forceinline__ int free_count(const PlanArgs& a) { return a.n_free[0] < a.free_cap ? a.n_free[0] : a.free_cap; }
+
+__device__ __forceinline__ long long wg_scan(long long v, long long* red, int tid, long long& total) {
+  // inclusive sum over the workgroup
+  const int lane = tid & 63, wave = tid >> 6;
+  long long x = v;
+#pragma unroll
+  for (int s = 1; s < 64; s <<= 1) {
+    const long long y = __shfl_up(x, s);
+    if (lane >= s) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) red[wave] = x;
+  __syncthreads();
+  long long base = 0, all = 0;
+  for (int w = 0; w < PLAN_NT / 64; ++w) {
+    const long long r = red[w];
+    if (w < wave) base += r;
+    all += r;
+  }
+  total = all;
+  return x + base;
+}
+
+__device__ void plan_rows(const PlanArgs& a, int t, int step, int total, int runs) {
+  const int n_free = free_count(a);
+  for (; t < a.rows; t += step) {
+    int slot = -1;
+    if (t < total) {
+      int lo = 0, hi = a.n;                       // request r: row_off[r] <= t < row_off[r + 1]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.row_off[mid] <= t) lo = mid; else hi = mid;
+      }
+      const int r = lo;
+      const int2 rq = a.req[r];
+      if (rq.x >= 0) {
+        const int first = a.row_off[r], len = a.lens[r];
+        const int pos = len + t - first, bi = pos / BS, have = (len + BS - 1) / BS;
+        const int block = bi < have ? a.table[(long long)r * a.width + bi] : a.free_ids[n_free - 1 - (rq.x + bi - have)];
+        slot = block * BS + pos % BS;
+        if (t == first || pos % BS == 0) {
+          const int run = rq.y + bi - len / BS;
+          const int left = a.row_off[r + 1] - t, room = BS - pos % BS;
+          a.run_row[run] = t;
+          a.run_len[run] = left < room ? left : room;
+          if (bi >= have) a.table[(long long)r * a.width + bi] = block;
+        }
+      }
+    }
+    a.slots[t] = slot;
+    if (t >= runs && t < a.max_runs) {
+      a.run_row[t] = -1;
+      a.run_len[t] = 0;
+    }
+  }
+}
+
+__global__ __launch_bounds__(PLAN_NT) void plan_kernel(const PlanArgs a, int small) {
+  __shared__ long long red[PLAN_NT / 64];
+  const int tid = threadIdx.x;
+  long long row_base = 0, need_base = 0, run_base = 0, taken = 0, refused = 0, tot;
+  const long long n_free = free_count(a);
+  for (int r0 = 0; r0 < a.n; r0 += PLAN_NT) {
+    const int r = r0 + tid;
+    const bool in = r < a.n;
+    const int len = in ? a.lens[r] : 0, nw = in ? a.new_lens[r] : 0;
+    const long long rows = nw > 0 ? nw : 0;
+    const long long row_end = row_base + wg_scan(rows, red, tid, tot);
+    row_base += tot;
+    const bool fits = in && nw >= 0 && len >= 0 && (long long)len + nw <= (long long)a.width * BS && row_end <= a.rows;
+    const long long need = fits ? ((long long)len + nw + BS - 1) / BS - ((long long)len + BS - 1) / BS : 0;
+    const long long need_end = need_base + wg_scan(need, red, tid, tot);
+    need_base += tot;
+    const bool ok = fits && (need == 0 || need_end <= n_free);
+    const long long runs = ok && nw > 0 ? ((long long)len + nw + BS - 1) / BS - len / BS : 0;
+    const long long run_end = run_base + wg_scan(runs, red, tid, tot);
+    run_base += tot;
+    wg_scan(ok ? need : 0, red, tid, tot);
+    taken += tot;
+    wg_scan(in && !ok ? 1 : 0, red, tid, tot);
+    refused += tot;
+    if (in) {
+      const long long row_first = row_end - rows;
+      a.row_off[r] = (int)(row_first < 0x7fffffffll ? row_first : 0x7fffffffll);
+      if (r == a.n - 1) a.row_off[a.n] = (int)(row_end < 0x7fffffffll ? row_end : 0x7fffffffll);
+      a.lens_out[r] = ok ? len + nw : len;
+      a.req[r] = make_int2(ok ? (int)(need_end - need) : -1, (int)(run_end - runs));
+    }
+  }
+  if (tid == 0) {
+    if (a.n == 0) a.row_off[0] = 0;
+    a.state[0] = (int)(n_free - taken);
+    a.state[1] = (int)refused;
+    a.totals[0] = (int)run_base;
+  }
+  if (small) {
+    __threadfence_block();
+    __syncthreads();
+    plan_rows(a, tid, PLAN_NT, row_base < 0x7fffffffll ? (int)row_base : 0x7fffffff, (int)run_base);
+  }
+}
+
+__global__ __launch_bounds__(256) void plan_rows_kernel(const PlanArgs a) {
+  plan_rows(a, blockIdx.x * 256 + threadIdx.x, 0x40000000, a.row_off[a.n], a.totals[0]);
+}
+
+__global__ __launch_bounds__(PLAN_NT) void release_kernel(int n, const int* done, int* lens, const int* table, int width, int* free_ids, int* n_free,
+                                                          int cap) {
+  __shared__ long long red[PLAN_NT / 64];
+  const int tid = threadIdx.x;
+  long long base = n_free[0], tot;
+  for (int r0 = 0; r0 < n; r0 += PLAN_NT) {
+    const int r = r0 + tid;
+    const bool in = r < n && done[r] != 0 && lens[r] > 0;
+    long long mine = in ? ((long long)lens[r] + BS - 1) / BS : 0;
+    if (mine > width) mine = width;
+    const long long end = base + wg_scan(mine, red, tid, tot);
+    base += tot;
+    if (in) {
+      long long at = end - mine;
+      for (int j = 0; j < (int)mine; ++j, ++at)
+        if (at >= 0 && at < cap) free_ids[at] = table[(long long)r * width + j];
+      lens[r] = 0;
+    }
+  }
+  __syncthreads();
+  if (tid == 0) n_free[0] = (int)(base < cap ? base : cap);
+}
+
+// ================================================================================================================ append / read
+struct Cache {
+  int Hkv, dh, n_blocks;
+  uint8_t* k; uint8_t* v;
+  float* ks; float* vs;
+};
+
+// One workgroup owns a (run, head): its rows are held in registers between the maximum and the rounding.
+__global__ __launch_bounds__(256) void append_kernel(const Cache c, int rows, const bf16_t* kr, long long k_rs, const bf16_t* vr, long long v_rs,
+                                                     const int* slots, const int* run_row, const int* run_len) {
+  __shared__ float red[2][4];
+  __shared__ __attribute__((aligned(16))) unsigned char vt[MAX_DH * BS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = blockIdx.y, dh = c.dh, ch = dh / 8;
+  const int row0 = run_row[blockIdx.x];
+  int len = run_len[blockIdx.x];
+  if (row0 < 0 || row0 >= rows || len <= 0) return;
+  const int slot = slots[row0], block = slot / BS, first = slot % BS;
+  if (slot < 0 || block >= c.n_blocks) return;
+  if (len > BS - first) len = BS - first;
+  if (len > rows - row0) len = rows - row0;
+  const long long bh = (long long)block * c.Hkv + hk;
+  uint8_t* kb = c.k + bh * BS * dh;
+  uint8_t* vb = c.v + bh * BS * dh;
+  uint4 kx[4], vx[4];
+  float ka = 0.f, va = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int cc = tid + i * 256, t = cc / ch, q = cc - t * ch;
+    if (t < len) {
+      kx[i] = *reinterpret_cast<const uint4*>(kr + (row0 + t) * k_rs + (long long)hk * dh + q * 8);
+      vx[i] = *reinterpret_cast<const uint4*>(vr + (row0 + t) * v_rs + (long long)hk * dh + q * 8);
+      const unsigned* kw = reinterpret_cast<const unsigned*>(&kx[i]);
+      const unsigned* vw = reinterpret_cast<const unsigned*>(&vx[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const float x = fabsf(__uint_as_float(s ? (kw[e] & 0xffff0000u) : (kw[e] << 16)));
+          const float y = fabsf(__uint_as_float(s ? (vw[e] & 0xffff0000u) : (vw[e] << 16)));
+          if (x < INFINITY) ka = fmaxf(ka, x);
+          if (y < INFINITY) va = fmaxf(va, y);
+        }
+      }
+    }
+  }
+  ka = wave_max(ka);
+  va = wave_max(va);
+  if (lane == 0) { red[0][wave] = ka; red[1][wave] = va; }
+  __syncthreads();
+  ka = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  va = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+  float ks = pow2(scale_exp(ka)), vs = pow2(scale_exp(va));
+  const float ks0 = c.ks[bh], vs0 = c.vs[bh];
+  const bool older = first > 0;
+  const bool k_grow = older && ks > ks0, v_grow = older && vs > vs0;
+  if (older) {
+    ks = fmaxf(ks, ks0);
+    vs = fmaxf(vs, vs0);
+  }
+  const float ki = 1.f / ks, vi = 1.f / vs;       // (powers of two: exact)
+  __syncthreads();                                // (every thread has read the old scales)
+  if (tid == 0) { c.ks[bh] = ks; c.vs[bh] = vs; }
+  if (k_grow) {
+    const float f = ks0 * ki;
+    for (int x = tid * 4; x < first * dh; x += 1024) {
+      const unsigned w = *reinterpret_cast<unsigned*>(kb + x);
+      const unsigned lo = f32_to_f8x2(f8_to_f32(w & 255) * f, f8_to_f32((w >> 8) & 255) * f);
+      const unsigned hi = f32_to_f8x2(f8_to_f32((w >> 16) & 255) * f, f8_to_f32(w >> 24) * f);
+      *reinterpret_cast<unsigned*>(kb + x) = lo | (hi << 16);
+    }
+  }
+  // V: the block passes through LDS (its bytes lie across the tokens)
+  for (int x = tid * 16; x < dh * BS; x += 4096) *reinterpret_cast<uint4*>(vt + x) = *reinterpret_cast<const uint4*>(vb + x);
+  __syncthreads();
+  if (v_grow) {
+    const float f = vs0 * vi;
+    for (int x = tid; x < dh * first; x += 256) {
+      const int dd = x / first, at = dd * BS + place_of(x - dd * first);
+      vt[at] = (unsigned char)f32_to_f8x2(f8_to_f32(vt[at]) * f, 0.f);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int cc = tid + i * 256, t = cc / ch, q = cc - t * ch;
+    if (t < len) {
+      const unsigned* kw = reinterpret_cast<const unsigned*>(&kx[i]);
+      const unsigned* vw = reinterpret_cast<const unsigned*>(&vx[i]);
+      unsigned o[2] = {0u, 0u};
+      const int pl = place_of(first + t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e >> 1] |= f32_to_f8x2(__uint_as_float(kw[e] << 16) * ki, __uint_as_float(kw[e] & 0xffff0000u) * ki) << (16 * (e & 1));
+        const unsigned y = f32_to_f8x2(__uint_as_float(vw[e] << 16) * vi, __uint_as_float(vw[e] & 0xffff0000u) * vi);
+        vt[(q * 8 + 2 * e) * BS + pl] = (unsigned char)y;
+        vt[(q * 8 + 2 * e + 1) * BS + pl] = (unsigned char)(y >> 8);
+      }
+      *reinterpret_cast<uint2*>(kb + (long long)(first + t) * dh + q * 8) = make_uint2(o[0], o[1]);
+    }
+  }
+  __syncthreads();
+  for (int x = tid * 16; x < dh * BS; x += 4096) *reinterpret_cast<uint4*>(vb + x) = *reinterpret_cast<const uint4*>(vt + x);
+}
+
+// A workgroup reads 64 listed slots of one head: K a lane per 8 dims, V a lane per slot (the tokens of a block share its 64-byte rows).
+__global__ __launch_bounds__(256) void read_kernel(const Cache c, int n, const int* slots, bf16_t* kr, long long k_rs, bf16_t* vr, long long v_rs) {
+  __shared__ __attribute__((aligned(16))) bf16_t tile[64 * (MAX_DH + 8)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = blockIdx.y, dh = c.dh, ch = dh / 8, ld = dh + 8;
+  const int i0 = blockIdx.x * 64;
+  const int cnt = n - i0 < 64 ? n - i0 : 64;
+  for (int x = tid; x < cnt * ch; x += 256) {
+    const int i = x / ch, q = x - i * ch, slot = slots[i0 + i], block = slot / BS;
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);
+    if (slot >= 0 && block < c.n_blocks) {
+      const long long bh = (long long)block * c.Hkv + hk;
+      const uint2 w = *reinterpret_cast<const uint2*>(c.k + (bh * BS + slot % BS) * dh + q * 8);
+      const float s = c.ks[bh];
+      unsigned* ow = reinterpret_cast<unsigned*>(&o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned h = (e < 2 ? w.x : w.y) >> (16 * (e & 1));
+        ow[e] = dmt_pack_bf16(f8_to_f32(h & 255) * s, f8_to_f32((h >> 8) & 255) * s);
+      }
+    }
+    *reinterpret_cast<uint4*>(kr + (long long)(i0 + i) * k_rs + (long long)hk * dh + q * 8) = o;
+  }
+  const int slot = lane < cnt ? slots[i0 + lane] : -1, block = slot / BS;
+  const bool ok = slot >= 0 && block < c.n_blocks;
+  const long long bh = ok ? (long long)block * c.Hkv + hk : 0;
+  const float s = ok ? c.vs[bh] : 0.f;
+  const uint8_t* src = c.v + bh * BS * dh + (ok ? place_of(slot % BS) : 0);
+  for (int j = wave; j < dh; j += 4) tile[lane * ld + j] = ok ? f2bf(f8_to_f32(src[(long long)j * BS]) * s) : (bf16_t)0;
+  __syncthreads();
+  for (int x = tid; x < cnt * ch; x += 256) {
+    const int i = x / ch, q = x - i * ch;
+    *reinterpret_cast<uint4*>(vr + (long long)(i0 + i) * v_rs + (long long)hk * dh + q * 8) = *reinterpret_cast<const uint4*>(tile + i * ld + q * 8);
+  }
+}
+
+// ================================================================================================================ attention
+struct KvArgs {
+  Cache c;
+  int n, Hq, G, max_q, max_len, width, causal;
+  long long rows;
+  const bf16_t* Q; long long q_rs;
+  const int* table; const int* lens; const int* row_off;
+  float scale, cap;
+  const float* slopes;
+  bf16_t* out; long long o_rs;
+  float* lse;
+};
+
+struct Req { int m, L; long long row0; };
+__device__ __forceinline__ Req request(const KvArgs& a, int r) {
+  Req q;
+  const long long lo = a.row_off[r], hi = a.row_off[r + 1];
+  q.row0 = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
+  long long m = (hi > a.rows ? a.rows : hi) - q.row0;
+  q.m = m < 0 ? 0 : (int)(m > a.max_q ? a.max_q : m);
+  const long long most = (long long)a.width * BS;
+  long long L = a.lens[r];
+  if (L > a.max_len) L = a.max_len;
+  if (L > most) L = most;
+  q.L = L < 0 ? 0 : (int)L;
+  return q;
+}
+// position of row i, and the number of tokens that it sees
+__device__ __forceinline__ int position(const KvArgs& a, const Req& q, int i) { return a.causal ? q.L - q.m + i : q.L; }
+__device__ __forceinline__ int sees(const KvArgs& a, const Req& q, int i) {
+  const int s = a.causal ? q.L - q.m + i + 1 : q.L;
+  return s < 0 ? 0 : s;
+}
+
+__device__ __forceinline__ float kv_z2(const KvArgs& a, float x, float slope2, float dist) {
+  float y = a.scale * LOG2E * x;
+  if (a.cap > 0.f) {
+    const float c2 = a.cap * LOG2E;
+    y = __builtin_fmaf(-2.f * c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * a.scale / a.cap * x)), c2);
+  }
+  return a.slopes ? __builtin_fmaf(-slope2, fabsf(dist), y) : y;
+}
+__device__ __forceinline__ void lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// One wavefront, one (row, head), plain arithmetic: a lane per token for the scores, a lane per dim for the sums.
+__device__ void kv_row(const KvArgs& a, const Req& rq, int r, int h, int i, float* lds, int lane) {
+  float* q = lds;
+  float* pl = lds + MAX_DH;
+  const int dh = a.c.dh, hk = h / a.G;
+  const long long row = rq.row0 + i;
+  for (int x = lane; x < dh; x += 64) q[x] = bf2f(a.Q[row * a.q_rs + (long long)h * dh + x]);
+  lds_fence();
+  const float slope2 = a.slopes ? a.slopes[h] * LOG2E : 0.f;
+  const int lim = sees(a, rq, i), pos = position(a, rq, i);
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int j0 = 0; j0 < lim; j0 += BS) {
+    const int block = a.table[(long long)r * a.width + j0 / BS];
+    if (block < 0 || block >= a.c.n_blocks) continue;
+    const long long bh = (long long)block * a.c.Hkv + hk;
+    const uint8_t* kb = a.c.k + (bh * BS + lane) * dh;
+    const uint8_t* vb = a.c.v + bh * BS * dh;
+    const float ks = a.c.ks[bh], vs = a.c.vs[bh];
+    const int j = j0 + lane;
+    const bool ok = j < lim;
+    float z = -INFINITY;
+    if (ok) {
+      float s = 0.f;
+      for (int x = 0; x < dh; ++x) s = __builtin_fmaf(q[x], f8_to_f32(kb[x]) * ks, s);
+      z = kv_z2(a, s, slope2, (float)(pos - j));
+    }
+    const float mn = fmaxf(m, wave_max(z));
+    const float mu = mn == -INFINITY ? 0.f : mn;
+    const float p = ok ? __builtin_amdgcn_exp2f(z - mu) : 0.f;
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    l = l * f + wave_sum(p);
+    o0 *= f;
+    o1 *= f;
+    pl[lane] = p;
+    lds_fence();
+    const int last = lim - j0 < BS ? lim - j0 : BS;
+    for (int t = 0; t < last; ++t) {
+      const float pt = pl[t] * vs;
+      const int pc = place_of(t);
+      if (lane < dh) o0 = __builtin_fmaf(pt, f8_to_f32(vb[(long long)lane * BS + pc]), o0);
+      if (lane + 64 < dh) o1 = __builtin_fmaf(pt, f8_to_f32(vb[(long long)(lane + 64) * BS + pc]), o1);
+    }
+    lds_fence();
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  bf16_t* O = a.out + row * a.o_rs + (long long)h * dh;
+  if (lane < dh) O[lane] = f2bf(o0 * inv);
+  if (lane + 64 < dh) O[lane + 64] = f2bf(o1 * inv);
+  if (a.lse && lane == 0) a.lse[row * a.Hq + h] = (m == -INFINITY && l == 0.f) ? -INFINITY : (m + __log2f(l)) * LN2;
+}
+
+__global__ __launch_bounds__(256) void kv_rows_kernel(const KvArgs a) {
+  __shared__ float lds[4][MAX_DH + 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.z, h = blockIdx.y;
+  const Req q = request(a, r);
+  const int i = blockIdx.x * 4 + wave;
+  if (i < q.m) kv_row(a, q, r, h, i, lds[wave], lane);
+}
+
+bool cache_ok(int Hkv, int dh, int n_blocks, const void* k, const void* v, const float* ks, const float* vs) {
+  return Hkv > 0 && Hkv <= 65535 && dh > 0 && dh <= MAX_DH && dh % 16 == 0 && n_blocks > 0 && n_blocks <= 0x7fffffff / BS && k && v && ks && vs &&
+         (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0;
+}
+const char* CACHE_MSG = "%s: bad cache (Hkv %d, dh %d -- a multiple of 16 up to 128 -- , %d blocks; 16-byte aligned pools, slots below 2^31)";
+
+}  // namespace
+
+extern "C" uint64_t dmt_kv_plan_ws_bytes(int32_t n) { return n < 0 ? 0 : 16 + 8ull * (uint64_t)n; }
+
+extern "C" int dmt_kv_plan(int32_t n, int32_t rows, const int32_t* lens, const int32_t* new_lens, int32_t* table, int32_t width,
+                           const int32_t* free_ids, int32_t free_cap, const int32_t* n_free, int32_t* row_off, int32_t* lens_out, int32_t* slots, int32_t* run_row,
+                           int32_t* run_len, int32_t* state, void* ws, uint64_t ws_bytes, void* stream) {
+  DMT_CHECK_ARG(n >= 0 && rows >= 0 && width >= 0 && rows <= 0x3fffffff, "dmt_kv_plan: n %d, rows %d (at most 2^30), width %d", n, rows, width);
+  DMT_CHECK_ARG(n_free && row_off && state && free_cap >= 0, "dmt_kv_plan: NULL n_free / row_off / state");
+  DMT_CHECK_ARG(n == 0 || (lens && new_lens && lens_out && table && free_ids), "dmt_kv_plan: NULL lens / new_lens / lens_out / table / free_ids");
+  DMT_CHECK_ARG(rows == 0 || (slots && run_row && run_len), "dmt_kv_plan: NULL slots / run_row / run_len");
+  DMT_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= dmt_kv_plan_ws_bytes(n), "dmt_kv_plan: workspace of %llu bytes needed",
+                (unsigned long long)dmt_kv_plan_ws_bytes(n));
+  PlanArgs a;
+  a.n = n; a.rows = rows; a.width = width;
+  const long long mr = (long long)rows / BS + 2ll * n;
+  a.max_runs = (int)(mr < rows ? mr : rows);
+  a.lens = lens; a.new_lens = new_lens; a.table = table; a.free_ids = free_ids; a.free_cap = free_cap; a.n_free = n_free;
+  a.row_off = row_off; a.lens_out = lens_out; a.slots = slots; a.run_row = run_row; a.run_len = run_len; a.state = state;
+  a.totals = (int*)ws;
+  a.req = (int2*)((char*)ws + 16);
+  const int small = rows <= PLAN_SMALL_ROWS;
+  plan_kernel<<<1, PLAN_NT, 0, (hipStream_t)stream>>>(a, small);
+  DMT_CHECK_LAUNCH("dmt_kv_plan");
+  if (!small) {
+    plan_rows_kernel<<<(unsigned)cdiv64(rows, 256), 256, 0, (hipStream_t)stream>>>(a);
+    DMT_CHECK_LAUNCH("dmt_kv_plan(rows)");
+  }
+  return DMT_OK;
+}
+
+extern "C" int dmt_kv_release(int32_t n, const int32_t* done, int32_t* lens, const int32_t* table, int32_t width, int32_t* free_ids, int32_t* n_free,
+                              int32_t cap, void* stream) {
+  DMT_CHECK_ARG(n >= 0 && width >= 0 && cap >= 0, "dmt_kv_release: negative size");
+  if (n == 0) return DMT_OK;
+  DMT_CHECK_ARG(done && lens && table && free_ids && n_free, "dmt_kv_release: NULL pointer");
+  release_kernel<<<1, PLAN_NT, 0, (hipStream_t)stream>>>(n, done, lens, table, width, free_ids, n_free, cap);
+  DMT_CHECK_LAUNCH("dmt_kv_release");
+  return DMT_OK;
+}
+
+extern "C" int dmt_kv_append(int32_t Hkv, int32_t dh, int32_t n_blocks, uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int32_t rows,
+                             const void* k_rows, int64_t k_rs, const void* v_rows, int64_t v_rs, const int32_t* slots, const int32_t* run_row,
+                             const int32_t* run_len, int32_t max_runs, void* stream) {
+  DMT_CHECK_ARG(cache_ok(Hkv, dh, n_blocks, k, v, k_scale, v_scale), CACHE_MSG, "dmt_kv_append", Hkv, dh, n_blocks);
+  DMT_CHECK_ARG(rows >= 0 && max_runs >= 0, "dmt_kv_append: negative size");
+  if (rows == 0 || max_runs == 0) return DMT_OK;
+  DMT_CHECK_ARG(k_rows && v_rows && slots && run_row && run_len, "dmt_kv_append: NULL rows / slots / runs");
+  DMT_CHECK_ARG(k_rs >= (int64_t)Hkv * dh && v_rs >= (int64_t)Hkv * dh && k_rs % 8 == 0 && v_rs % 8 == 0 && (uintptr_t)k_rows % 16 == 0 &&
+                    (uintptr_t)v_rows % 16 == 0, "dmt_kv_append: rows of at least Hkv * dh, 16-byte aligned");
+  const Cache c = {Hkv, dh, n_blocks, k, v, k_scale, v_scale};
+  append_kernel<<<dim3(max_runs, Hkv), 256, 0, (hipStream_t)stream>>>(c, rows, (const bf16_t*)k_rows, k_rs, (const bf16_t*)v_rows, v_rs, slots, run_row,
+                                                                      run_len);
+  DMT_CHECK_LAUNCH("dmt_kv_append");
+  return DMT_OK;
+}
+
+extern "C" int dmt_kv_read(int32_t Hkv, int32_t dh, int32_t n_blocks, const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
+                           int32_t n, const int32_t* slots, void* k_rows, int64_t k_rs, void* v_rows, int64_t v_rs, void* stream) {
+  DMT_CHECK_ARG(cache_ok(Hkv, dh, n_blocks, k, v, k_scale, v_scale), CACHE_MSG, "dmt_kv_read", Hkv, dh, n_blocks);
+  DMT_CHECK_ARG(n >= 0, "dmt_kv_read: negative size");
+  if (n == 0) return DMT_OK;
+  DMT_CHECK_ARG(k_rows && v_rows && slots, "dmt_kv_read: NULL rows / slots");
+  DMT_CHECK_ARG(k_rs >= (int64_t)Hkv * dh && v_rs >= (int64_t)Hkv * dh && k_rs % 8 == 0 && v_rs % 8 == 0 && (uintptr_t)k_rows % 16 == 0 &&
+                    (uintptr_t)v_rows % 16 == 0, "dmt_kv_read: rows of at least Hkv * dh, 16-byte aligned");
+  const Cache c = {Hkv, dh, n_blocks, (uint8_t*)k, (uint8_t*)v, (float*)k_scale, (float*)v_scale};
+  read_kernel<<<dim3((unsigned)cdiv64(n, 64), Hkv), 256, 0, (hipStream_t)stream>>>(c, n, slots, (bf16_t*)k_rows, k_rs, (bf16_t*)v_rows, v_rs);
+  DMT_CHECK_LAUNCH("dmt_kv_read");
+  return DMT_OK;
+}
+
+extern "C" uint64_t dmt_kv_attn_ws_bytes(const dmt_kv_attn_desc* d) {
+  (void)d;
+  return 0;
+}
+
+extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
+  DMT_CHECK_ARG(d, "dmt_kv_attn: no descriptor");
+  DMT_CHECK_ARG(cache_ok(d->Hkv, d->dh, d->n_blocks, d->k, d->v, d->k_scale, d->v_scale), CACHE_MSG, "dmt_kv_attn", d->Hkv, d->dh, d->n_blocks);
+  DMT_CHECK_ARG(d->Hq > 0 && d->Hq <= 65535 && d->Hq % d->Hkv == 0, "dmt_kv_attn: Hq %d is not a multiple of Hkv %d", d->Hq, d->Hkv);
+  DMT_CHECK_ARG(d->n >= 0 && d->n <= 65535 && d->max_q >= 0 && d->max_len >= 0 && d->width >= 0 && d->rows >= 0 && d->rows < (1ll << 31),
+                "dmt_kv_attn: n %d (at most 65535), max_q %d, max_len %d, width %d", d->n, d->max_q, d->max_len, d->width);
+  DMT_CHECK_ARG(d->scale > 0.f && d->scale < 3.4e38f && d->cap >= 0.f && d->cap < 3.4e38f, "dmt_kv_attn: scale must be positive, cap 0 or positive");
+  if (d->n == 0 || d->max_q == 0 || d->rows == 0) return DMT_OK;
+  DMT_CHECK_ARG(d->Q && d->out && d->lens && d->row_off && (d->table || d->width == 0), "dmt_kv_attn: NULL pointer");
+  const int64_t wq = (int64_t)d->Hq * d->dh;
+  DMT_CHECK_ARG(d->q_rs >= wq && d->o_rs >= wq && d->q_rs % 8 == 0 && d->o_rs % 8 == 0 && (uintptr_t)d->Q % 16 == 0 && (uintptr_t)d->out % 16 == 0,
+                "dmt_kv_attn: rows of at least Hq * dh, 16-byte aligned");
+  KvArgs a;
+  a.c = {d->Hkv, d->dh, d->n_blocks, (uint8_t*)d->k, (uint8_t*)d->v, (float*)d->k_scale, (float*)d->v_scale};
+  a.n = d->n; a.Hq = d->Hq; a.G = d->Hq / d->Hkv; a.max_q = d->max_q; a.max_len = d->max_len; a.width = d->width; a.causal = d->causal != 0;
+  a.rows = d->rows; a.Q = (const bf16_t*)d->Q; a.q_rs = d->q_rs; a.table = d->table; a.lens = d->lens; a.row_off = d->row_off;
+  a.scale = d->scale; a.cap = d->cap; a.slopes = d->slopes; a.out = (bf16_t*)d->out; a.o_rs = d->o_rs; a.lse = d->lse;
+  kv_rows_kernel<<<dim3((unsigned)cdiv64(a.max_q, 4), a.Hq, a.n), 256, 0, (hipStream_t)stream>>>(a);
+  DMT_CHECK_LAUNCH("dmt_kv_attn(rows)");
+  return DMT_OK;
+}

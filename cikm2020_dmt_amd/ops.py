@@ -11,6 +11,7 @@ import os
 import ctypes as _ct
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -1176,6 +1177,197 @@ class AttnFn(torch.autograd.Function):
         attn_core_bwd(q, k, v, q_lens, k_lens, ctx.P, dout, dq, dk, dv, H, *ctx.drop, causal=ctx.causal)
         ctx.P = None
         return dpq, dpkv, (dout if ctx.has_resid else None), None, None, None, None, None, None, None, None, None
+
+
+# ---- attention over packed rows of any length: shared heads, capped scores, distance bias, causal / prefix / document masks
+def _host_ints(x, what):
+    t = x.detach().cpu().numpy() if isinstance(x, torch.Tensor) else np.asarray(x, dtype=None if len(x) else np.int64)
+    if t.ndim != 1 or t.dtype.kind not in "iu":
+        raise ValueError("%s must be a 1-D list, array or tensor of integers" % what)
+    return t.astype(np.int64)
+
+
+class AttnSeqs:
+    """Where the examples of attn_var lie: example b has q_lens[b] query rows from row q_off[b] on and k_lens[b] key rows from k_off[b] on
+    (offsets default to the exclusive sums of the lengths: rows side by side; k_* default to q_*: self-attention).  A dense [B, T] batch is
+    q_off = b * T.  Lengths may be lists, arrays or tensors; they are checked HERE, once (a device tensor is read back: build the object
+    with the batch, outside of a graph capture).  Rows of no example get zeros in what attn_var returns.
+    max_q / max_k: bounds of the lengths (default: the largest).  A captured graph that is replayed with other lengths copies them into
+    .q_lens / .q_off / ... in place; the bounds and `zero_fill` (pass True) must then hold for every replay."""
+
+    def __init__(self, q_lens, k_lens=None, q_off=None, k_off=None, max_q=None, max_k=None, device=None, zero_fill=None):
+        if device is None:
+            device = next((t.device for t in (q_lens, k_lens) if isinstance(t, torch.Tensor) and t.is_cuda), torch.device("cuda"))
+        self.zero_fill = zero_fill
+        ql = _host_ints(q_lens, "q_lens")
+        qo = (np.cumsum(ql) - ql) if q_off is None else _host_ints(q_off, "q_off")
+        self.self_attention = k_lens is None
+        if k_lens is None:
+            if k_off is not None:
+                raise ValueError("k_off without k_lens")
+            kl, ko = ql, qo
+        else:
+            kl = _host_ints(k_lens, "k_lens")
+            ko = (np.cumsum(kl) - kl) if k_off is None else _host_ints(k_off, "k_off")
+        self.B = len(ql)
+        if not len(ql) == len(qo) == len(kl) == len(ko):
+            raise ValueError("one length and offset for each example: got %d, %d, %d, %d" % (len(ql), len(qo), len(kl), len(ko)))
+        for x, what in ((ql, "q_lens"), (qo, "q_off"), (kl, "k_lens"), (ko, "k_off")):
+            if len(x) and (x.min() < 0 or x.max() > 0x7FFFFFFF):
+                raise ValueError("%s must lie in 0 .. 2^31 - 1" % what)
+        self.end_q, self.total_q, over_q = self._extent(qo, ql)
+        self.end_k, self.total_k, self.k_shared = self._extent(ko, kl)
+        if over_q:
+            raise ValueError("two examples share query rows")
+        top = lambda x: int(x.max()) if len(x) else 0  # noqa: E731
+        self.max_q, self.max_k = top(ql) if max_q is None else int(max_q), top(kl) if max_k is None else int(max_k)
+        if self.max_q < top(ql) or self.max_k < top(kl):
+            raise ValueError("a length passes max_q %d / max_k %d" % (self.max_q, self.max_k))
+        dev = lambda x, given: (given.to(device=device, dtype=torch.int32).contiguous() if isinstance(given, torch.Tensor)  # noqa: E731
+                                else torch.as_tensor(x.astype(np.int32)).to(device))
+        self.q_lens, self.q_off = dev(ql, q_lens), dev(qo, q_off)
+        self.k_lens, self.k_off = (self.q_lens, self.q_off) if k_lens is None else (dev(kl, k_lens), dev(ko, k_off))
+
+    @staticmethod
+    def _extent(off, lens):
+        """(end of the last row, rows held, whether two examples share a row)"""
+        some = lens > 0
+        o, n = off[some], lens[some]
+        if not len(o):
+            return 0, 0, False
+        order = np.argsort(o, kind="stable")
+        o, n = o[order], n[order]
+        return int((o + n).max()), int(n.sum()), bool((o[:-1] + n[:-1] > o[1:]).any())
+
+
+def _rows2(t, what, heads, dtype):
+    if t.dim() != 2 or t.dtype != dtype or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("%s must be a 2-D view of %s with unit inner stride, got %s %s strides %s" % (what, dtype, t.dtype, tuple(t.shape), t.stride()))
+    if t.shape[1] % heads:
+        raise ValueError("%s: %d columns are not a whole number for each of %d heads" % (what, t.shape[1], heads))
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _aligned_rows(t):
+    """t itself when its rows are 16-byte aligned with unit inner stride, else a copy that is"""
+    es = t.element_size()
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) * es % 16 == 0 and t.stride(0) >= t.shape[1])):
+        return t
+    return t.contiguous()
+
+
+def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, lens, out, lse, cfg):
+    H, Hkv, scale, cap, causal, max_q, max_k = cfg
+    d = L.AttnVarDesc()
+    d.dtype, d.B, d.Hq, d.Hkv, d.dh, d.max_q, d.max_k = dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k
+    d.rows_q, d.rows_k = q.shape[0], k.shape[0]
+    d.Q, d.q_rs = q.data_ptr(), _rows2(q, "q", H, q.dtype)
+    d.K, d.k_rs = k.data_ptr(), _rows2(k, "k", Hkv, q.dtype)
+    d.V, d.v_rs = v.data_ptr(), _rows2(v, "v", Hkv, q.dtype)
+    d.q_lens, d.q_off, d.k_lens, d.k_off = (x.data_ptr() for x in lens)
+    d.scale, d.cap, d.causal = scale, cap, 1 if causal else 0
+    d.slopes, d.prefix, d.q_doc, d.k_doc = (x.data_ptr() if x is not None else None for x in (slopes, prefix, q_doc, k_doc))
+    d.out, d.o_rs, d.lse = out.data_ptr(), out.shape[1], p(lse)
+    return d
+
+
+def _var_ws(d, backward, device):
+    need = int(L.load().dmt_attn_var_ws_bytes(C.byref(d), backward))
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    d.ws, d.ws_bytes = p(ws), need
+    return ws
+
+
+class AttnVarFn(torch.autograd.Function):
+    """(out, lse) of dmt_attn_var_fwd; gradients of q, k, v and the slopes by dmt_attn_var_bwd (workspaces come from torch's allocator in
+    every call: two captured graphs never share one)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, prefix, q_doc, k_doc, q_lens, q_off, k_lens, k_off, cfg, fill, k_shared):
+        H, Hkv = cfg[:2]
+        rows, d = q.shape
+        new = torch.zeros if fill[0] else torch.empty
+        out = new((rows, d), dtype=q.dtype, device=q.device)
+        lse = torch.full((rows, H), -float("inf"), device=q.device) if fill[0] else torch.empty((rows, H), dtype=F32, device=q.device)
+        need_sl = slopes is not None and ctx.needs_input_grad[3]
+        lens = (q_lens, q_off, k_lens, k_off)
+        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, lens, out, lse, cfg)
+        ws = _var_ws(desc, 0, q.device)
+        L.call("dmt_attn_var_fwd", C.byref(desc), stream_ptr())
+        del ws
+        ctx.save_for_backward(q, k, v, slopes, prefix, q_doc, k_doc, *lens, out, lse)
+        ctx.cfg, ctx.fill, ctx.need_sl, ctx.k_shared = cfg, fill, need_sl, k_shared
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, dout, _dlse):
+        q, k, v, slopes, prefix, q_doc, k_doc, q_lens, q_off, k_lens, k_off, out, lse = ctx.saved_tensors
+        if dout is None:
+            return (None,) * 14
+        if ctx.k_shared:
+            raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
+        dout = _aligned_rows(dout)
+        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, (q_lens, q_off, k_lens, k_off), out, lse, ctx.cfg)
+        nq, nk = (torch.zeros if f else torch.empty for f in ctx.fill)
+        dq = nq(q.shape, dtype=q.dtype, device=q.device)
+        dk, dv = nk(k.shape, dtype=k.dtype, device=k.device), nk(v.shape, dtype=v.dtype, device=v.device)
+        dsl = torch.zeros_like(slopes) if ctx.need_sl else None
+        desc.dout, desc.do_rs = dout.data_ptr(), dout.stride(0) if dout.shape[0] > 1 else dout.shape[1]
+        desc.dQ, desc.dq_rs, desc.dK, desc.dk_rs, desc.dV, desc.dv_rs = (dq.data_ptr(), dq.shape[1], dk.data_ptr(), dk.shape[1], dv.data_ptr(),
+                                                                         dv.shape[1])
+        desc.dslopes = p(dsl)
+        ws = _var_ws(desc, 1, q.device)
+        L.call("dmt_attn_var_bwd", C.byref(desc), stream_ptr())
+        del ws
+        return (dq, dk, dv, dsl) + (None,) * 10
+
+
+def _ids(t, n, what, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous int32 tensor [%d] on %s" % (what, n, device))
+    return t
+
+
+def attn_var(q, k, v, seqs: AttnSeqs, H, Hkv=None, *, scale=None, cap=0.0, slopes=None, causal=False, prefix=None, docs=None, want_lse=False):
+    """Attention over packed rows q [Rq, H * dh], k, v [Rk, Hkv * dh] (bf16 or fp32), forward and backward, histories of any length:
+        z_ij = y_ij - slopes[h] |i + Lk - Lq - j|,   y = cap tanh(x / cap) (cap > 0),   x_ij = scale q_i . k_j   (scale: 1 / sqrt(dh))
+        query i sees key j of its own example if  j < prefix[b]  or  ((not causal or j <= i + Lk - Lq) and docs agree)
+    slopes: fp32 [H] (gets a gradient), prefix: int32 [B], docs: (int32 [Rq], int32 [Rk]) document ids.  want_lse: (out, lse [Rq, H]) --
+    lse is not differentiable.  A row that sees nothing is zero, its lse -inf.  Unaligned operands are copied once."""
+    require_cuda(q, k, v, slopes)
+    Hkv = H if Hkv is None else Hkv
+    if H <= 0 or Hkv <= 0 or H % Hkv:
+        raise ValueError("H = %d query heads cannot share Hkv = %d key heads evenly" % (H, Hkv))
+    for t, what, h in ((q, "q", H), (k, "k", Hkv), (v, "v", Hkv)):
+        _rows2(t, what, h, q.dtype)
+        if t.device != q.device:
+            raise ValueError("attn_var: operands on different devices")
+    dh = q.shape[1] // H
+    if k.shape != v.shape or k.shape[1] != Hkv * dh:
+        raise ValueError("k and v must be [Rk, %d], got %s and %s" % (Hkv * dh, tuple(k.shape), tuple(v.shape)))
+    if not L.load().dmt_attn_var_supported(dt_code(q.dtype), dh, H, Hkv):
+        raise ValueError("attn_var takes bf16 with dh %% 8 == 0 or fp32 with dh %% 4 == 0, dh <= 128: got %s, dh = %d" % (q.dtype, dh))
+    if seqs.end_q > q.shape[0] or seqs.end_k > k.shape[0]:
+        raise ValueError("the examples' rows end at %d / %d, the operands have %d / %d" % (seqs.end_q, seqs.end_k, q.shape[0], k.shape[0]))
+    if seqs.q_lens.device != q.device:
+        raise ValueError("attn_var: the examples' lengths are on %s, the operands on %s" % (seqs.q_lens.device, q.device))
+    if slopes is not None and (slopes.dtype != F32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous() or slopes.device != q.device):
+        raise ValueError("slopes must be a contiguous fp32 tensor [%d] on %s" % (H, q.device))
+    scale = 1.0 / float(dh) ** 0.5 if scale is None else float(scale)
+    if not (0.0 < scale < 3e38) or not (0.0 <= cap < 3e38):
+        raise ValueError("scale must be positive and finite, cap 0 or positive and finite: got %r, %r" % (scale, cap))
+    prefix = _ids(prefix, seqs.B, "prefix", q.device)
+    q_doc, k_doc = (None, None) if docs is None else (_ids(docs[0], q.shape[0], "docs[0]", q.device), _ids(docs[1], k.shape[0], "docs[1]", q.device))
+    fill = (seqs.zero_fill, seqs.zero_fill) if seqs.zero_fill is not None else (seqs.total_q != q.shape[0], seqs.total_k != k.shape[0] or seqs.k_shared)
+    cfg = (H, Hkv, scale, float(cap), bool(causal), seqs.max_q, seqs.max_k)
+    with torch.cuda.device(q.device):
+        out, lse = AttnVarFn.apply(_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), slopes, prefix, q_doc, k_doc, seqs.q_lens, seqs.q_off,
+                                   seqs.k_lens, seqs.k_off, cfg, fill, seqs.k_shared)
+    return (out, lse) if want_lse else out
 
 
 def q1mem_supported(d, H, T, dtype=BF16):

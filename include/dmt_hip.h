@@ -47,6 +47,7 @@ extern "C" {
  *   seq_row_len), dmt_attn_desc (row_off, ex_list, n_list), dmt_mhsa_desc (packed-row fields), dmt_q1mem_desc (row_off); dmt_colsum_rows_packed added.
  *   6  round 6: dmt_mhsa_block_bwd + dmt_mhsa_bwd_image_* added; dmt_sort_pairs / dmt_segment_heads are the library's own kernels (vals_in may be NULL; 16-byte aligned workspace; the
  *   workspace sizes changed), dmt_embgrad_keys takes vals == NULL.
+ *   7  dmt_attn_var_* (attention over packed rows of any length with shaped scores and masks) and dmt_kv_* (8-bit K / V cache) added.
  *
  * PACKED ROWS.  A behaviour sequence of a batch may be stored WITHOUT its padding: example b's rows t = 0 .. len[b] - 1 are rows
  * row_off[b] + t of an [R, d] matrix, R = sum_b len[b] (row_off: int32 [B], any order of the examples -- the engine groups examples of
@@ -54,14 +55,14 @@ extern "C" {
  * know about examples take row_off (NULL = the dense [B, T, d] layout, row b * T + t).  Rows t >= len[b] do not exist: in the dense
  * layout they hold finite values nothing reads (the reference masks them as keys, and their gradients are zero), so the
  * two layouts agree on every row that exists.  Dropout counters keep the DENSE element index, so a packed and a dense run draw the same mask. */
-#define DMT_ABI_VERSION 6
+#define DMT_ABI_VERSION 7
 const char* dmt_last_error(void);
 int dmt_version(void);
 /* gfx arch string the device code was built for ("gfx950"). */
 const char* dmt_build_arch(void);
 /* sizeof() of the ABI structs: 0 gather_feature, 1 gather_desc, 2 embgrad_desc, 3 gemm_desc, 4 attn_desc,
  * 5 attn_bwd_desc, 6 table_map, 7 cast_job, 8 chain_desc, 9 wgrad_desc, 10 mhsa_desc, 11 mmoe_desc, 12 heads_desc, 13 q1mem_desc,
- * 14 mhsa_bwd_desc (lets a binding verify its struct layout). */
+ * 14 mhsa_bwd_desc, 15 attn_var_desc, 16 kv_attn_desc (lets a binding verify its struct layout). */
 int dmt_struct_size(int which);
 /* Launch-route trace (diagnostic, off by default).  dmt_route_trace(1) clears the counters and starts counting every successful launch
  * under its route label (the name of the kernel variant an entry point dispatched to, e.g. "dmt_attn_fwd(mfma, coalesced)",
@@ -809,6 +810,113 @@ typedef struct {
 int dmt_q1mem_supported(int32_t dtype, int32_t d, int32_t H, int32_t T);
 int dmt_q1mem_fwd(const dmt_q1mem_desc* d, void* stream);
 int dmt_q1mem_bwd(const dmt_q1mem_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * revision 7.  Multi-head attention over packed rows of ANY length, with shared key / value heads, shaped scores and masks
+ * (forward and backward; no [B, H, T, T] tensor reaches memory).  Example b has q_lens[b] query rows q_off[b] + i of Q / out and
+ * k_lens[b] key rows k_off[b] + j of K / V; query head h reads key / value head h / (Hq / Hkv); off_b = k_lens[b] - q_lens[b].
+ *     x_ij = scale q_i . k_j       y_ij = cap > 0 ? cap tanh(x_ij / cap) : x_ij       z_ij = y_ij - slopes[h] |i + off_b - j|
+ *     allowed(i, j) = j < k_lens[b] and (j < prefix[b]  or  ((not causal or j <= i + off_b) and (no documents or q_doc[i] == k_doc[j])))
+ *     out_i = sum_j softmax_j(z_ij over the allowed j) v_j        lse[i, h] = log sum_j exp z_ij  (natural log)
+ * A row that may see nothing gets out = 0, lse = -inf and no gradient.  What stands in a masked place -- NaN and infinities too -- does
+ * not reach a row that may not see it.  Rows that belong to no example are neither read nor written.
+ * Types: DMT_BF16 (dh a multiple of 8) and DMT_F32 (dh a multiple of 4), dh <= 128; sums, softmax statistics and gradients in fp32.
+ * Every operand row 16-byte aligned (base and row stride).  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
+ * caller's promise: it sizes the grid; longer examples are cut there).
+ * Backward: dq, dk, dv for the rows of every example, and dslopes [Hq] (accumulated in a fixed order, then ADDED to what dslopes holds).
+ * Bit-reproducible: no atomics.  ws: dmt_attn_var_ws_bytes(...) bytes, 16-byte aligned, no initialisation needed; one call at a time.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct {
+  int32_t dtype;
+  int32_t B, Hq, Hkv, dh;
+  int32_t max_q, max_k;
+  int64_t rows_q, rows_k;                  /* rows of Q / K: examples that name rows past them are cut there */
+  const void* Q; int64_t q_rs;             /* Q[row * q_rs + h * dh + j], elements                     */
+  const void* K; int64_t k_rs;
+  const void* V; int64_t v_rs;
+  const int32_t* q_off; const int32_t* q_lens;
+  const int32_t* k_off; const int32_t* k_lens;
+  float scale;                             /* > 0                                                      */
+  float cap;                               /* 0: none                                                  */
+  int32_t causal;
+  const float* slopes;                     /* [Hq] or NULL                                             */
+  const int32_t* prefix;                   /* [B] or NULL                                              */
+  const int32_t* q_doc; const int32_t* k_doc;   /* one id for each row of Q / K, or both NULL          */
+  void* out; int64_t o_rs;
+  float* lse;                              /* [rows_q, Hq] or NULL (forward); required in the backward */
+  const void* dout; int64_t do_rs;         /* backward from here on (out, lse: the forward's) */
+  void* dQ; int64_t dq_rs;
+  void* dK; int64_t dk_rs;
+  void* dV; int64_t dv_rs;
+  float* dslopes;                          /* [Hq] or NULL; needs slopes                               */
+  void* ws; uint64_t ws_bytes;             /* documents (both directions) and the backward             */
+} dmt_attn_var_desc;
+uint64_t dmt_attn_var_ws_bytes(const dmt_attn_var_desc* d, int32_t backward);
+int dmt_attn_var_supported(int32_t dtype, int32_t dh, int32_t Hq, int32_t Hkv);
+int dmt_attn_var_fwd(const dmt_attn_var_desc* d, void* stream);
+int dmt_attn_var_bwd(const dmt_attn_var_desc* d, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * revision 7.  K / V cache in 8 bits for served histories.  Memory is a pool of blocks of DMT_KV_BLOCK tokens; block p holds, for every
+ * key / value head, OCP e4m3 bytes and ONE scale for K and one for V (a power of two: e4m3 is a floating type, so the power loses no
+ * precision, the value byte * scale is exact in bf16, and a scale that grows re-rounds only what falls to the subnormals):
+ *     k [n_blocks, Hkv, 64 tokens, dh]        v [n_blocks, Hkv, dh, 64 places]  (token 16 a + 4 b + r of the block at place 16 b + 4 a + r:
+ *     a lane of the attention kernel then finds its 16 tokens of one dim in one 16-byte load)        k_scale, v_scale fp32 [n_blocks, Hkv]
+ * slot = block * 64 + token; position t of request r is in block table[r, t / 64].  dh a multiple of 16, <= 128.
+ * ------------------------------------------------------------------------------------------------ */
+#define DMT_KV_BLOCK 64
+/* Block tables and slots from request lengths, on the device.  Request r has lens[r] tokens and gets new_lens[r] more, whose rows are
+ * row_off[r] .. of the step's row matrices (row_off: exclusive sums of new_lens, [n + 1], cut at
+ * 2^31 - 1).  Blocks come from the stack free_ids[0 .. n_free):
+ * the last entry first, requests in order.  A request is refused (lens_out = lens, its slots -1) when new_lens < 0 (counted as 0 rows), when
+ * lens + new would pass the table's width or its rows would pass `rows`, or when the requests up to and including it need more blocks than
+ * are free.  Out: row_off, lens_out [n], table (the new blocks' entries), slots [rows] (-1: not stored), runs: run w = rows run_row[w] ..
+ * + run_len[w] of one request in one block, in row order, then (-1, 0) up to max_runs = min(rows, rows / 64 + 2 n); free_cap: entries of
+ * free_ids (n_free is cut there); state = {blocks left
+ * free, requests refused}.  free_ids and n_free are read only: the caller keeps state[0] for its next step.
+ * ws: dmt_kv_plan_ws_bytes(n) bytes, 16-byte aligned. */
+uint64_t dmt_kv_plan_ws_bytes(int32_t n);
+int dmt_kv_plan(int32_t n, int32_t rows, const int32_t* lens, const int32_t* new_lens, int32_t* table, int32_t width,
+                const int32_t* free_ids, int32_t free_cap, const int32_t* n_free, int32_t* row_off, int32_t* lens_out, int32_t* slots,
+                int32_t* run_row, int32_t* run_len, int32_t* state, void* ws, uint64_t ws_bytes, void* stream);
+/* Requests with done[r] != 0 give their blocks back: pushed on free_ids in request and position order from n_free[0], lens[r] = 0, and
+ * n_free[0] counts them.  cap: entries of free_ids (blocks past it are dropped: a table that holds a block twice). */
+int dmt_kv_release(int32_t n, const int32_t* done, int32_t* lens, const int32_t* table, int32_t width, int32_t* free_ids, int32_t* n_free,
+                   int32_t cap, void* stream);
+/* The rows of a step into their slots (bf16 rows [rows, Hkv * dh], row strides k_rs / v_rs): one workgroup owns a (run, head).  The scale of
+ * a block is the least power of two s >= 2^-100 with max |x| <= 448 s over its new rows (finite values only), and not under the one it had
+ * when it holds older tokens of the same request (positions before the run's first); a scale that grows re-rounds those.  Infinities are
+ * stored as +-448 s, NaN as NaN.  Runs as dmt_kv_plan leaves them; run_row < 0 or a slot outside the pool: skipped. */
+int dmt_kv_append(int32_t Hkv, int32_t dh, int32_t n_blocks, uint8_t* k, uint8_t* v, float* k_scale, float* v_scale, int32_t rows,
+                  const void* k_rows, int64_t k_rs, const void* v_rows, int64_t v_rs, const int32_t* slots, const int32_t* run_row,
+                  const int32_t* run_len, int32_t max_runs, void* stream);
+/* Values of n slots as bf16 rows [n, Hkv * dh] (exact: no rounding); a slot outside the pool gives zeros. */
+int dmt_kv_read(int32_t Hkv, int32_t dh, int32_t n_blocks, const uint8_t* k, const uint8_t* v, const float* k_scale, const float* v_scale,
+                int32_t n, const int32_t* slots, void* k_rows, int64_t k_rs, void* v_rows, int64_t v_rs, void* stream);
+/* Attention of n requests' query rows over their cached tokens; scores as dmt_attn_var_fwd.  Request r: query rows row_off[r] .. row_off[r + 1]
+ * (at most max_q of them are computed), lens[r] cached tokens.  causal: row i of m stands at position lens - m + i and sees the tokens up
+ * to itself (the step's own tokens were appended before); otherwise every row stands at position lens and sees them all.  Distance of the
+ * slopes: |position - j|.  A row that sees nothing gets 0 and lse -inf.  max_len bounds the lengths (a promise that sizes the grid and the
+ * split over the length; longer requests are cut there; lens past the table's width too).  Table entries outside the pool: masked.
+ * One wavefront takes 64 tokens at a time; the length is split over workgroups by a rule on (n, Hkv, max_q, max_len) alone, and the pieces
+ * are joined in their order: bit-reproducible.  ws: dmt_kv_attn_ws_bytes(d), 16-byte aligned, one call at a time. */
+typedef struct {
+  int32_t n, Hq, Hkv, dh, n_blocks;
+  int32_t max_q, max_len, width;
+  int64_t rows;                              /* rows of Q / out */
+  const uint8_t* k; const uint8_t* v;
+  const float* k_scale; const float* v_scale;
+  const void* Q; int64_t q_rs;               /* bf16 [rows, Hq * dh] */
+  const int32_t* table; const int32_t* lens; const int32_t* row_off;
+  float scale, cap;
+  int32_t causal;
+  const float* slopes;
+  void* out; int64_t o_rs;
+  float* lse;                                /* [rows, Hq] or NULL */
+  void* ws; uint64_t ws_bytes;
+} dmt_kv_attn_desc;
+uint64_t dmt_kv_attn_ws_bytes(const dmt_kv_attn_desc* d);
+int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,274 @@
+"""Attention over packed rows (ops.attn_var) against its definition in 64 bits, forward and gradients, at the sizes and masks where it can
+go wrong; bounds derived in attn_ref."""
+import numpy as np
+import pytest
+import torch
+
+from cikm2020_dmt_amd import _lib as L
+from cikm2020_dmt_amd import ops
+from tests import attn_ref as A
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _make(ql, kl, H, Hkv, dh, dtype, seed, std=1.0, gap=0):
+    g = torch.Generator().manual_seed(seed)
+    qo = np.concatenate([[0], np.cumsum(np.array(ql) + gap)])[:-1].tolist()
+    ko = np.concatenate([[0], np.cumsum(np.array(kl) + gap)])[:-1].tolist()
+    rq, rk = int(sum(ql) + gap * len(ql)), int(sum(kl) + gap * len(kl))
+    n = lambda r, w, s=1.0: (torch.randn((r, w), generator=g) * s).to(dtype)  # noqa: E731
+    return n(rq, H * dh, std), n(rk, Hkv * dh, std), n(rk, Hkv * dh), n(rq, H * dh), qo, ko
+
+
+def _check(cuda, ql, kl, H, Hkv, dh, dtype=BF, seed=0, std=1.0, gap=0, slopes=None, docs=None, prefix=None, train=True, **kw):
+    q, k, v, do, qo, ko = _make(ql, kl, H, Hkv, dh, dtype, seed, std, gap)
+    sl = None if slopes is None else torch.tensor(slopes, dtype=F32)
+    ref = A.attn_var(q, k, v, H, Hkv, ql, kl, qo, ko, slopes=sl, docs=docs, prefix=prefix, dout=do if train else None, **kw)
+    seqs = ops.AttnSeqs(ql, kl, qo, ko, device=cuda)
+    lv = [t.to(cuda).requires_grad_(train) for t in (q, k, v)] + ([sl.to(cuda).requires_grad_(train)] if sl is not None else [])
+    i32 = lambda t: torch.as_tensor(t, dtype=torch.int32).to(cuda)  # noqa: E731
+    out, lse = ops.attn_var(*lv[:3], seqs, H, Hkv, slopes=lv[3] if sl is not None else None, want_lse=True,
+                            docs=None if docs is None else tuple(map(i32, docs)), prefix=None if prefix is None else i32(prefix), **kw)
+    A.close(out, ref["out"], ref["out_tol"], "out")
+    A.close(lse, ref["lse"], ref["lse_tol"], "lse")
+    if not train:
+        return
+    grads = torch.autograd.grad(out, lv, do.to(cuda))
+    for t, n in zip(grads, ("dq", "dk", "dv", "dslope")):
+        A.close(t, ref[n], ref[n + "_tol"], n)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("dh", [16, 24, 40, 64, 80, 96, 128])
+def test_head_sizes(cuda, dh, dtype):
+    _check(cuda, [70, 1, 33], [70, 1, 33], 4, 2, dh, dtype, causal=True)
+    _check(cuda, [5, 130], [67, 129], 2, 1, dh, dtype, slopes=[0.3, 0.02])
+
+
+@pytest.mark.parametrize("dh", [4, 20, 100])
+def test_head_sizes_of_fp32(cuda, dh):
+    _check(cuda, [70, 1, 33], [70, 1, 33], 4, 4, dh, F32, causal=True, cap=3.0)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("ql,kl", [([1], [1]), ([1], [2]), ([2], [1]), ([31, 32, 33], [31, 32, 33]), ([63, 64, 65], [63, 64, 65]),
+                                   ([127, 128, 129], [127, 128, 129]), ([1, 1, 3], [200, 64, 65]), ([200, 65], [7, 64]), ([0, 5, 0], [9, 0, 0]),
+                                   ([0, 5, 4], [0, 5, 4]), ([257, 300], [257, 511])])
+def test_lengths(cuda, ql, kl, causal):
+    _check(cuda, ql, kl, 2, 2, 32, causal=causal)
+
+
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (3, 1), (8, 1), (8, 2), (6, 3), (16, 16)])
+def test_shared_heads(cuda, H, Hkv):
+    _check(cuda, [40, 77], [90, 77], H, Hkv, 32, causal=True, slopes=[0.5 / (h + 1) for h in range(H)])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("kw", [dict(cap=5.0), dict(cap=5.0, causal=True, slopes=[0.1, 0.0, 1.0, 0.01]), dict(slopes=[0.0, 2.0, -0.01, 0.3]),
+                                dict(cap=0.01), dict(scale=0.5), dict(cap=30.0, scale=2.0, causal=True)])
+def test_shaped_scores(cuda, kw, dtype):
+    _check(cuda, [100, 37], [100, 90], 4, 2, 64, dtype, std=1.5, **kw)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("prefix", [[0, 0, 0], [1, 64, 10], [1000, 65, 130], [-5, 3, 63]])
+def test_prefix(cuda, prefix, causal):
+    pre = [min(max(x, 0), k) for x, k in zip(prefix, [150, 65, 200])]
+    ql, kl = [150, 65, 70], [150, 65, 200]
+    q, k, v, do, qo, ko = _make(ql, kl, 2, 1, 32, BF, 3)
+    ref = A.attn_var(q, k, v, 2, 1, ql, kl, qo, ko, causal=causal, prefix=pre)
+    out = ops.attn_var(q.to(cuda), k.to(cuda), v.to(cuda), ops.AttnSeqs(ql, kl, device=cuda), 2, 1, causal=causal,
+                       prefix=torch.tensor(prefix, dtype=torch.int32, device=cuda))
+    A.close(out, ref["out"], ref["out_tol"], "out")
+    _check(cuda, ql, kl, 2, 1, 32, causal=causal, prefix=pre, seed=3)
+
+
+def _docs(kind, ql, kl, seed):
+    r = np.random.RandomState(seed)
+    kd = [{"rising": lambda n: np.arange(n) // 37, "any": lambda n: r.randint(-3, 4, n), "own": lambda n: np.arange(n)}[kind](n) for n in kl]
+    qd = [d[len(d) - n:] if n <= len(d) else np.concatenate([np.full(n - len(d), 99), d]) for n, d in zip(ql, kd)]
+    return tuple(torch.as_tensor(np.concatenate(x), dtype=torch.int32) for x in (qd, kd))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal,prefix", [(False, None), (True, None), (False, [70, 0, 5]), (True, [70, 0, 5])])
+@pytest.mark.parametrize("kind", ["rising", "any", "own"])
+def test_documents(cuda, kind, causal, prefix, dtype):
+    """query ids 99 (rows before the first key) match no key: rows that see nothing"""
+    ql, kl = [200, 90, 150], [200, 64, 150]
+    _check(cuda, ql, kl, 2, 1, 32, dtype, causal=causal, prefix=prefix, docs=_docs(kind, ql, kl, 1))
+
+
+def test_long_histories(cuda):
+    _check(cuda, [1100], [1100], 2, 1, 80, causal=True, slopes=[0.01, 0.2])
+    _check(cuda, [3, 600], [2500, 1300], 2, 2, 128, cap=8.0)
+
+
+def test_rows_of_no_example_stay(cuda):
+    """gaps between the examples: zeros in what autograd returns, untouched in buffers handed to the C entry"""
+    _check(cuda, [40, 0, 65], [40, 0, 65], 2, 1, 32, gap=3, causal=True)
+    q, k, v, do, qo, ko = (t.to(cuda) if isinstance(t, torch.Tensor) else t for t in _make([40, 65], [40, 65], 2, 1, 32, BF, 5, gap=3))
+    seqs = ops.AttnSeqs([40, 65], None, qo, device=cuda)
+    cfg = (2, 1, 0.2, 0.0, True, 65, 65)
+    out, lse = torch.full_like(q, 7.0), torch.full((q.shape[0], 2), 7.0, device=cuda)
+    lens = (seqs.q_lens, seqs.q_off, seqs.k_lens, seqs.k_off)
+    d = ops._attn_var_desc(q, k, v, None, None, None, None, lens, out, lse, cfg)
+    L.check(L.load().dmt_attn_var_fwd(d, ops.stream_ptr()))
+    dq, dk, dv = torch.full_like(q, 7.0), torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    d.dout, d.do_rs, d.dQ, d.dq_rs, d.dK, d.dk_rs, d.dV, d.dv_rs = (do.data_ptr(), 64, dq.data_ptr(), 64, dk.data_ptr(), 32, dv.data_ptr(), 32)
+    ws = ops._var_ws(d, 1, cuda)
+    L.check(L.load().dmt_attn_var_bwd(d, ops.stream_ptr()))
+    torch.cuda.synchronize()
+    gap = torch.ones(q.shape[0], dtype=torch.bool, device=cuda)
+    for o, n in zip(qo, (40, 65)):
+        gap[o:o + n] = False
+    for t in (out, lse, dq, dk, dv):
+        assert (t[gap] == 7.0).all() and not (t[~gap] == 7.0).all(1).any()
+    del ws
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("where", ["k", "v", "kv"])
+def test_masked_places_may_hold_anything(cuda, where, bad, dtype):
+    """NaN / infinity in the last key of a causal history reaches the last row alone; in a document of its own it reaches nobody; rows of no
+    example hold it too"""
+    ql = [100, 150]
+    q, k, v, do, qo, ko = _make(ql, ql, 2, 1, 32, dtype, 9, gap=2)
+    last = [qo[0] + 99, qo[1] + 149]
+    for r in last + [qo[0] + 100, qo[1] + 151]:
+        if "k" in where:
+            k[r] = bad
+        if "v" in where:
+            v[r] = bad
+    q[qo[0] + 101], do[qo[1] + 150] = bad, bad
+    do[last] = 0
+    own = torch.zeros(q.shape[0], dtype=torch.int32)
+    own[last] = 1
+    for kw, docs, clean in ((dict(causal=True), None, last), (dict(), (torch.zeros_like(own), own), [])):
+        seqs = ops.AttnSeqs(ql, None, qo, device=cuda)
+        lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+        out = ops.attn_var(*lv, seqs, 2, 1, docs=None if docs is None else tuple(t.to(cuda) for t in docs), **kw)
+        k0, v0 = k.clone(), v.clone()
+        k0[~torch.isfinite(k0)], v0[~torch.isfinite(v0)] = 0, 0
+        ref = A.attn_var(q, k0, v0, 2, 1, ql, ql, qo, ko, docs=docs, dout=do, **kw)
+        keep = torch.ones(q.shape[0], dtype=torch.bool)
+        keep[clean] = False
+        A.close(out[keep.to(cuda)], ref["out"][keep], ref["out_tol"][keep], "out")
+        if clean:
+            continue                                   # (rows that see the value have gradients of their own)
+        for t, n in zip(torch.autograd.grad(out, lv, do.to(cuda)), ("dq", "dk", "dv")):
+            A.close(t[keep.to(cuda)], ref[n][keep], ref[n + "_tol"][keep], n)
+
+
+def test_lowest_and_large_scores(cuda):
+    """scores of 1e4 and more (one key takes all), and columns of the type's lowest value in V"""
+    _check(cuda, [70], [70], 2, 1, 32, std=60.0, causal=True)
+    q, k, v, do, qo, ko = _make([64], [64], 1, 1, 32, BF, 2)
+    v[:, 0] = torch.finfo(BF).min
+    ref = A.attn_var(q, k, v, 1, 1, [64], [64], qo, ko, causal=True)
+    out = ops.attn_var(q.to(cuda), k.to(cuda), v.to(cuda), ops.AttnSeqs([64], device=cuda), 1, causal=True)
+    A.close(out[:, 1:], ref["out"][:, 1:], ref["out_tol"][:, 1:], "out")
+    assert (out[:, 0].float() < -3.3e38).all()
+
+
+def test_strides_alignment_and_order(cuda):
+    """column slices of a packed projection, examples in any order, an operand whose rows are not aligned"""
+    H, Hkv, dh = 4, 2, 16
+    ql, qo = [50, 70, 9], [79, 9, 0]
+    g = torch.Generator().manual_seed(1)
+    pk = torch.randn((129, (H + 2 * Hkv) * dh), generator=g).to(BF)
+    do = torch.randn((129, H * dh), generator=g).to(BF)
+    cut = lambda t: (t[:, :64], t[:, 64:96], t[:, 96:])  # noqa: E731
+    ref = A.attn_var(*cut(pk), H, Hkv, ql, ql, qo, qo, causal=True, dout=do)
+    x = pk.to(cuda).requires_grad_(True)
+    seqs = ops.AttnSeqs(ql, None, qo, device=cuda)
+    out = ops.attn_var(*cut(x), seqs, H, Hkv, causal=True)
+    A.close(out, ref["out"], ref["out_tol"], "out")
+    (dx,) = torch.autograd.grad(out, x, do.to(cuda))
+    for t, n in zip(cut(dx), ("dq", "dk", "dv")):
+        A.close(t, ref[n], ref[n + "_tol"], n)
+    odd = torch.zeros((129, 65), dtype=BF, device=cuda)[:, 1:]
+    odd.copy_(x[:, :64].detach())
+    out = ops.attn_var(odd, x.detach()[:, 64:96], x.detach()[:, 96:], seqs, H, Hkv, causal=True)
+    A.close(out, ref["out"], ref["out_tol"], "out of unaligned rows")
+    wide = torch.zeros((129, 130), dtype=BF, device=cuda)
+    out = ops.attn_var(*cut(x), seqs, H, Hkv, causal=True)
+    (dx2,) = torch.autograd.grad(out, x, wide[:, 1:65].copy_(do.to(cuda)))
+    assert torch.equal(dx2, dx)
+
+
+def test_shared_key_rows_forward_only(cuda):
+    """several examples over the same keys (candidates of one user): forward; the backward refuses"""
+    q, k, v, do, qo, ko = _make([5, 7, 3], [90], 2, 1, 32, BF, 4)
+    kl, ko = [90, 90, 50], [0, 0, 20]
+    ref = A.attn_var(q, k, v, 2, 1, [5, 7, 3], kl, qo, ko)
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+    out = ops.attn_var(*lv, ops.AttnSeqs([5, 7, 3], kl, None, ko, device=cuda), 2, 1)
+    A.close(out, ref["out"], ref["out_tol"], "out")
+    with pytest.raises(RuntimeError, match="share key rows"):
+        out.sum().backward()
+
+
+def test_gradients_against_differences(cuda):
+    """fp32, every feature at once: the directional derivative of a weighted sum against central differences in 64 bits of the definition"""
+    ql, kl, H, Hkv, dh = [20, 9], [25, 9], 2, 1, 20
+    q, k, v, do, qo, ko = _make(ql, kl, H, Hkv, dh, F32, 11)
+    sl, pre, docs = torch.tensor([0.1, 0.4]), [4, 0], _docs("any", ql, kl, 2)
+    kw = dict(causal=True, cap=2.0)
+
+    def f(q, k, v, sl):
+        return float((A.attn_var(q, k, v, H, Hkv, ql, kl, qo, ko, slopes=sl, prefix=pre, docs=docs, **kw)["out"] * do.double()).sum())
+
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v, sl)]
+    out = ops.attn_var(*lv[:3], ops.AttnSeqs(ql, kl, device=cuda), H, Hkv, slopes=lv[3], prefix=torch.tensor(pre, dtype=torch.int32, device=cuda),
+                       docs=tuple(t.to(cuda) for t in docs), **kw)
+    grads = torch.autograd.grad(out, lv, do.to(cuda))
+    g = torch.Generator().manual_seed(5)
+    for i, x in enumerate((q, k, v, sl)):
+        d = torch.randn(x.shape, generator=g).double()
+        a = [t.double() for t in (q, k, v, sl)]
+        a[i] = x.double() + 1e-5 * d
+        hi = f(*a)
+        a[i] = x.double() - 1e-5 * d
+        lo = f(*a)
+        want, got = (hi - lo) / 2e-5, float((grads[i].cpu().double() * d).sum())
+        assert abs(got - want) <= 2e-5 * float((grads[i].cpu().double() * d).abs().sum()) + 1e-6, (i, got, want)
+
+
+def test_replays_and_runs_are_identical(cuda):
+    """a forward + backward captured in a graph, replayed with eager work of the same leaves between: every replay equals the eager result"""
+    ql = [130, 64, 201]
+    q, k, v, do, qo, ko = (t.to(cuda) if isinstance(t, torch.Tensor) else t for t in _make(ql, ql, 4, 2, 64, BF, 7))
+    seqs = ops.AttnSeqs(ql, device=cuda)
+    sl = torch.tensor([0.1, 0.2, 0.3, 0.4], device=cuda)
+    docs = tuple(t.to(cuda) for t in _docs("rising", ql, ql, 1))
+    lv = [t.requires_grad_(True) for t in (q, k, v, sl)]
+
+    def step():
+        out, lse = ops.attn_var(*lv[:3], seqs, 4, 2, slopes=lv[3], causal=True, cap=9.0, docs=docs, want_lse=True)
+        return (out.detach(), lse) + torch.autograd.grad(out, lv, do)
+
+    want = [t.clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want, again):
+        assert torch.equal(a, b)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        r1 = step()
+    with torch.cuda.graph(g2):
+        r2 = step()
+    for _ in range(3):
+        for t in r1 + r2:
+            t.fill_(float("nan"))
+        g1.replay()
+        step()
+        g2.replay()
+        torch.cuda.synchronize()
+        for a, b, c in zip(want, r1, r2):
+            assert torch.equal(a, b) and torch.equal(a, c)
