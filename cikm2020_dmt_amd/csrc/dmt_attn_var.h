@@ -169,8 +169,12 @@ __device__ void row_fwd(const Args& a, const Ex& e, int h, int i, float* lds, in
 }
 
 // dq of one row; returns this row's part of dslopes[h] (all lanes):
-//     - sum_j |d_j| P_j (dP_j - D)  =  S0 S2 - S1,   S0 = sum P dP, S1 = sum P dP |d|, S2 = sum P |d|
+//     - sum_j |d_j| P_j (dP_j - D)  =  S0 S2 - S1,   S0 = sum P dP, S1 = sum P dP |d|, S2 = sum P |d|,  each over Sp = sum P
 // with D = S0 from the same weights, not from the rounded output: the terms cancel, and dslopes is an fp32 result.
+__device__ __forceinline__ float slope_part(float s0, float s1, float s2, float sp) {
+  const float i = sp == 0.f ? 0.f : 1.f / sp;
+  return i * __builtin_fmaf(s0 * i, s2, -s1);
+}
 template <typename T>
 __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, int lane) {
   float* q = lds;
@@ -188,7 +192,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, in
   const Shape s = shape_of(a, h);
   const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
   const float lse2 = a.lse[row * a.Hq + h] * LOG2E, D = a.D[row * a.Hq + h];
-  float o0 = 0.f, o1 = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f;
+  float o0 = 0.f, o1 = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
   for (int j0 = 0; j0 < e.kl; j0 += 64) {
     const int j = j0 + lane;
     const bool ok = may_see(a, e, i, j, qd);
@@ -201,6 +205,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, in
       const float p = exp2_hw(z2_of(s, x, dist) - lse2);
       const float dp = dot_rows<T>(g, V + (long long)j * a.v_rs, dh), pd = p * dp;
       s0 += pd;
+      sp += p;
       s1 = __builtin_fmaf(pd, fabsf(dist), s1);
       s2 = __builtin_fmaf(p, fabsf(dist), s2);
       dx = p * (dp - D);
@@ -223,8 +228,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, in
   T* O = (T*)a.dQ + row * a.dq_rs + (long long)h * dh;
   if (lane < dh) stf<T>(O + lane, o0 * a.scale);
   if (lane + 64 < dh) stf<T>(O + lane + 64, o1 * a.scale);
-  s0 = wave_sum(s0);
-  return __builtin_fmaf(s0, wave_sum(s2), -wave_sum(s1));
+  return slope_part(wave_sum(s0), wave_sum(s1), wave_sum(s2), wave_sum(sp));
 }
 
 // dk and dv of one key row: over the query heads of its group, then over the queries
@@ -286,6 +290,188 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int j, float* lds, i
   T* dv = (T*)a.dV + row * a.dv_rs + (long long)hk * dh;
   if (lane < dh) { stf<T>(dk + lane, k0 * a.scale); stf<T>(dv + lane, v0); }
   if (lane + 64 < dh) { stf<T>(dk + lane + 64, k1 * a.scale); stf<T>(dv + lane + 64, v1); }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- tiles
+// 32 x 32 products (v_mfma_f32_32x32x16_bf16, v_mfma_f32_32x32x2_f32): a lane l holds column l % 32 of the result and the 16 rows
+// 8 (r / 4) + 4 (l / 32) + r % 4, r = 0 .. 15.  Scores are computed with the OWNED row (a query in the forward and dQ kernels, a key in the
+// dK / dV kernel) as the column: its statistics are one value of a lane, a softmax needs one exchange between the halves, and the weights
+// are already the B operand of the next product -- the sum over the 16 register rows may run in any order, so the A operand is read in the
+// registers' order (two transposing 8-byte LDS reads of 4 rows each in bf16; one element a register in fp32).
+typedef __attribute__((ext_vector_type(8))) short bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) short bf16x4_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
+typedef __attribute__((address_space(3))) bf16x4_t* lds_p4;
+
+__device__ __forceinline__ f32x16_t zero16() {
+  f32x16_t z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+__device__ __forceinline__ int reg_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+__device__ __forceinline__ float other_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <typename T, int DHP> struct Tile;
+template <int DHP> struct Tile<bf16_t, DHP> {
+  typedef bf16x8_t Frag;
+  static constexpr int NS = DHP / 16;             // contraction steps of a head
+  static constexpr int NDT = (DHP + 31) / 32;     // 32-dim tiles of a head
+  static constexpr int CH = DHP / 8;              // 16-byte chunks of a row
+  static constexpr int CHE = 8;                   // elements of a chunk
+  static constexpr int RS = DHP + 8;              // LDS row stride: 16-byte reads of 8 consecutive rows hit 8 different bank groups
+  static constexpr int rst() { int r = DHP; while (r % 128 != 32 && r % 128 != 96) r += 8; return r; }
+  static constexpr int RST = rst();               // and of a tile read transposed only: 4 rows on disjoint banks
+  static __device__ __forceinline__ Frag natural(const bf16_t* X, int rs, int row, int s, int half) {
+    return *reinterpret_cast<const bf16x8_t*>(X + row * rs + 16 * s + 8 * half);
+  }
+  static __device__ __forceinline__ int col(int s, int half) { return 16 * s + 8 * half; }
+  static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, const f32x16_t& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int rs, int row0, const f32x16_t& w, int lane) {
+    const int half = lane >> 5, i16 = lane & 15, grp = (lane >> 4) & 1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      union { bf16x8_t v; unsigned d[4]; } b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) b.d[i] = dmt_pack_bf16(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+      const bf16_t* x = X + (row0 + 16 * u + 4 * half + (i16 >> 2)) * rs + 16 * grp + 4 * (i16 & 3);
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + dt * 32));
+        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + dt * 32 + 8 * rs));
+        acc[dt] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b.v, acc[dt]);
+      }
+    }
+  }
+};
+template <int DHP> struct Tile<float, DHP> {
+  typedef f32x4_t Frag;
+  static constexpr int NS = DHP / 8;
+  static constexpr int NDT = (DHP + 31) / 32;
+  static constexpr int CH = DHP / 4;
+  static constexpr int CHE = 4;
+  static constexpr int RS = DHP + 4;
+  static constexpr int RST = DHP + 4;
+  static __device__ __forceinline__ Frag natural(const float* X, int rs, int row, int s, int half) {
+    return *reinterpret_cast<const f32x4_t*>(X + row * rs + 8 * s + 4 * half);
+  }
+  static __device__ __forceinline__ int col(int s, int half) { return 8 * s + 4 * half; }
+  static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, f32x16_t c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int rs, int row0, const f32x16_t& w, int lane) {
+    const float* x = X + (row0 + 4 * (lane >> 5)) * rs + (lane & 31);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[(8 * (r >> 2) + (r & 3)) * rs + dt * 32], w[r], acc[dt], 0, 0, 0);
+    }
+  }
+};
+
+// A buffer descriptor over `rows` rows of one head: what lies past the last row or past dim dh reads as zero, so that neither a ragged end
+// nor a padded head size needs a branch, and nothing outside the example is touched.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+template <typename T> __device__ __forceinline__ rsrc_t rows_rsrc(const T* base, long long rs, int rows, int dh) {
+  const unsigned bytes = rows > 0 ? (unsigned)((rows - 1) * (int)(rs * (int)sizeof(T)) + dh * (int)sizeof(T)) : 0u;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00027000);
+}
+constexpr int OUTSIDE = 0x7ffffff0;
+__device__ __forceinline__ u32x4_t load16(rsrc_t r, int off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
+
+// one lane's fragments of its own row (the B operands that stay in registers)
+template <typename T, int DHP>
+__device__ __forceinline__ void own_row(typename Tile<T, DHP>::Frag* f, const T* base, long long rs, int rows, int dh, int row, int half) {
+  const rsrc_t r = rows_rsrc<T>(base, rs, rows, dh);
+  const int at = row * (int)(rs * (int)sizeof(T));
+#pragma unroll
+  for (int s = 0; s < Tile<T, DHP>::NS; ++s) {
+    const int c = Tile<T, DHP>::col(s, half);
+    f[s] = __builtin_bit_cast(typename Tile<T, DHP>::Frag, load16(r, c < dh ? at + c * (int)sizeof(T) : OUTSIDE));
+  }
+}
+
+// The 64-row tiles of two operands on their way into LDS: requested into registers one tile ahead, written when the tile before is done with.
+template <typename T, int DHP> struct Stage {
+  typedef Tile<T, DHP> TL;
+  static constexpr int IT = (KT * TL::CH + 255) / 256;
+  u32x4_t a[IT], b[IT];
+  int off_a[IT], off_b[IT], dst[IT];     // byte offsets within a tile; row << 8 | chunk of the destination
+  __device__ __forceinline__ void init(long long rs_a, long long rs_b, int dh, int tid) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int c = tid + i * 256, row = c / TL::CH, ch = c - row * TL::CH;
+      const bool in = row < KT && ch * TL::CHE < dh;
+      off_a[i] = in ? row * (int)(rs_a * (int)sizeof(T)) + ch * 16 : OUTSIDE;
+      off_b[i] = in ? row * (int)(rs_b * (int)sizeof(T)) + ch * 16 : OUTSIDE;
+      dst[i] = row < KT ? (row << 8 | ch) : -1;
+    }
+  }
+  __device__ __forceinline__ void request(const T* pa, long long rs_a, const T* pb, long long rs_b, int rows, int dh) {
+    const rsrc_t ra = rows_rsrc<T>(pa, rs_a, rows, dh), rb = rows_rsrc<T>(pb, rs_b, rows, dh);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) a[i] = load16(ra, off_a[i]);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) b[i] = load16(rb, off_b[i]);
+  }
+  __device__ __forceinline__ void write(T* la, int lds_a, T* lb, int lds_b) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if ((KT * TL::CH) % 256 != 0 && dst[i] < 0) continue;
+      const int row = dst[i] >> 8, ch = dst[i] & 255;
+      *reinterpret_cast<u32x4_t*>(la + row * lds_a + ch * TL::CHE) = a[i];
+      *reinterpret_cast<u32x4_t*>(lb + row * lds_b + ch * TL::CHE) = b[i];
+    }
+  }
+};
+
+// one 32 x 32 result (lane = row of the matrix, registers = dims) to memory
+template <typename T>
+__device__ __forceinline__ void store_dims(const f32x16_t& o, float f, T* row, int dt, int half, int dh) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const int j = dt * 32 + 8 * g + 4 * half;
+    if (j + 4 > dh) continue;
+    if (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(row + j) = make_uint2(dmt_pack_bf16(o[4 * g] * f, o[4 * g + 1] * f), dmt_pack_bf16(o[4 * g + 2] * f, o[4 * g + 3] * f));
+    } else {
+      *reinterpret_cast<float4*>(row + j) = make_float4(o[4 * g] * f, o[4 * g + 1] * f, o[4 * g + 2] * f, o[4 * g + 3] * f);
+    }
+  }
+}
+// 0 when every dim < dh of the lane's half row is finite, else not
+__device__ __forceinline__ float not_finite(const f32x16_t& o, int dt, int half, int dh) {
+  float t = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (dt * 32 + reg_row(r, half) < dh) t += o[r] * 0.f;
+  return t;
+}
+
+// which 128 rows of which head a workgroup takes: workgroups go round the 8 dies, each with an L2 of its own, so a die gets whole heads (the
+// heads that share keys side by side); the tiles with the longest rows of a causal mask start first.
+__device__ __forceinline__ void place(int id, int heads, int nt, bool last_first, int& head, int& tile) {
+  int t;
+  if (heads % 8 == 0) {
+    const int per = heads / 8, s = id >> 3;
+    head = (id & 7) * per + s % per;
+    t = s / per;
+  } else {
+    head = id % heads;
+    t = id / heads;
+  }
+  tile = last_first ? nt - 1 - t : t;
 }
 
 }  // namespace attn_var

@@ -5,14 +5,186 @@ using namespace attn_var;
 
 namespace {
 
-template <typename T>
-__global__ __launch_bounds__(256) void rows_fwd_kernel(const Args a) {
-  __shared__ float lds[4][ROW_LDS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.z, h = blockIdx.y;
+// One workgroup of 4 wavefronts owns 128 queries of a head (a wavefront 32) and walks over the keys in tiles of 64, one tile in LDS, the next
+// one on its way through registers.  One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
+// are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
+template <typename T, int DHP, bool SHAPED>
+__global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) {
+  typedef Tile<T, DHP> TL;
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1;               // tiles in LDS
+  constexpr int KE = KT * TL::RS, VE = KT * TL::RST + 32;
+  __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
+  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
+  int head, qt;
+  place(blockIdx.x, a.B * a.Hq, nt, a.causal, head, qt);
+  const int b = head / a.Hq, h = head - b * a.Hq, hk = h / a.G;
   const Ex e = example(a, b);
-  const int i = blockIdx.x * 4 + wave;
-  if (i < e.ql) row_fwd<T>(a, e, h, i, lds[wave], lane);
+  if (qt * 128 >= e.ql) return;
+  const int iw = qt * 128 + wave * 32, i = iw + l31;
+  const bool active = iw < e.ql;
+  const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
+  const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
+  const Shape sh = shape_of(a, h);
+  typename TL::Frag q[TL::NS];
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
+  // what the workgroup, the wavefront and the lane's row may see
+  const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
+  const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
+  const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
+  const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
+  const int nk = (lim_wg + KT - 1) / KT;
+  int qlo = 0, qhi = 0, wlo = 0, whi = 0, qd = 0;
+  const int2* kr = nullptr;
+  if (a.q_doc) {
+    const int2* qr = a.q_rng + (long long)b * a.nqt;
+    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0;
+    qlo = min(r0.x, r1.x);
+    qhi = max(r0.y, r1.y);
+    const int2 rw = wave < 2 ? r0 : r1;
+    wlo = rw.x;
+    whi = rw.y;
+    qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
+    kr = a.k_rng + (long long)b * a.nkt;
+  }
+  const auto next = [&](int t) {
+    if (kr)
+      while (t < nk && t * KT >= e.pre && (kr[t].x > qhi || kr[t].y < qlo)) ++t;
+    return t;
+  };
+  Stage<T, DHP> st;
+  st.init(a.k_rs, a.v_rs, a.dh, tid);
+  int kd = 0;
+  const auto request = [&](int t) {
+    const int k0 = t * KT;
+    st.request(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh);
+    if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
+  };
+  const auto write = [&](int buf) {
+    st.write(lds + buf * (KE + VE), TL::RS, lds + buf * (KE + VE) + KE, TL::RST);
+    if (kr && tid < KT) docs[buf][tid] = kd;
+  };
+  f32x16_t o[TL::NDT];
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
+  float m = -INFINITY, l = 0.f;
+  int t = next(0), buf = 0;
+  if (t < nk) {
+    request(t);
+    write(0);
+  }
+  __syncthreads();
+  while (t < nk) {
+    const int tn = next(t + 1), k0 = t * KT;
+    if (tn < nk) request(tn);
+    const T* Kl = lds + buf * (KE + VE);
+    const T* Vl = Kl + KE;
+    bool work = active && k0 < lim_w, docs_differ = false;
+    if (kr && k0 + KT > e.pre) {
+      if (k0 >= e.pre && (kr[t].x > whi || kr[t].y < wlo)) work = false;
+      docs_differ = !(kr[t].x == kr[t].y && wlo == whi && wlo == kr[t].x);
+    }
+    if (work) {
+      f32x16_t s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = zero16();
+#pragma unroll
+        for (int x = 0; x < TL::NS; ++x) s[u] = TL::mma(TL::natural(Kl, TL::RS, 32 * u + l31, x, half), q[x], s[u]);
+      }
+      if (SHAPED) {
+        if (sh.cap) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(-2.f * sh.cap2, cap_r(sh, s[u][r]), sh.cap2);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] *= sh.c1;
+        }
+        if (sh.slope) {
+          const float d0 = (float)(i + e.off - k0 - 4 * half);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(-sh.sl2, fabsf(d0 - (float)(32 * u + reg_row(r, 0))), s[u][r]);
+        }
+      }
+      // masked places become -inf: only in the tiles that the lengths, the diagonal or a document boundary cross
+      if (docs_differ) {
+        const int pre = e.pre - k0 - 4 * half, lm = lim0 - k0 - 4 * half;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 d = *reinterpret_cast<const int4*>(&docs[buf][32 * u + 8 * g + 4 * half]);
+            const int dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = 32 * u + 8 * g + c;
+              s[u][4 * g + c] = (key < pre || (key < lm && dd[c] == qd)) ? s[u][4 * g + c] : -INFINITY;
+            }
+          }
+      } else if (k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off)) {
+        const int lm = lim - k0 - 4 * half;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[u][r] = 32 * u + reg_row(r, 0) < lm ? s[u][r] : -INFINITY;
+      }
+      float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
+      mx = fmaxf(mx, other_half(mx));
+      const float c = SHAPED ? 1.f : sh.c1;
+      const float mt = mx * c;
+      if (__any(mt > m + 8.f)) {
+        const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.f : exp2_hw(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < TL::NDT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = exp2_hw(SHAPED ? s[u][r] - mu : __builtin_fmaf(s[u][r], c, -mu));
+          l += s[u][r];
+        }
+        TL::accumulate(o, Vl, TL::RST, 32 * u, s[u], lane);
+      }
+    }
+    if (NB == 1) __syncthreads();
+    if (tn < nk) write(NB == 2 ? buf ^ 1 : 0);
+    __syncthreads();
+    if (NB == 2) buf ^= 1;
+    t = tn;
+  }
+  if (!active) return;
+  l += other_half(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float bad = l * 0.f;
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(o[dt], dt, half, a.dh);
+  const long long row = e.q0 + i;
+  const bool in = i < e.ql;
+  if (in) {
+    T* O = (T*)a.out + row * a.o_rs + (long long)h * a.dh;
+#pragma unroll
+    for (int dt = 0; dt < TL::NDT; ++dt) store_dims<T>(o[dt], inv, O, dt, half, a.dh);
+    if (a.lse && half == 0) a.lse[row * a.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
+  }
+  unsigned long long again = __ballot(in && !(bad == 0.f));
+  again |= again >> 32;
+  for (int r = 0; r < 32; ++r)
+    if ((again >> r) & 1) row_fwd<T>(a, e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
 __global__ void doc_ranges_kernel(const int* off, const int* lens, const int* doc, int most, long long rows, int nt, int B, int2* out) {
@@ -29,9 +201,24 @@ __global__ void doc_ranges_kernel(const int* off, const int* lens, const int* do
   if (lane == 0) out[(long long)b * nt + t] = make_int2(lo, hi);
 }
 
+template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
+  const int nt = (int)cdiv64(a.max_q, 128);
+  const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
+  if (a.cap > 0.f || a.slopes) tile_fwd_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
+  else tile_fwd_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+}
+template <typename T> int launch_fwd(const Args& a, hipStream_t st) {
+  if (a.dh <= 32) launch_tile<T, 32>(a, st);
+  else if (a.dh <= 64) launch_tile<T, 64>(a, st);
+  else if (a.dh <= 80) launch_tile<T, 80>(a, st);
+  else launch_tile<T, 128>(a, st);
+  DMT_CHECK_LAUNCH("dmt_attn_var_fwd");
+  return DMT_OK;
+}
+
 }  // namespace
 
-uint64_t up16(uint64_t x) { return (x + 15) & ~15ull; }
+static uint64_t up16(uint64_t x) { return (x + 15) & ~15ull; }
 
 extern "C" int dmt_attn_var_supported(int32_t dtype, int32_t dh, int32_t Hq, int32_t Hkv) {
   if (dtype != DMT_F32 && dtype != DMT_BF16) return 0;
@@ -70,6 +257,7 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   DMT_CHECK_ARG(dmt_attn_var_supported(d->dtype, d->dh, d->Hq, d->Hkv),
                 "%s: needs bf16 (dh %% 8 == 0) or fp32 (dh %% 4 == 0), dh <= 128 and Hq a multiple of Hkv: got dtype %d, dh %d, Hq %d, Hkv %d", what,
                 d->dtype, d->dh, d->Hq, d->Hkv);
+  DMT_CHECK_ARG((int64_t)d->B * d->Hq * (cdiv64(d->max_q > d->max_k ? d->max_q : d->max_k, 128) + 1) < (1ll << 31), "%s: B * Hq * max length / 128 passes 2^31", what);
   DMT_CHECK_ARG(d->B <= 65535 && d->Hq <= 65535, "%s: B and Hq <= 65535", what);
   DMT_CHECK_ARG(d->rows_q < (1ll << 31) && d->rows_k < (1ll << 31), "%s: row numbers are int32", what);
   DMT_CHECK_ARG(d->scale > 0.f && d->scale < 3.4e38f, "%s: scale must be positive and finite", what);
@@ -132,11 +320,7 @@ extern "C" int dmt_attn_var_fwd(const dmt_attn_var_desc* d, void* stream) {
   Args a;
   const int rc = dmt_attn_var_args(d, &a, false, "dmt_attn_var_fwd");
   if (rc) return rc < 0 ? rc : DMT_OK;
-  const dim3 grid((a.max_q + 3) / 4, a.Hq, a.B);
-  if (d->dtype == DMT_F32)
-    rows_fwd_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-  else
-    rows_fwd_kernel<bf16_t><<<grid, 256, 0, (hipStream_t)stream>>>(a);
-  DMT_CHECK_LAUNCH("dmt_attn_var_fwd(rows)");
-  return DMT_OK;
+  const int rr = dmt_attn_var_doc_ranges(a, stream);
+  if (rr) return rr;
+  return d->dtype == DMT_F32 ? launch_fwd<float>(a, (hipStream_t)stream) : launch_fwd<bf16_t>(a, (hipStream_t)stream);
 }

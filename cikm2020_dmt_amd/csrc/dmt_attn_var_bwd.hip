@@ -25,30 +25,362 @@ __global__ __launch_bounds__(256) void rowsum_kernel(const Args a) {
   if (l16 == 0) a.D[item] = s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void rows_dq_kernel(const Args a) {
-  __shared__ float lds[4][ROW_LDS];
-  __shared__ float part[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.z, h = blockIdx.y;
-  const Ex e = example(a, b);
-  float sl = 0.f;
-  for (int i = blockIdx.x * 128 + wave; i < e.ql && i < (int)blockIdx.x * 128 + 128; i += 4) sl += row_dq<T>(a, e, h, i, lds[wave], lane);
-  if (a.slope_part) {
-    if (lane == 0) part[wave] = sl;
-    __syncthreads();
-    if (threadIdx.x == 0) a.slope_part[((long long)h * a.B + b) * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+// The scores of one 32 x 32 tile, in place: z2 (the row's statistic is subtracted by the caller).  d0: distance of register row 0 and the lane's
+// column; STEP: what a register row adds to it.
+template <int STEP>
+__device__ __forceinline__ void shaped(f32x16_t& s, f32x16_t& r2, const Shape& sh, float d0) {
+  if (sh.cap) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      r2[r] = cap_r(sh, s[r]);
+      s[r] = __builtin_fmaf(-2.f * sh.cap2, r2[r], sh.cap2);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= sh.c1;
+  }
+  if (sh.slope) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), s[r]);
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void rows_dkv_kernel(const Args a) {
-  __shared__ float lds[4][ROW_LDS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.z, hk = blockIdx.y;
+// dQ: one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
+template <typename T, int DHP, bool SHAPED>
+__global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
+  typedef Tile<T, DHP> TL;
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1;
+  constexpr int KE = KT * TL::RS + 32, VE = KT * TL::RS;
+  __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
+  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  __shared__ float part[4];
+  static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
+  int head, qt;
+  place(blockIdx.x, a.B * a.Hq, nt, a.causal, head, qt);
+  const int b = head / a.Hq, h = head - b * a.Hq, hk = h / a.G;
   const Ex e = example(a, b);
-  const int j = blockIdx.x * 4 + wave;
-  if (j < e.kl) row_dkv<T>(a, e, hk, j, lds[wave], lane);
+  if (qt * 128 >= e.ql) {
+    if (a.slope_part && tid == 0) a.slope_part[((long long)h * a.B + b) * nt + qt] = 0.f;
+    return;
+  }
+  const int iw = qt * 128 + wave * 32, i = iw + l31;
+  const bool active = iw < e.ql, in = i < e.ql;
+  const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
+  const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
+  const Shape sh = shape_of(a, h);
+  typename TL::Frag q[TL::NS], g[TL::NS];
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
+  own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, i, half);
+  const long long stat = (e.q0 + (in ? i : 0)) * a.Hq + h;
+  // (a row that sees nothing: lse = -inf; its weights 2^(z - inf) are 0)
+  const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY, D = in ? a.D[stat] : 0.f;
+  const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
+  const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
+  const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
+  const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
+  const int nk = (lim_wg + KT - 1) / KT;
+  int qlo = 0, qhi = 0, wlo = 0, whi = 0, qd = 0;
+  const int2* kr = nullptr;
+  if (a.q_doc) {
+    const int2* qr = a.q_rng + (long long)b * a.nqt;
+    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0;
+    qlo = min(r0.x, r1.x);
+    qhi = max(r0.y, r1.y);
+    const int2 rw = wave < 2 ? r0 : r1;
+    wlo = rw.x;
+    whi = rw.y;
+    qd = in ? a.q_doc[e.q0 + i] : 0;
+    kr = a.k_rng + (long long)b * a.nkt;
+  }
+  const auto next = [&](int t) {
+    if (kr)
+      while (t < nk && t * KT >= e.pre && (kr[t].x > qhi || kr[t].y < qlo)) ++t;
+    return t;
+  };
+  Stage<T, DHP> st;
+  st.init(a.k_rs, a.v_rs, a.dh, tid);
+  int kd = 0;
+  const auto request = [&](int t) {
+    const int k0 = t * KT;
+    st.request(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh);
+    if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
+  };
+  const auto write = [&](int buf) {
+    st.write(lds + buf * (KE + VE), TL::RS, lds + buf * (KE + VE) + KE, TL::RS);
+    if (kr && tid < KT) docs[buf][tid] = kd;
+  };
+  f32x16_t o[TL::NDT];
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
+  int t = next(0), buf = 0;
+  if (t < nk) {
+    request(t);
+    write(0);
+  }
+  __syncthreads();
+  while (t < nk) {
+    const int tn = next(t + 1), k0 = t * KT;
+    if (tn < nk) request(tn);
+    const T* Kl = lds + buf * (KE + VE);
+    const T* Vl = Kl + KE;
+    bool work = active && k0 < lim_w, docs_differ = false;
+    if (kr && k0 + KT > e.pre) {
+      if (k0 >= e.pre && (kr[t].x > whi || kr[t].y < wlo)) work = false;
+      docs_differ = !(kr[t].x == kr[t].y && wlo == whi && wlo == kr[t].x);
+    }
+    if (work) {
+      const bool cut = k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16_t s = zero16(), dp = zero16(), r2;
+#pragma unroll
+        for (int x = 0; x < TL::NS; ++x) {
+          s = TL::mma(TL::natural(Kl, TL::RS, 32 * u + l31, x, half), q[x], s);
+          dp = TL::mma(TL::natural(Vl, TL::RS, 32 * u + l31, x, half), g[x], dp);
+        }
+        const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
+        if (SHAPED) shaped<-1>(s, r2, sh, d0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(SHAPED ? s[r] - lse2 : __builtin_fmaf(s[r], sh.c1, -lse2));
+        if (docs_differ || cut) {
+          // (a masked place gives weight and gradient 0 whatever stands there)
+          const int pre = e.pre - k0 - 32 * u - 4 * half, lm = (docs_differ ? lim0 : lim) - k0 - 32 * u - 4 * half;
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg) {
+            int4 d = make_int4(qd, qd, qd, qd);
+            if (docs_differ) d = *reinterpret_cast<const int4*>(&docs[buf][32 * u + 8 * gg + 4 * half]);
+            const int dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = 8 * gg + c;
+              const bool ok = key < pre || (key < lm && dd[c] == qd);
+              s[4 * gg + c] = ok ? s[4 * gg + c] : 0.f;
+              dp[4 * gg + c] = ok ? dp[4 * gg + c] : 0.f;
+            }
+          }
+        }
+        if (SHAPED && a.slope_part) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float ad = fabsf(d0 - (float)reg_row(r, 0)), pd = s[r] * dp[r];
+            s0 += pd;
+            s1 = __builtin_fmaf(pd, ad, s1);
+            s2 = __builtin_fmaf(s[r], ad, s2);
+            sp += s[r];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] *= dp[r] - D;
+          if (SHAPED && sh.cap) s[r] *= 4.f * r2[r] * (1.f - r2[r]);
+        }
+        TL::accumulate(o, Kl, TL::RS, 32 * u, s, lane);
+      }
+    }
+    if (NB == 1) __syncthreads();
+    if (tn < nk) write(NB == 2 ? buf ^ 1 : 0);
+    __syncthreads();
+    if (NB == 2) buf ^= 1;
+    t = tn;
+  }
+  float sl = 0.f;
+  if (active) {
+    if (SHAPED && a.slope_part) {
+      s0 += other_half(s0);
+      s1 += other_half(s1);
+      s2 += other_half(s2);
+      sp += other_half(sp);
+      sl = in ? slope_part(s0, s1, s2, sp) : 0.f;
+    }
+    float bad = sl * 0.f;
+#pragma unroll
+    for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(o[dt], dt, half, a.dh);
+    if (in) {
+      T* O = (T*)a.dQ + (e.q0 + i) * a.dq_rs + (long long)h * a.dh;
+#pragma unroll
+      for (int dt = 0; dt < TL::NDT; ++dt) store_dims<T>(o[dt], a.scale, O, dt, half, a.dh);
+    }
+    unsigned long long again = __ballot(in && !(bad == 0.f));
+    again |= again >> 32;
+    if ((again >> l31) & 1) sl = 0.f;
+    if (half) sl = 0.f;                                  // (both halves hold the row's)
+    sl = wave_sum(sl);
+    for (int r = 0; r < 32; ++r)
+      if ((again >> r) & 1) sl += row_dq<T>(a, e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
+  }
+  if (a.slope_part) {
+    if (lane == 0) part[wave] = sl;
+    __syncthreads();
+    if (tid == 0) a.slope_part[((long long)h * a.B + b) * nt + qt] = (part[0] + part[1]) + (part[2] + part[3]);
+  }
+}
+
+// dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
+// tiles of 64: S and dP with lane = key, P and dX packed are the B operands of dV^T += dO^T P and dK^T += Q^T dX.  Nothing crosses wavefronts.
+template <typename T, int DHP, bool SHAPED>
+__global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv_kernel(const Args a, int nt) {
+  typedef Tile<T, DHP> TL;
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1;
+  constexpr int QE = KT * TL::RS + 32;
+  __shared__ __attribute__((aligned(16))) T lds[NB * 2 * QE];
+  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  __shared__ __attribute__((aligned(16))) float stats[NB][2][KT];
+  static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
+  int head, kt;
+  place(blockIdx.x, a.B * a.Hkv, nt, false, head, kt);
+  const int b = head / a.Hkv, hk = head - b * a.Hkv;
+  const Ex e = example(a, b);
+  if (kt * 128 >= e.kl) return;
+  const int jw = kt * 128 + wave * 32, j = jw + l31;
+  const bool active = jw < e.kl;
+  typename TL::Frag k[TL::NS], v[TL::NS];
+  own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, j, half);
+  own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
+  // queries that may see some key of the workgroup / wavefront / lane: from `lo` on (rows before it sit above the diagonal, unless the key
+  // belongs to the prefix)
+  const int lo_wg = a.causal && kt * 128 >= e.pre ? max(0, kt * 128 - e.off) : 0;
+  const int lo_w = a.causal && jw >= e.pre ? max(0, jw - e.off) : 0;
+  const int lo_l = j >= e.kl ? 0x7fffffff : (a.causal && j >= e.pre ? max(0, j - e.off) : 0);
+  const int t0 = lo_wg / KT, nq = (e.ql + KT - 1) / KT, per = nq > t0 ? nq - t0 : 0, total = per * a.G;
+  const bool free_keys = jw < e.pre;                      // some key of the wavefront is in the prefix: no document hides it
+  int klo = 0, khi = 0, wlo = 0, whi = 0, kd_l = 0;
+  const int2* qr = nullptr;
+  if (a.q_doc) {
+    const int2* kr = a.k_rng + (long long)b * a.nkt;
+    const int2 r0 = kr[kt * 2], r1 = kt * 2 + 1 < a.nkt ? kr[kt * 2 + 1] : r0;
+    klo = min(r0.x, r1.x);
+    khi = max(r0.y, r1.y);
+    const int2 rw = wave < 2 ? r0 : r1;
+    wlo = rw.x;
+    whi = rw.y;
+    kd_l = j < e.kl ? a.k_doc[e.k0 + j] : 0;
+    qr = a.q_rng + (long long)b * a.nqt;
+  }
+  // step n of the walk: head n / per of the group, tile t0 + n % per
+  const auto next = [&](int n) {
+    if (qr && kt * 128 >= e.pre)
+      while (n < total && (qr[t0 + n % per].x > khi || qr[t0 + n % per].y < klo)) ++n;
+    return n;
+  };
+  Stage<T, DHP> st;
+  st.init(a.q_rs, a.do_rs, a.dh, tid);
+  int qd = 0;
+  float lse2 = 0.f;
+  const auto request = [&](int n) {
+    const int h = hk * a.G + n / per, i0 = (t0 + n % per) * KT;
+    st.request((const T*)a.Q + (e.q0 + i0) * a.q_rs + (long long)h * a.dh, a.q_rs, (const T*)a.dout + (e.q0 + i0) * a.do_rs + (long long)h * a.dh, a.do_rs,
+               min(KT, e.ql - i0), a.dh);
+    if (tid < 2 * KT) {
+      const int i = i0 + (tid & (KT - 1));
+      const long long stat = (e.q0 + i) * a.Hq + h;
+      if (tid < KT) {
+        const float x = i < e.ql ? a.lse[stat] : -INFINITY;
+        lse2 = x != -INFINITY ? x * LOG2E : INFINITY;     // (rows that see nothing, rows past the end: weight 0)
+        if (qr) qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
+      } else {
+        lse2 = i < e.ql ? a.D[stat] : 0.f;
+      }
+    }
+  };
+  const auto write = [&](int buf) {
+    st.write(lds + buf * 2 * QE, TL::RS, lds + buf * 2 * QE + QE, TL::RS);
+    if (tid < 2 * KT) stats[buf][tid / KT][tid & (KT - 1)] = lse2;
+    if (qr && tid < KT) docs[buf][tid] = qd;
+  };
+  f32x16_t dk[TL::NDT], dv[TL::NDT];
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) dk[dt] = dv[dt] = zero16();
+  int n = next(0), buf = 0;
+  if (n < total) {
+    request(n);
+    write(0);
+  }
+  __syncthreads();
+  while (n < total) {
+    const int nn = next(n + 1), tq = t0 + n % per, i0 = tq * KT;
+    if (nn < total) request(nn);
+    const T* Ql = lds + buf * 2 * QE;
+    const T* Gl = Ql + QE;
+    const Shape sh = shape_of(a, hk * a.G + n / per);
+    bool work = active && i0 + KT > lo_w, docs_differ = false;
+    if (qr) {
+      if (!free_keys && (qr[tq].x > whi || qr[tq].y < wlo)) work = false;
+      docs_differ = jw + 32 > e.pre && !(qr[tq].x == qr[tq].y && wlo == whi && wlo == qr[tq].x);
+    }
+    if (work) {
+      const bool cut = jw + 32 > e.kl || (a.causal && jw + 32 > e.pre && i0 + e.off < jw + 31);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        f32x16_t s = zero16(), dp = zero16(), r2;
+#pragma unroll
+        for (int x = 0; x < TL::NS; ++x) {
+          s = TL::mma(TL::natural(Ql, TL::RS, 32 * u + l31, x, half), k[x], s);
+          dp = TL::mma(TL::natural(Gl, TL::RS, 32 * u + l31, x, half), v[x], dp);
+        }
+        if (SHAPED) shaped<1>(s, r2, sh, (float)(i0 + 32 * u + 4 * half + e.off - j));
+#pragma unroll
+        for (int gg = 0; gg < 4; ++gg) {
+          const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
+          const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[4 * gg + c] = exp2_hw(SHAPED ? s[4 * gg + c] - lv[c] : __builtin_fmaf(s[4 * gg + c], sh.c1, -lv[c]));
+        }
+        if (docs_differ || cut) {
+          const int lo = lo_l - i0 - 32 * u - 4 * half;
+#pragma unroll
+          for (int gg = 0; gg < 4; ++gg) {
+            int4 d = make_int4(kd_l, kd_l, kd_l, kd_l);
+            if (docs_differ && j >= e.pre) d = *reinterpret_cast<const int4*>(&docs[buf][32 * u + 8 * gg + 4 * half]);
+            const int dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const bool ok = 8 * gg + c >= lo && dd[c] == kd_l;
+              s[4 * gg + c] = ok ? s[4 * gg + c] : 0.f;
+              dp[4 * gg + c] = ok ? dp[4 * gg + c] : 0.f;
+            }
+          }
+        }
+        TL::accumulate(dv, Gl, TL::RS, 32 * u, s, lane);
+#pragma unroll
+        for (int gg = 0; gg < 4; ++gg) {
+          const float4 ds = *reinterpret_cast<const float4*>(&stats[buf][1][32 * u + 8 * gg + 4 * half]);
+          const float D[4] = {ds.x, ds.y, ds.z, ds.w};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            s[4 * gg + c] *= dp[4 * gg + c] - D[c];
+            if (SHAPED && sh.cap) s[4 * gg + c] *= 4.f * r2[4 * gg + c] * (1.f - r2[4 * gg + c]);
+          }
+        }
+        TL::accumulate(dk, Ql, TL::RS, 32 * u, s, lane);
+      }
+    }
+    if (NB == 1) __syncthreads();
+    if (nn < total) write(NB == 2 ? buf ^ 1 : 0);
+    __syncthreads();
+    if (NB == 2) buf ^= 1;
+    n = nn;
+  }
+  if (!active) return;
+  const bool in = j < e.kl;
+  float bad = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(dk[dt], dt, half, a.dh) + not_finite(dv[dt], dt, half, a.dh);
+  if (in) {
+    T* pk = (T*)a.dK + (e.k0 + j) * a.dk_rs + (long long)hk * a.dh;
+    T* pv = (T*)a.dV + (e.k0 + j) * a.dv_rs + (long long)hk * a.dh;
+#pragma unroll
+    for (int dt = 0; dt < TL::NDT; ++dt) {
+      store_dims<T>(dk[dt], a.scale, pk, dt, half, a.dh);
+      store_dims<T>(dv[dt], 1.f, pv, dt, half, a.dh);
+    }
+  }
+  unsigned long long again = __ballot(in && !(bad == 0.f));
+  again |= again >> 32;
+  for (int r = 0; r < 32; ++r)
+    if ((again >> r) & 1) row_dkv<T>(a, e, hk, jw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
 // dslopes[h] += sum of its parts, in their order (64 bits: the terms cancel)
@@ -66,6 +398,17 @@ __global__ __launch_bounds__(256) void slopes_kernel(const float* part, long lon
   if (threadIdx.x == 0) out[blockIdx.x] += (float)red[0];
 }
 
+template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
+  if (a.cap > 0.f || a.slopes) tile_dq_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
+  else tile_dq_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+}
+template <typename T, int DHP> void launch_dkv(const Args& a, int nt, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B);
+  if (a.cap > 0.f || a.slopes) tile_dkv_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
+  else tile_dkv_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+}
+
 template <typename T>
 int launch_bwd(const Args& a, hipStream_t st) {
   const long long items = a.rows_q * a.Hq;
@@ -73,16 +416,23 @@ int launch_bwd(const Args& a, hipStream_t st) {
     rowsum_kernel<T><<<(unsigned)cdiv64(items, 16), 256, 0, st>>>(a);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(row sums)");
     const int nt = (int)cdiv64(a.max_q, 128);
-    rows_dq_kernel<T><<<dim3(nt, a.Hq, a.B), 256, 0, st>>>(a);
-    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq rows)");
+    if (a.dh <= 32) launch_dq<T, 32>(a, nt, st);
+    else if (a.dh <= 64) launch_dq<T, 64>(a, nt, st);
+    else if (a.dh <= 80) launch_dq<T, 80>(a, nt, st);
+    else launch_dq<T, 128>(a, nt, st);
+    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq)");
     if (a.slope_part) {
       slopes_kernel<<<a.Hq, 256, 0, st>>>(a.slope_part, (long long)a.B * nt, a.dslopes);
       DMT_CHECK_LAUNCH("dmt_attn_var_bwd(slopes)");
     }
   }
   if (a.rows_k && a.max_k) {
-    rows_dkv_kernel<T><<<dim3((a.max_k + 3) / 4, a.Hkv, a.B), 256, 0, st>>>(a);
-    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dkv rows)");
+    const int nt = (int)cdiv64(a.max_k, 128);
+    if (a.dh <= 32) launch_dkv<T, 32>(a, nt, st);
+    else if (a.dh <= 64) launch_dkv<T, 64>(a, nt, st);
+    else if (a.dh <= 80) launch_dkv<T, 80>(a, nt, st);
+    else launch_dkv<T, 128>(a, nt, st);
+    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dkv)");
   }
   return DMT_OK;
 }
@@ -93,5 +443,7 @@ extern "C" int dmt_attn_var_bwd(const dmt_attn_var_desc* d, void* stream) {
   Args a;
   int rc = dmt_attn_var_args(d, &a, true, "dmt_attn_var_bwd");
   if (rc) return rc < 0 ? rc : DMT_OK;
+  rc = dmt_attn_var_doc_ranges(a, stream);
+  if (rc) return rc;
   return d->dtype == DMT_F32 ? launch_bwd<float>(a, (hipStream_t)stream) : launch_bwd<bf16_t>(a, (hipStream_t)stream);
 }
