@@ -416,12 +416,390 @@ __device__ void kv_row(const KvArgs& a, const Req& rq, int r, int h, int i, floa
   if (a.lse && lane == 0) a.lse[row * a.Hq + h] = (m == -INFINITY && l == 0.f) ? -INFINITY : (m + __log2f(l)) * LN2;
 }
 
-__global__ __launch_bounds__(256) void kv_rows_kernel(const KvArgs a) {
+// Tiles.  A wavefront takes a block of 64 tokens at a time and the columns of a tile -- 16 NQ (row, head of the group) pairs: heads that share a
+// key head read its bytes together -- and keeps its own running maximum, sum and output; the four wavefronts of a workgroup walk over every
+// fourth block of the workgroup's piece of the length.  K and V go from memory to registers in 16-byte loads (each byte once a tile of columns)
+// and become bf16 by v_cvt_scalef32_pk_bf16_fp8, which takes the block's scale along: the products see the stored values exactly.
+//   S^T = K Q^T   (16x16x32, tokens x columns): the contraction runs over the dims in the order in which a lane loads them -- 16 bytes of a
+//                 row are two steps of 8 -- and Q is laid out the same way; a remainder of 16 dims is a step whose upper half is zero
+//                 (a 16x16x16 product that adds to the result of a 16x16x32 one just before it came out wrong here).
+//   O^T = V^T P^T (dims x columns): the weights of S^T, packed, are the B operand; the places of V are in that order.
+// What bounds it: the cache's bytes for few columns; beyond about 100 columns a key head the conversion and the softmax.
+typedef __attribute__((ext_vector_type(8))) short bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) short bf16x4_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+
+// 4 bytes -> 4 bf16 (two registers)
+__device__ __forceinline__ uint2 f8x4_bf16(unsigned w, float scale) {
+  return make_uint2(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false)),
+                    __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true)));
+}
+__device__ __forceinline__ bf16x8_t f8x8_bf16(unsigned lo, unsigned hi, float scale) {
+  union { bf16x8_t v; uint2 d[2]; } u;
+  u.d[0] = f8x4_bf16(lo, scale);
+  u.d[1] = f8x4_bf16(hi, scale);
+  return u.v;
+}
+__device__ __forceinline__ bf16x8_t f8x4_frag(unsigned w, float scale) {
+  union { bf16x8_t v; uint2 d[2]; } u;
+  u.d[0] = f8x4_bf16(w, scale);
+  u.d[1] = make_uint2(0u, 0u);
+  return u.v;
+}
+
+// max / sum over the four 16-lane groups (the tokens of one column)
+__device__ __forceinline__ float xor16(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 16) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float xor32(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float col_max(float x) {
+  x = fmaxf(x, xor16(x));
+  return fmaxf(x, xor32(x));
+}
+__device__ __forceinline__ float col_sum(float x) {
+  x += xor16(x);
+  return x + xor32(x);
+}
+
+struct Split { int pieces, chunk, nqt; };          // pieces of the length, blocks of a piece, tiles of columns
+
+template <int DH> struct Dims {
+  static constexpr int N64 = DH / 64, R = DH % 64, N32 = R / 32, N16 = (R % 32) / 16;    // 16-byte, 8-byte and 4-byte loads of a row
+  static constexpr int KW = 4 * N64 + 2 * N32 + N16;                                       // dwords of a lane
+};
+
+template <int DH, int NQ, bool SHAPED>
+__global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+  typedef Dims<DH> DM;
+  constexpr int NC = 16 * NQ, NDT = DH / 16, LO = DH + 4;
+  __shared__ __attribute__((aligned(16))) float lo[4][NC * LO];
+  __shared__ float lm[4][NC], ll[4][NC];
+  static_assert(sizeof(lo[0]) >= (MAX_DH + 64) * sizeof(float), "the row form works in a wavefront's part");
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4, l15 = lane & 15;
+  const int pairs = a.n * a.c.Hkv, items = pairs * sp.pieces, id = blockIdx.x;
+  // the column tiles of one piece read the same bytes: side by side on one die (workgroups go round the 8 dies)
+  int item, qt;
+  if (items % 8 == 0) {
+    item = (id & 7) * (items / 8) + (id >> 3) / sp.nqt;
+    qt = (id >> 3) % sp.nqt;
+  } else {
+    item = id / sp.nqt;
+    qt = id % sp.nqt;
+  }
+  const int piece = item % sp.pieces, pair = item / sp.pieces, hk = pair % a.c.Hkv, r = pair / a.c.Hkv;
+  const Req rq = request(a, r);
+  const int cols = rq.m * a.G, nb = (rq.L + BS - 1) / BS;
+  if (qt * NC >= cols || (piece > 0 && piece * sp.chunk >= nb)) return;
+  int lim[NQ], pos[NQ], lim_wg = 0;
+  float sl2[NQ];
+  constexpr int NF = 2 * DM::N64 + DM::N32;
+  bf16x8_t q[NQ][NF ? NF : 1];
+  bf16x8_t q16[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    const int c = qt * NC + 16 * x + l15;
+    const bool in = c < cols;
+    const int i = in ? c / a.G : 0, g = in ? c - i * a.G : 0, h = hk * a.G + g;
+    lim[x] = in ? sees(a, rq, i) : 0;
+    pos[x] = position(a, rq, i);
+    sl2[x] = SHAPED && a.slopes ? a.slopes[h] * LOG2E : 0.f;
+    const bf16_t* Q = a.Q + (rq.row0 + i) * a.q_rs + (long long)h * DH;
+    const bf16x8_t z8 = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < DM::N64; ++s) {
+      q[x][2 * s] = in ? *reinterpret_cast<const bf16x8_t*>(Q + 64 * s + 16 * grp) : z8;
+      q[x][2 * s + 1] = in ? *reinterpret_cast<const bf16x8_t*>(Q + 64 * s + 16 * grp + 8) : z8;
+    }
+    if (DM::N32) q[x][2 * DM::N64] = in ? *reinterpret_cast<const bf16x8_t*>(Q + 64 * DM::N64 + 8 * grp) : z8;
+    q16[x] = z8;
+    if (DM::N16 && in) {
+      const bf16x4_t w = *reinterpret_cast<const bf16x4_t*>(Q + DH - 16 + 4 * grp);
+      q16[x] = bf16x8_t{w[0], w[1], w[2], w[3], 0, 0, 0, 0};
+    }
+  }
+  {
+    const int last = min(qt * NC + NC, cols) - 1;
+    lim_wg = sees(a, rq, last / a.G);
+  }
+  const int b0 = piece * sp.chunk, b1 = min(min(b0 + sp.chunk, nb), (lim_wg + BS - 1) / BS);
+  f32x4_t o[NQ][NDT];
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    m[x] = -INFINITY;
+    l[x] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[x][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  const float c1 = a.scale * LOG2E, cap2 = a.cap * LOG2E, ck = a.cap > 0.f ? 2.f * LOG2E * a.scale / a.cap : 0.f;
+  const int* tb = a.table + (long long)r * a.width;
+  int block = b0 + wave < b1 ? tb[b0 + wave] : 0;
+  for (int t = b0 + wave; t < b1; t += 4) {
+    const int cur = __builtin_amdgcn_readfirstlane(block), j0 = t * BS;
+    if (t + 4 < b1) block = tb[t + 4];
+    if (cur < 0 || cur >= a.c.n_blocks) continue;
+    const long long bh = (long long)cur * a.c.Hkv + hk;
+    const uint8_t* kb = a.c.k + bh * BS * DH;
+    const uint8_t* vb = a.c.v + bh * BS * DH;
+    const float ks = a.c.ks[bh], vs = a.c.vs[bh];
+    unsigned kw[4][DM::KW];
+    unsigned vw[NDT][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint8_t* row = kb + (16 * u + l15) * DH;
+#pragma unroll
+      for (int s = 0; s < DM::N64; ++s) {
+        const uint4 w = *reinterpret_cast<const uint4*>(row + 64 * s + 16 * grp);
+        kw[u][4 * s] = w.x;
+        kw[u][4 * s + 1] = w.y;
+        kw[u][4 * s + 2] = w.z;
+        kw[u][4 * s + 3] = w.w;
+      }
+      if (DM::N32) {
+        const uint2 w = *reinterpret_cast<const uint2*>(row + 64 * DM::N64 + 8 * grp);
+        kw[u][4 * DM::N64] = w.x;
+        kw[u][4 * DM::N64 + 1] = w.y;
+      }
+      if (DM::N16) kw[u][DM::KW - 1] = *reinterpret_cast<const unsigned*>(row + DH - 16 + 4 * grp);
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      const uint4 w = *reinterpret_cast<const uint4*>(vb + (16 * dt + l15) * BS + 16 * grp);
+      vw[dt][0] = w.x;
+      vw[dt][1] = w.y;
+      vw[dt][2] = w.z;
+      vw[dt][3] = w.w;
+    }
+    f32x4_t s[NQ][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) s[x][u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        const bf16x8_t k = f8x8_bf16(kw[u][2 * f], kw[u][2 * f + 1], ks);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) s[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[x][f], s[x][u], 0, 0, 0);
+      }
+      if (DM::N16) {
+        const bf16x8_t k = f8x4_frag(kw[u][DM::KW - 1], ks);
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) s[x][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q16[x], s[x][u], 0, 0, 0);
+      }
+    }
+    if (j0 + BS > rq.L) {       // the last block: what stands behind the last token may be anything, and its weight 0 does not silence NaN
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int n = rq.L - j0 - 16 * u - 4 * grp;
+        const unsigned keep = n >= 4 ? 0xffffffffu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) vw[dt][u] &= keep;
+      }
+    }
+    bf16x8_t p[NQ][2];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+      const int lx = lim[x] - j0 - 4 * grp;
+      const float d0 = (float)(pos[x] - j0 - 4 * grp);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float z = s[x][u][e];
+          if (SHAPED) {
+            z = a.cap > 0.f ? __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(ck * z)), cap2) : c1 * z;
+            z = __builtin_fmaf(-sl2[x], fabsf(d0 - (float)(16 * u + e)), z);
+          }
+          z = 16 * u + e < lx ? z : -INFINITY;
+          s[x][u][e] = z;
+          mx = fmaxf(mx, z);
+        }
+      mx = col_max(mx) * (SHAPED ? 1.f : c1);
+      if (__any(mx > m[x] + 8.f)) {               // (as in the tile kernels of attn_var: weights up to 2^8 before the output is rescaled)
+        const float mn = fmaxf(m[x], mx), f = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - mn);
+        m[x] = mn;
+        l[x] *= f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x][dt][e] *= f;
+      }
+      const float mu = m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[x][u][e] = __builtin_amdgcn_exp2f(SHAPED ? s[x][u][e] - mu : __builtin_fmaf(s[x][u][e], c1, -mu));
+          l[x] += s[x][u][e];
+        }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        union { bf16x8_t v; unsigned d[4]; } w;
+        w.d[0] = dmt_pack_bf16(s[x][2 * u][0], s[x][2 * u][1]);
+        w.d[1] = dmt_pack_bf16(s[x][2 * u][2], s[x][2 * u][3]);
+        w.d[2] = dmt_pack_bf16(s[x][2 * u + 1][0], s[x][2 * u + 1][1]);
+        w.d[3] = dmt_pack_bf16(s[x][2 * u + 1][2], s[x][2 * u + 1][3]);
+        p[x][u] = w.v;
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      const bf16x8_t v0 = f8x8_bf16(vw[dt][0], vw[dt][1], vs), v1 = f8x8_bf16(vw[dt][2], vw[dt][3], vs);
+#pragma unroll
+      for (int x = 0; x < NQ; ++x) {
+        o[x][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, p[x][0], o[x][dt], 0, 0, 0);
+        o[x][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, p[x][1], o[x][dt], 0, 0, 0);
+      }
+    }
+  }
+  // the four wavefronts' parts, joined in their order
+#pragma unroll
+  for (int x = 0; x < NQ; ++x) {
+    l[x] = col_sum(l[x]);
+    if (grp == 0) {
+      lm[wave][16 * x + l15] = m[x];
+      ll[wave][16 * x + l15] = l[x];
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) *reinterpret_cast<f32x4_t*>(&lo[wave][(16 * x + l15) * LO + 16 * dt + 4 * grp]) = o[x][dt];
+  }
+  __syncthreads();
+  const long long part = ((long long)item * sp.nqt + qt) * NC;
+  unsigned long long again = 0;
+  for (int y = tid; y < NC * (DH / 8); y += 256) {
+    const int cl = y / (DH / 8), d8 = (y - cl * (DH / 8)) * 8, c = qt * NC + cl;
+    if (c >= cols) continue;
+    float M = fmaxf(fmaxf(lm[0][cl], lm[1][cl]), fmaxf(lm[2][cl], lm[3][cl])), Ls = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lm[w][cl] - mu);
+      Ls = __builtin_fmaf(ll[w][cl], f, Ls);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(lo[w][cl * LO + d8 + e], f, acc[e]);
+    }
+    if (sp.pieces > 1) {
+      float* po = part_o + (part + cl) * DH + d8;
+      *reinterpret_cast<float4*>(po) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      *reinterpret_cast<float4*>(po + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      if (d8 == 0) part_ml[part + cl] = make_float2(M, Ls);
+      continue;
+    }
+    const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+    const int i = c / a.G, h = hk * a.G + c - i * a.G;
+    const long long row = rq.row0 + i;
+    *reinterpret_cast<uint4*>(a.out + row * a.o_rs + (long long)h * DH + d8) =
+        make_uint4(dmt_pack_bf16(acc[0] * inv, acc[1] * inv), dmt_pack_bf16(acc[2] * inv, acc[3] * inv), dmt_pack_bf16(acc[4] * inv, acc[5] * inv),
+                   dmt_pack_bf16(acc[6] * inv, acc[7] * inv));
+    if (a.lse && d8 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
+    float bad = Ls * 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad += acc[e] * 0.f;
+    if (!(bad == 0.f)) again |= 1ull << cl;
+  }
+  if (sp.pieces > 1) return;
+  // columns that came out not finite once more, by what they may see alone
+  __shared__ unsigned long long redo;
+  if (tid == 0) redo = 0;
+  __syncthreads();
+  if (again) atomicOr(&redo, again);
+  __syncthreads();
+  if (redo)
+    for (int cl = wave; cl < NC; cl += 4)
+      if ((redo >> cl) & 1) {
+        const int c = qt * NC + cl, i = c / a.G;
+        kv_row(a, rq, r, hk * a.G + c - i * a.G, i, lo[wave], lane);
+      }
+}
+
+// joins the pieces of a (row, head), in their order; 16 lanes a column
+template <int NQ>
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvArgs a, const Split sp, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
   __shared__ float lds[4][MAX_DH + 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = blockIdx.z, h = blockIdx.y;
-  const Req q = request(a, r);
-  const int i = blockIdx.x * 4 + wave;
-  if (i < q.m) kv_row(a, q, r, h, i, lds[wave], lane);
+  constexpr int NC = 16 * NQ;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, r = blockIdx.z, hk = blockIdx.y, dh = a.c.dh;
+  const Req rq = request(a, r);
+  const int c = blockIdx.x * 16 + (threadIdx.x >> 4), nb = (rq.L + BS - 1) / BS;
+  const bool in = c < rq.m * a.G;
+  if (!__any(in)) return;
+  const int i = in ? c / a.G : 0, h = hk * a.G + (in ? c - i * a.G : 0);
+  const int np = in ? max(1, (nb + sp.chunk - 1) / sp.chunk) : 0;
+  const long long item0 = ((long long)r * a.c.Hkv + hk) * sp.pieces;
+  const auto at = [&](int p) { return ((item0 + p) * sp.nqt + c / NC) * NC + c % NC; };
+  float M = -INFINITY;
+  for (int p = 0; p < np; ++p) M = fmaxf(M, part_ml[at(p)].x);
+  const float mu = M == -INFINITY ? 0.f : M;
+  float Ls = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < np; ++p) {
+    const float2 ml = part_ml[at(p)];
+    const float f = __builtin_amdgcn_exp2f(ml.x - mu);
+    Ls = __builtin_fmaf(ml.y, f, Ls);
+    if (l15 * 8 < dh) {
+      const float* po = part_o + at(p) * dh + l15 * 8;
+      const float4 x = *reinterpret_cast<const float4*>(po), y = *reinterpret_cast<const float4*>(po + 4);
+      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(v[e], f, acc[e]);
+    }
+  }
+  const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
+  const long long row = rq.row0 + i;
+  float bad = Ls * 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bad += acc[e] * 0.f;
+  if (in && l15 * 8 < dh)
+    *reinterpret_cast<uint4*>(a.out + row * a.o_rs + (long long)h * dh + l15 * 8) =
+        make_uint4(dmt_pack_bf16(acc[0] * inv, acc[1] * inv), dmt_pack_bf16(acc[2] * inv, acc[3] * inv), dmt_pack_bf16(acc[4] * inv, acc[5] * inv),
+                   dmt_pack_bf16(acc[6] * inv, acc[7] * inv));
+  if (in && a.lse && l15 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
+  const unsigned long long again = __ballot(in && !(bad == 0.f));
+  for (int g = 0; g < 4; ++g)
+    if ((again >> (16 * g)) & 0xffff) {
+      const int cc = blockIdx.x * 16 + wave * 4 + g, ii = cc / a.G;
+      kv_row(a, rq, r, hk * a.G + cc - ii * a.G, ii, lds[wave], lane);
+    }
+}
+
+// How a call is cut up.  Columns: 16 a tile while a request's rows fit one, else 32 (each conversion of a block then serves twice the columns).
+// Length: enough workgroups to give every compute unit a few, but at least 4 blocks -- one for each wavefront -- a piece; a length that one
+// piece holds needs no joining launch.
+constexpr long long WANT_WG = 1024;
+Split split_of(int n, int Hkv, int G, int max_q, int max_len, int& nq) {
+  Split s;
+  const long long cols = (long long)max_q * G;
+  nq = cols <= 16 ? 1 : 2;
+  s.nqt = (int)cdiv64(cols, 16 * nq);
+  const long long base = (long long)n * Hkv * s.nqt, nb = cdiv64(max_len, BS);
+  long long chunk = cdiv64(nb * base, WANT_WG);
+  if (chunk < 4) chunk = 4;
+  if (chunk > nb) chunk = nb > 0 ? nb : 1;
+  s.chunk = (int)chunk;
+  s.pieces = (int)(nb > 0 ? cdiv64(nb, chunk) : 1);
+  return s;
+}
+
+template <int DH, int NQ> void launch_kv(const KvArgs& a, const Split& s, float* po, float2* ml, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)a.n * a.c.Hkv * s.pieces * s.nqt);
+  if (a.cap > 0.f || a.slopes) kv_tile_kernel<DH, NQ, true><<<grid, 256, 0, st>>>(a, s, po, ml);
+  else kv_tile_kernel<DH, NQ, false><<<grid, 256, 0, st>>>(a, s, po, ml);
+}
+template <int NQ> void launch_kv_dh(const KvArgs& a, const Split& s, float* po, float2* ml, hipStream_t st) {
+  switch (a.c.dh) {
+    case 16: launch_kv<16, NQ>(a, s, po, ml, st); break;
+    case 32: launch_kv<32, NQ>(a, s, po, ml, st); break;
+    case 48: launch_kv<48, NQ>(a, s, po, ml, st); break;
+    case 64: launch_kv<64, NQ>(a, s, po, ml, st); break;
+    case 80: launch_kv<80, NQ>(a, s, po, ml, st); break;
+    case 96: launch_kv<96, NQ>(a, s, po, ml, st); break;
+    case 112: launch_kv<112, NQ>(a, s, po, ml, st); break;
+    default: launch_kv<128, NQ>(a, s, po, ml, st); break;
+  }
 }
 
 bool cache_ok(int Hkv, int dh, int n_blocks, const void* k, const void* v, const float* ks, const float* vs) {
@@ -501,9 +879,19 @@ extern "C" int dmt_kv_read(int32_t Hkv, int32_t dh, int32_t n_blocks, const uint
   return DMT_OK;
 }
 
+static uint64_t kv_ws(const dmt_kv_attn_desc* d, Split* s, int* nq, uint64_t* ml_at) {
+  *s = split_of(d->n, d->Hkv, d->Hq / d->Hkv, d->max_q, d->max_len, *nq);
+  const uint64_t cols = (uint64_t)d->n * d->Hkv * s->pieces * s->nqt * 16 * (uint64_t)*nq;
+  *ml_at = cols * (uint64_t)d->dh * 4;
+  return s->pieces > 1 ? cols * ((uint64_t)d->dh * 4 + 8) : 0;
+}
+
 extern "C" uint64_t dmt_kv_attn_ws_bytes(const dmt_kv_attn_desc* d) {
-  (void)d;
-  return 0;
+  if (!d || d->n <= 0 || d->Hkv <= 0 || d->Hq < d->Hkv || d->max_q <= 0 || d->max_len <= 0 || d->dh <= 0) return 0;
+  Split s;
+  int nq;
+  uint64_t ml;
+  return kv_ws(d, &s, &nq, &ml);
 }
 
 extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
@@ -523,7 +911,23 @@ extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
   a.n = d->n; a.Hq = d->Hq; a.G = d->Hq / d->Hkv; a.max_q = d->max_q; a.max_len = d->max_len; a.width = d->width; a.causal = d->causal != 0;
   a.rows = d->rows; a.Q = (const bf16_t*)d->Q; a.q_rs = d->q_rs; a.table = d->table; a.lens = d->lens; a.row_off = d->row_off;
   a.scale = d->scale; a.cap = d->cap; a.slopes = d->slopes; a.out = (bf16_t*)d->out; a.o_rs = d->o_rs; a.lse = d->lse;
-  kv_rows_kernel<<<dim3((unsigned)cdiv64(a.max_q, 4), a.Hq, a.n), 256, 0, (hipStream_t)stream>>>(a);
-  DMT_CHECK_LAUNCH("dmt_kv_attn(rows)");
+  Split s;
+  int nq;
+  uint64_t ml_at;
+  const uint64_t need = kv_ws(d, &s, &nq, &ml_at);
+  DMT_CHECK_ARG(need == 0 || (d->ws && (uintptr_t)d->ws % 16 == 0 && d->ws_bytes >= need), "dmt_kv_attn: workspace of %llu bytes needed",
+                (unsigned long long)need);
+  DMT_CHECK_ARG((long long)d->n * d->Hkv * s.pieces * s.nqt < (1ll << 31), "dmt_kv_attn: the launch passes 2^31 workgroups");
+  float* po = (float*)d->ws;
+  float2* ml = need ? (float2*)((char*)d->ws + ml_at) : nullptr;
+  if (nq == 1) launch_kv_dh<1>(a, s, po, ml, (hipStream_t)stream);
+  else launch_kv_dh<2>(a, s, po, ml, (hipStream_t)stream);
+  DMT_CHECK_LAUNCH(s.pieces > 1 ? "dmt_kv_attn(pieces)" : "dmt_kv_attn");
+  if (s.pieces > 1) {
+    const dim3 grid((unsigned)cdiv64((long long)a.max_q * a.G, 16), a.c.Hkv, a.n);
+    if (nq == 1) kv_join_kernel<1><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, po, ml);
+    else kv_join_kernel<2><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, po, ml);
+    DMT_CHECK_LAUNCH("dmt_kv_attn(join)");
+  }
   return DMT_OK;
 }
