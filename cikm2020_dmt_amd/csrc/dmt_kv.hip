@@ -718,58 +718,86 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
       }
 }
 
-// joins the pieces of a (row, head), in their order; 16 lanes a column
+// Joins the pieces of a (row, head), in their order: 16 lanes a column and 8 dims a lane; with many pieces `gpc` such groups take every
+// gpc-th piece of one column and meet in LDS (one group alone would wait for one piece after the other: 400 of them took 230 us).
 template <int NQ>
-__global__ __launch_bounds__(256) void kv_join_kernel(const KvArgs a, const Split sp, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
-  __shared__ float lds[4][MAX_DH + 64];
+__global__ __launch_bounds__(256) void kv_join_kernel(const KvArgs a, const Split sp, int gpc, const float* __restrict__ part_o,
+                                                      const float2* __restrict__ part_ml) {
+  __shared__ __attribute__((aligned(16))) float lo[16][MAX_DH];
+  __shared__ float lm[16], ll[16];
   constexpr int NC = 16 * NQ;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, r = blockIdx.z, hk = blockIdx.y, dh = a.c.dh;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, grp = threadIdx.x >> 4, r = blockIdx.z, hk = blockIdx.y, dh = a.c.dh;
   const Req rq = request(a, r);
-  const int c = blockIdx.x * 16 + (threadIdx.x >> 4), nb = (rq.L + BS - 1) / BS;
+  const int per = 16 / gpc, c = blockIdx.x * per + grp / gpc, g0 = grp % gpc, nb = (rq.L + BS - 1) / BS;
+  if ((int)blockIdx.x * per >= rq.m * a.G) return;
   const bool in = c < rq.m * a.G;
-  if (!__any(in)) return;
   const int i = in ? c / a.G : 0, h = hk * a.G + (in ? c - i * a.G : 0);
   const int np = in ? max(1, (nb + sp.chunk - 1) / sp.chunk) : 0;
   const long long item0 = ((long long)r * a.c.Hkv + hk) * sp.pieces;
-  const auto at = [&](int p) { return ((item0 + p) * sp.nqt + c / NC) * NC + c % NC; };
-  float M = -INFINITY;
-  for (int p = 0; p < np; ++p) M = fmaxf(M, part_ml[at(p)].x);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float Ls = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < np; ++p) {
-    const float2 ml = part_ml[at(p)];
-    const float f = __builtin_amdgcn_exp2f(ml.x - mu);
-    Ls = __builtin_fmaf(ml.y, f, Ls);
+  float M = -INFINITY, Ls = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = g0; p < np; p += gpc) {
+    const long long at = ((item0 + p) * sp.nqt + c / NC) * NC + c % NC;
+    const float2 ml = part_ml[at];
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (l15 * 8 < dh) {
-      const float* po = part_o + at(p) * dh + l15 * 8;
+      const float* po = part_o + at * dh + l15 * 8;
       const float4 x = *reinterpret_cast<const float4*>(po), y = *reinterpret_cast<const float4*>(po + 4);
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(v[e], f, acc[e]);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
     }
+    const float mn = fmaxf(M, ml.x), mu = mn == -INFINITY ? 0.f : mn;
+    const float f0 = __builtin_amdgcn_exp2f(M - mu), f1 = __builtin_amdgcn_exp2f(ml.x - mu);
+    M = mn;
+    Ls = __builtin_fmaf(Ls, f0, ml.y * f1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(acc[e], f0, v[e] * f1);
   }
+  if (gpc > 1) {
+    if (l15 == 0) { lm[grp] = M; ll[grp] = Ls; }
+    *reinterpret_cast<float4*>(&lo[grp][l15 * 8]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&lo[grp][l15 * 8 + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    __syncthreads();
+    if (g0 == 0) {
+      M = -INFINITY;
+      for (int g = 0; g < gpc; ++g) M = fmaxf(M, lm[grp + g]);
+      const float mu = M == -INFINITY ? 0.f : M;
+      Ls = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      for (int g = 0; g < gpc; ++g) {
+        const float f = __builtin_amdgcn_exp2f(lm[grp + g] - mu);
+        Ls = __builtin_fmaf(ll[grp + g], f, Ls);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = __builtin_fmaf(lo[grp + g][l15 * 8 + e], f, acc[e]);
+      }
+    }
+    __syncthreads();
+  }
+  const bool mine = in && g0 == 0;
   const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
   const long long row = rq.row0 + i;
   float bad = Ls * 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) bad += acc[e] * 0.f;
-  if (in && l15 * 8 < dh)
+  if (mine && l15 * 8 < dh)
     *reinterpret_cast<uint4*>(a.out + row * a.o_rs + (long long)h * dh + l15 * 8) =
         make_uint4(dmt_pack_bf16(acc[0] * inv, acc[1] * inv), dmt_pack_bf16(acc[2] * inv, acc[3] * inv), dmt_pack_bf16(acc[4] * inv, acc[5] * inv),
                    dmt_pack_bf16(acc[6] * inv, acc[7] * inv));
-  if (in && a.lse && l15 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
-  const unsigned long long again = __ballot(in && !(bad == 0.f));
+  if (mine && a.lse && l15 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
+  const unsigned long long again = __ballot(mine && !(bad == 0.f));
   for (int g = 0; g < 4; ++g)
     if ((again >> (16 * g)) & 0xffff) {
-      const int cc = blockIdx.x * 16 + wave * 4 + g, ii = cc / a.G;
-      kv_row(a, rq, r, hk * a.G + cc - ii * a.G, ii, lds[wave], lane);
+      const int cc = blockIdx.x * per + (wave * 4 + g) / gpc, ii = cc / a.G;
+      kv_row(a, rq, r, hk * a.G + cc - ii * a.G, ii, lo[wave * 4], lane);
     }
 }
 
 // How a call is cut up.  Columns: 16 a tile while a request's rows fit one, else 32 (each conversion of a block then serves twice the columns).
-// Length: enough workgroups to give every compute unit a few, but at least 4 blocks -- one for each wavefront -- a piece; a length that one
-// piece holds needs no joining launch.
-constexpr long long WANT_WG = 1024;
+// Length: 512 workgroups -- two for each compute unit -- but at least 4 blocks, one for each wavefront, a piece; a length that one piece holds
+// needs no joining launch.  (64 ragged requests of up to 8192 tokens, 8 key heads: 120 us in 512 whole-length workgroups, 130 us in 1024 and
+// more pieces; one of 100001 tokens, 2 key heads: 21 us at 512, 24 us at 1024; 16 x 300 candidates over 1000 tokens: 23 against 34 us.)
+
+constexpr long long WANT_WG = 512;
 Split split_of(int n, int Hkv, int G, int max_q, int max_len, int& nq) {
   Split s;
   const long long cols = (long long)max_q * G;
@@ -924,9 +952,10 @@ extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
   else launch_kv_dh<2>(a, s, po, ml, (hipStream_t)stream);
   DMT_CHECK_LAUNCH(s.pieces > 1 ? "dmt_kv_attn(pieces)" : "dmt_kv_attn");
   if (s.pieces > 1) {
-    const dim3 grid((unsigned)cdiv64((long long)a.max_q * a.G, 16), a.c.Hkv, a.n);
-    if (nq == 1) kv_join_kernel<1><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, po, ml);
-    else kv_join_kernel<2><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, po, ml);
+    const int gpc = s.pieces <= 4 ? 1 : (s.pieces <= 16 ? 4 : 16);
+    const dim3 grid((unsigned)cdiv64((long long)a.max_q * a.G, 16 / gpc), a.c.Hkv, a.n);
+    if (nq == 1) kv_join_kernel<1><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, gpc, po, ml);
+    else kv_join_kernel<2><<<grid, 256, 0, (hipStream_t)stream>>>(a, s, gpc, po, ml);
     DMT_CHECK_LAUNCH("dmt_kv_attn(join)");
   }
   return DMT_OK;
