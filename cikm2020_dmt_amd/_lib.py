@@ -143,7 +143,7 @@ class AttnVarDesc(C.Structure):
                 ("q_off", c_vp), ("q_lens", c_vp), ("k_off", c_vp), ("k_lens", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32),
                 ("slopes", c_vp), ("prefix", c_vp), ("q_doc", c_vp), ("k_doc", c_vp), ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp),
                 ("dout", c_vp), ("do_rs", c_i64), ("dQ", c_vp), ("dq_rs", c_i64), ("dK", c_vp), ("dk_rs", c_i64),
-                ("dV", c_vp), ("dv_rs", c_i64), ("dslopes", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
+                ("dV", c_vp), ("dv_rs", c_i64), ("dslopes", c_vp), ("doc_ranges", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
 
 
 class KvAttnDesc(C.Structure):
@@ -242,7 +242,7 @@ _SIGS = {
 
 EXPORTED_SYMBOLS = sorted(list(_SIGS.keys()) + ["dmt_last_error", "dmt_version", "dmt_build_arch", "dmt_ln_bwd_partials", "dmt_struct_size", "dmt_chain_supported", "dmt_proj_supported", "dmt_image_job_bytes",
                                                  "dmt_attn_long_supported", "dmt_mmoe_experts_supported", "dmt_mmoe_experts_ws_bytes", "dmt_heads_supported", "dmt_q1mem_supported", "dmt_reduce_det_ws_bytes", "dmt_wgrad320_det_ws_bytes", "dmt_route_trace", "dmt_route_count", "dmt_route_dump",
-                                                 "dmt_attn_var_supported", "dmt_attn_var_ws_bytes", "dmt_kv_plan_ws_bytes", "dmt_kv_attn_ws_bytes"])
+                                                 "dmt_attn_var_supported", "dmt_attn_var_ws_bytes", "dmt_attn_var_doc_bytes", "dmt_kv_plan_ws_bytes", "dmt_kv_attn_ws_bytes"])
 
 _lib = None
 
@@ -301,7 +301,9 @@ def load():
     lib.dmt_attn_var_supported.restype = c_i32
     lib.dmt_attn_var_supported.argtypes = [c_i32] * 4
     lib.dmt_attn_var_ws_bytes.restype = C.c_uint64
-    lib.dmt_attn_var_ws_bytes.argtypes = [C.POINTER(AttnVarDesc), c_i32]
+    lib.dmt_attn_var_ws_bytes.argtypes = [C.POINTER(AttnVarDesc)]
+    lib.dmt_attn_var_doc_bytes.restype = C.c_uint64
+    lib.dmt_attn_var_doc_bytes.argtypes = [c_i32] * 3
     lib.dmt_kv_plan_ws_bytes.restype = C.c_uint64
     lib.dmt_kv_plan_ws_bytes.argtypes = [c_i32]
     lib.dmt_kv_attn_ws_bytes.restype = C.c_uint64

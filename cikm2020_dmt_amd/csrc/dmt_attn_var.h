@@ -34,7 +34,9 @@ struct Args {
   float* dslopes;
   float* D;                         // [rows_q, Hq]: rowsum(dout * out)
   float* slope_part;                // [Hq][B * ceil(max_q / 128)]
-  const int2* q_rng; const int2* k_rng;   // (least, largest) document id of every 64-row tile: [B][ceil(max / 64)]
+  int parts;                        // dK, dV: the heads of a group in so many pieces, summed by a launch of their own
+  float* part_k; float* part_v;     // [parts][rows_k][Hkv * dh] when parts > 1
+  int2* q_rng; int2* k_rng;         // (least, largest) document id of every 64-row tile: [B][ceil(max / 64)]
   int nqt, nkt;                     // 64-row tiles of max_q, max_k
 };
 
@@ -176,7 +178,7 @@ __device__ __forceinline__ float slope_part(float s0, float s1, float s2, float 
   return i * __builtin_fmaf(s0 * i, s2, -s1);
 }
 template <typename T>
-__device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, int lane) {
+__device__ float row_dq(const Args& a, const Ex& e, int h, int i, float D, float* lds, int lane) {
   float* q = lds;
   float* g = lds + MAX_DH;
   float* xl = lds + 2 * MAX_DH;
@@ -191,7 +193,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, in
   lds_fence();
   const Shape s = shape_of(a, h);
   const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
-  const float lse2 = a.lse[row * a.Hq + h] * LOG2E, D = a.D[row * a.Hq + h];
+  const float lse2 = a.lse[row * a.Hq + h] * LOG2E;
   float o0 = 0.f, o1 = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
   for (int j0 = 0; j0 < e.kl; j0 += 64) {
     const int j = j0 + lane;
@@ -231,9 +233,10 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float* lds, in
   return slope_part(wave_sum(s0), wave_sum(s1), wave_sum(s2), wave_sum(sp));
 }
 
-// dk and dv of one key row: over the query heads of its group, then over the queries
+// dk and dv of one key row: over the query heads of its group (those of one part), then over the queries
+__device__ __forceinline__ int part_head(const Args& a, int part) { return (int)((long long)a.G * part / a.parts); }
 template <typename T>
-__device__ void row_dkv(const Args& a, const Ex& e, int hk, int j, float* lds, int lane) {
+__device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int j, float* lds, int lane) {
   float* k = lds;
   float* v = lds + MAX_DH;
   float* pl = lds + 2 * MAX_DH;
@@ -246,7 +249,7 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int j, float* lds, i
   }
   lds_fence();
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int h = hk * a.G; h < hk * a.G + a.G; ++h) {
+  for (int h = hk * a.G + part_head(a, part); h < hk * a.G + part_head(a, part + 1); ++h) {
     const Shape s = shape_of(a, h);
     const T* Q = (const T*)a.Q + e.q0 * a.q_rs + (long long)h * dh;
     const T* O = (const T*)a.dout + e.q0 * a.do_rs + (long long)h * dh;
@@ -285,6 +288,12 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int j, float* lds, i
       }
       lds_fence();
     }
+  }
+  if (a.parts > 1) {
+    const long long at = (((long long)part * a.rows_k + row) * a.Hkv + hk) * dh;
+    if (lane < dh) { a.part_k[at + lane] = k0; a.part_v[at + lane] = v0; }
+    if (lane + 64 < dh) { a.part_k[at + lane + 64] = k1; a.part_v[at + lane + 64] = v1; }
+    return;
   }
   T* dk = (T*)a.dK + row * a.dk_rs + (long long)hk * dh;
   T* dv = (T*)a.dV + row * a.dv_rs + (long long)hk * dh;
@@ -331,6 +340,11 @@ template <int DHP> struct Tile<bf16_t, DHP> {
     return *reinterpret_cast<const bf16x8_t*>(X + row * rs + 16 * s + 8 * half);
   }
   static __device__ __forceinline__ int col(int s, int half) { return 16 * s + 8 * half; }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_fmaf(bf2f((bf16_t)a[e]), bf2f((bf16_t)b[e]), c);
+    return c;
+  }
   static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -364,6 +378,11 @@ template <int DHP> struct Tile<float, DHP> {
     return *reinterpret_cast<const f32x4_t*>(X + row * rs + 8 * s + 4 * half);
   }
   static __device__ __forceinline__ int col(int s, int half) { return 8 * s + 4 * half; }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_fmaf(a[e], b[e], c);
+    return c;
+  }
   static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, f32x16_t c) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
@@ -477,4 +496,3 @@ __device__ __forceinline__ void place(int id, int heads, int nt, bool last_first
 }  // namespace attn_var
 
 int dmt_attn_var_args(const dmt_attn_var_desc* d, attn_var::Args* a, bool backward, const char* what);
-int dmt_attn_var_doc_ranges(const attn_var::Args& a, void* stream);

@@ -187,18 +187,21 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     if ((again >> r) & 1) row_fwd<T>(a, e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
-__global__ void doc_ranges_kernel(const int* off, const int* lens, const int* doc, int most, long long rows, int nt, int B, int2* out) {
-  const int t = blockIdx.x * blockDim.y + threadIdx.y, b = blockIdx.y, lane = threadIdx.x;
+// (least, largest) document id of every 64 rows, of the queries (blockIdx.z = 0) and of the keys: tiles that share no id are skipped, tiles of
+// one id need no mask
+__global__ __launch_bounds__(256) void doc_ranges_kernel(const Args a) {
+  const bool keys = blockIdx.z == 1;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y, lane = threadIdx.x & 63, nt = keys ? a.nkt : a.nqt;
   if (t >= nt) return;
-  const int len = clip_len(lens[b], most, off[b], rows);
-  const int i = t * 64 + lane;
+  const Ex e = example(a, b);
+  const int i = t * 64 + lane, len = keys ? e.kl : e.ql;
   int lo = 0x7fffffff, hi = -0x7fffffff - 1;
-  if (i < len) lo = hi = doc[(long long)off[b] + i];
+  if (i < len) lo = hi = keys ? a.k_doc[e.k0 + i] : a.q_doc[e.q0 + i];
   for (int s = 32; s; s >>= 1) {
     lo = min(lo, __shfl_xor(lo, s));
     hi = max(hi, __shfl_xor(hi, s));
   }
-  if (lane == 0) out[(long long)b * nt + t] = make_int2(lo, hi);
+  if (lane == 0) (keys ? a.k_rng : a.q_rng)[(long long)b * nt + t] = make_int2(lo, hi);
 }
 
 template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
@@ -227,28 +230,40 @@ extern "C" int dmt_attn_var_supported(int32_t dtype, int32_t dh, int32_t Hq, int
 }
 
 namespace {
-struct WsLayout { uint64_t qr, kr, D, sp, total; };
-WsLayout ws_layout(const dmt_attn_var_desc* d, bool backward) {
-  const uint64_t nqt = (uint64_t)cdiv64(d->max_q, 64), nkt = (uint64_t)cdiv64(d->max_k, 64);
+// dK, dV: the query heads of a group run one after the other in a workgroup, unless that leaves fewer than four workgroups a compute unit: then
+// they are cut into pieces that run side by side and leave fp32 sums to be added in their order.
+constexpr int64_t WANT_WG = 1024;
+int parts_of(const dmt_attn_var_desc* d) {
+  const int64_t G = d->Hq / d->Hkv, base = (int64_t)d->B * d->Hkv * cdiv64(d->max_k, 128);
+  const int64_t p = base > 0 ? cdiv64(WANT_WG, base) : 1;
+  return (int)(p < G ? p : G);
+}
+struct WsLayout { uint64_t D, sp, pk, pv, total; };
+WsLayout ws_layout(const dmt_attn_var_desc* d) {
   WsLayout w;
   uint64_t at = 0;
-  w.qr = at;
-  if (d->q_doc) at += up16(8 * nqt * (uint64_t)d->B);
-  w.kr = at;
-  if (d->q_doc) at += up16(8 * nkt * (uint64_t)d->B);
   w.D = at;
-  if (backward) at += up16(4 * (uint64_t)d->rows_q * (uint64_t)d->Hq);
+  at += up16(4 * (uint64_t)d->rows_q * (uint64_t)d->Hq);
   w.sp = at;
-  if (backward && d->dslopes) at += up16(4 * (uint64_t)d->Hq * (uint64_t)d->B * (uint64_t)cdiv64(d->max_q, 128));
-  w.total = at;
+  if (d->dslopes) at += up16(4 * (uint64_t)d->Hq * (uint64_t)d->B * (uint64_t)cdiv64(d->max_q, 128));
+  const int parts = parts_of(d);
+  const uint64_t part = parts > 1 ? up16(4 * (uint64_t)parts * (uint64_t)d->rows_k * (uint64_t)d->Hkv * (uint64_t)d->dh) : 0;
+  w.pk = at;
+  at += part;
+  w.pv = at;
+  w.total = at + part;
   return w;
 }
 bool al16(const void* p, int64_t rs, int es) { return ((uintptr_t)p % 16) == 0 && (rs * es) % 16 == 0; }
 }  // namespace
 
-extern "C" uint64_t dmt_attn_var_ws_bytes(const dmt_attn_var_desc* d, int32_t backward) {
-  if (!d || d->B <= 0 || d->max_q <= 0 || d->max_k <= 0) return 0;
-  return ws_layout(d, backward != 0).total;
+extern "C" uint64_t dmt_attn_var_ws_bytes(const dmt_attn_var_desc* d) {
+  if (!d || d->B <= 0 || d->max_q < 0 || d->max_k < 0 || d->Hkv <= 0 || d->Hq < d->Hkv || d->dh <= 0 || d->rows_q < 0 || d->rows_k < 0) return 0;
+  return ws_layout(d).total;
+}
+extern "C" uint64_t dmt_attn_var_doc_bytes(int32_t B, int32_t max_q, int32_t max_k) {
+  if (B <= 0 || max_q < 0 || max_k < 0) return 0;
+  return up16(8 * (uint64_t)B * (uint64_t)cdiv64(max_q, 64)) + up16(8 * (uint64_t)B * (uint64_t)cdiv64(max_k, 64));
 }
 
 int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const char* what) {
@@ -285,9 +300,13 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
                   "%s: gradient rows must be 16-byte aligned", what);
     DMT_CHECK_ARG(!d->dslopes || d->slopes, "%s: dslopes without slopes", what);
   }
-  const WsLayout w = ws_layout(d, backward);
-  DMT_CHECK_ARG(w.total == 0 || (d->ws && ((uintptr_t)d->ws % 16) == 0 && d->ws_bytes >= w.total), "%s: workspace of %llu bytes needed", what,
-                (unsigned long long)w.total);
+  DMT_CHECK_ARG(!d->q_doc || (d->doc_ranges && ((uintptr_t)d->doc_ranges % 16) == 0), "%s: documents need doc_ranges (16-byte aligned)", what);
+  WsLayout w = {0, 0, 0, 0, 0};
+  if (backward) {
+    w = ws_layout(d);
+    DMT_CHECK_ARG(w.total == 0 || (d->ws && ((uintptr_t)d->ws % 16) == 0 && d->ws_bytes >= w.total), "%s: workspace of %llu bytes needed", what,
+                  (unsigned long long)w.total);
+  }
   char* ws = (char*)d->ws;
   a->B = d->B; a->Hq = d->Hq; a->Hkv = d->Hkv; a->dh = d->dh; a->G = d->Hq / d->Hkv;
   a->max_q = d->max_q; a->max_k = d->max_k; a->rows_q = d->rows_q; a->rows_k = d->rows_k;
@@ -300,19 +319,13 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   a->dslopes = d->dslopes;
   a->nqt = (int)cdiv64(d->max_q, 64);
   a->nkt = (int)cdiv64(d->max_k, 64);
-  a->q_rng = d->q_doc ? (const int2*)(ws + w.qr) : nullptr;
-  a->k_rng = d->q_doc ? (const int2*)(ws + w.kr) : nullptr;
+  a->q_rng = (int2*)d->doc_ranges;
+  a->k_rng = d->q_doc ? (int2*)((char*)d->doc_ranges + up16(8 * (uint64_t)d->B * (uint64_t)a->nqt)) : nullptr;
   a->D = backward ? (float*)(ws + w.D) : nullptr;
   a->slope_part = backward && d->dslopes ? (float*)(ws + w.sp) : nullptr;
-  return DMT_OK;
-}
-
-int dmt_attn_var_doc_ranges(const Args& a, void* stream) {
-  if (!a.q_doc) return DMT_OK;
-  hipStream_t st = (hipStream_t)stream;
-  if (a.nqt) doc_ranges_kernel<<<dim3((a.nqt + 3) / 4, a.B), dim3(64, 4), 0, st>>>(a.q_off, a.q_lens, a.q_doc, a.max_q, a.rows_q, a.nqt, a.B, (int2*)a.q_rng);
-  if (a.nkt) doc_ranges_kernel<<<dim3((a.nkt + 3) / 4, a.B), dim3(64, 4), 0, st>>>(a.k_off, a.k_lens, a.k_doc, a.max_k, a.rows_k, a.nkt, a.B, (int2*)a.k_rng);
-  DMT_CHECK_LAUNCH("dmt_attn_var(doc ranges)");
+  a->parts = backward ? parts_of(d) : 1;
+  a->part_k = backward ? (float*)(ws + w.pk) : nullptr;
+  a->part_v = backward ? (float*)(ws + w.pv) : nullptr;
   return DMT_OK;
 }
 
@@ -320,7 +333,10 @@ extern "C" int dmt_attn_var_fwd(const dmt_attn_var_desc* d, void* stream) {
   Args a;
   const int rc = dmt_attn_var_args(d, &a, false, "dmt_attn_var_fwd");
   if (rc) return rc < 0 ? rc : DMT_OK;
-  const int rr = dmt_attn_var_doc_ranges(a, stream);
-  if (rr) return rr;
+  if (a.q_doc) {
+    const int nt = a.nqt > a.nkt ? a.nqt : a.nkt;
+    doc_ranges_kernel<<<dim3((nt + 3) / 4, a.B, 2), 256, 0, (hipStream_t)stream>>>(a);
+    DMT_CHECK_LAUNCH("dmt_attn_var_fwd(document ranges)");
+  }
   return d->dtype == DMT_F32 ? launch_fwd<float>(a, (hipStream_t)stream) : launch_fwd<bf16_t>(a, (hipStream_t)stream);
 }

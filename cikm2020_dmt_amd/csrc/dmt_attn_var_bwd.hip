@@ -6,25 +6,6 @@ using namespace attn_var;
 
 namespace {
 
-// D[row, h] = sum_c dout[row, h, c] out[row, h, c]; a row per 16 lanes
-template <typename T>
-__global__ __launch_bounds__(256) void rowsum_kernel(const Args a) {
-  const long long item = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int l16 = threadIdx.x & 15;
-  if (item >= a.rows_q * a.Hq) return;
-  const long long row = item / a.Hq;
-  const int h = (int)(item - row * a.Hq);
-  const T* g = (const T*)a.dout + row * a.do_rs + (long long)h * a.dh;
-  float s = 0.f;
-  const T* o = (const T*)a.out + row * a.o_rs + (long long)h * a.dh;
-  for (int c = l16; c < a.dh; c += 16) s = __builtin_fmaf(ldf<T>(g + c), ldf<T>(o + c), s);
-  s += __shfl_xor(s, 8);
-  s += __shfl_xor(s, 4);
-  s += __shfl_xor(s, 2);
-  s += __shfl_xor(s, 1);
-  if (l16 == 0) a.D[item] = s;
-}
-
 // The scores of one 32 x 32 tile, in place: z2 (the row's statistic is subtracted by the caller).  d0: distance of register row 0 and the lane's
 // column; STEP: what a register row adds to it.
 template <int STEP>
@@ -45,7 +26,7 @@ __device__ __forceinline__ void shaped(f32x16_t& s, f32x16_t& r2, const Shape& s
   }
 }
 
-// dQ: one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
+// dQ (and D): one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
 template <typename T, int DHP, bool SHAPED>
 __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
@@ -74,7 +55,16 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, i, half);
   const long long stat = (e.q0 + (in ? i : 0)) * a.Hq + h;
   // (a row that sees nothing: lse = -inf; its weights 2^(z - inf) are 0)
-  const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY, D = in ? a.D[stat] : 0.f;
+  const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY;
+  float D = 0.f;                                         // rowsum(dout * out), for this kernel and the next
+  {
+    typename TL::Frag ov[TL::NS];
+    own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, i, half);
+#pragma unroll
+    for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
+    D += other_half(D);
+    if (in && half == 0) a.D[stat] = D;
+  }
   const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
@@ -208,7 +198,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     if (half) sl = 0.f;                                  // (both halves hold the row's)
     sl = wave_sum(sl);
     for (int r = 0; r < 32; ++r)
-      if ((again >> r) & 1) sl += row_dq<T>(a, e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
+      if ((again >> r) & 1) sl += row_dq<T>(a, e, h, iw + r, __shfl(D, r), (float*)lds + wave * ROW_LDS, lane);
   }
   if (a.slope_part) {
     if (lane == 0) part[wave] = sl;
@@ -217,10 +207,23 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   }
 }
 
+// dslopes[h] += sum of its parts, in their order (64 bits: the terms cancel)
+__device__ void sum_slopes(const float* part, long long n, float* out, double* red) {
+  double s = 0.0;
+  for (long long i = threadIdx.x; i < n; i += 256) s += (double)part[i];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int w = 128; w; w >>= 1) {
+    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *out += (float)red[0];
+}
+
 // dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
 // tiles of 64: S and dP with lane = key, P and dX packed are the B operands of dV^T += dO^T P and dK^T += Q^T dX.  Nothing crosses wavefronts.
 template <typename T, int DHP, bool SHAPED>
-__global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv_kernel(const Args a, int nt) {
+__global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv_kernel(const Args a, int nt, int nqt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
   constexpr int QE = KT * TL::RS + 32;
@@ -229,9 +232,16 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   __shared__ __attribute__((aligned(16))) float stats[NB][2][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
+  const int id = (int)blockIdx.x - (SHAPED && a.slope_part ? a.Hq : 0);
+  if (SHAPED && id < 0) {                                 // the first workgroups finish the slopes' gradient that the dQ kernel left in parts
+    const long long n = (long long)a.B * nqt;
+    sum_slopes(a.slope_part + (long long)blockIdx.x * n, n, a.dslopes + blockIdx.x, (double*)lds);
+    return;
+  }
   int head, kt;
-  place(blockIdx.x, a.B * a.Hkv, nt, false, head, kt);
-  const int b = head / a.Hkv, hk = head - b * a.Hkv;
+  place(id, a.B * a.Hkv * a.parts, nt, false, head, kt);
+  const int part = head % a.parts, b = head / (a.parts * a.Hkv), hk = head / a.parts - b * a.Hkv;
+  const int g0 = part_head(a, part), ng = part_head(a, part + 1) - g0;
   const Ex e = example(a, b);
   if (kt * 128 >= e.kl) return;
   const int jw = kt * 128 + wave * 32, j = jw + l31;
@@ -244,7 +254,7 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   const int lo_wg = a.causal && kt * 128 >= e.pre ? max(0, kt * 128 - e.off) : 0;
   const int lo_w = a.causal && jw >= e.pre ? max(0, jw - e.off) : 0;
   const int lo_l = j >= e.kl ? 0x7fffffff : (a.causal && j >= e.pre ? max(0, j - e.off) : 0);
-  const int t0 = lo_wg / KT, nq = (e.ql + KT - 1) / KT, per = nq > t0 ? nq - t0 : 0, total = per * a.G;
+  const int t0 = lo_wg / KT, nq = (e.ql + KT - 1) / KT, per = nq > t0 ? nq - t0 : 0, total = per * ng;
   const bool free_keys = jw < e.pre;                      // some key of the wavefront is in the prefix: no document hides it
   int klo = 0, khi = 0, wlo = 0, whi = 0, kd_l = 0;
   const int2* qr = nullptr;
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   int qd = 0;
   float lse2 = 0.f;
   const auto request = [&](int n) {
-    const int h = hk * a.G + n / per, i0 = (t0 + n % per) * KT;
+    const int h = hk * a.G + g0 + n / per, i0 = (t0 + n % per) * KT;
     st.request((const T*)a.Q + (e.q0 + i0) * a.q_rs + (long long)h * a.dh, a.q_rs, (const T*)a.dout + (e.q0 + i0) * a.do_rs + (long long)h * a.dh, a.do_rs,
                min(KT, e.ql - i0), a.dh);
     if (tid < 2 * KT) {
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
     if (nn < total) request(nn);
     const T* Ql = lds + buf * 2 * QE;
     const T* Gl = Ql + QE;
-    const Shape sh = shape_of(a, hk * a.G + n / per);
+    const Shape sh = shape_of(a, hk * a.G + g0 + n / per);
     bool work = active && i0 + KT > lo_w, docs_differ = false;
     if (qr) {
       if (!free_keys && (qr[tq].x > whi || qr[tq].y < wlo)) work = false;
@@ -368,7 +378,14 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   float bad = 0.f;
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(dk[dt], dt, half, a.dh) + not_finite(dv[dt], dt, half, a.dh);
-  if (in) {
+  if (in && a.parts > 1) {
+    const long long at = (((long long)part * a.rows_k + e.k0 + j) * a.Hkv + hk) * a.dh;
+#pragma unroll
+    for (int dt = 0; dt < TL::NDT; ++dt) {
+      store_dims<float>(dk[dt], 1.f, a.part_k + at, dt, half, a.dh);
+      store_dims<float>(dv[dt], 1.f, a.part_v + at, dt, half, a.dh);
+    }
+  } else if (in) {
     T* pk = (T*)a.dK + (e.k0 + j) * a.dk_rs + (long long)hk * a.dh;
     T* pv = (T*)a.dV + (e.k0 + j) * a.dv_rs + (long long)hk * a.dh;
 #pragma unroll
@@ -380,22 +397,30 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   unsigned long long again = __ballot(in && !(bad == 0.f));
   again |= again >> 32;
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_dkv<T>(a, e, hk, jw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1) row_dkv<T>(a, e, hk, part, jw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
-// dslopes[h] += sum of its parts, in their order (64 bits: the terms cancel)
-__global__ __launch_bounds__(256) void slopes_kernel(const float* part, long long n, float* out) {
-  __shared__ double red[256];
-  const float* p = part + (long long)blockIdx.x * n;
-  double s = 0.0;
-  for (long long i = threadIdx.x; i < n; i += 256) s += (double)p[i];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  for (int w = 128; w; w >>= 1) {
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
-    __syncthreads();
+// dK = scale (sum of its parts), dV = sum of its parts, in their order: 16 key rows of one example a workgroup
+template <typename T>
+__global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
+  const Ex e = example(a, blockIdx.y);
+  const int w = a.Hkv * a.dh, c4 = w / 4, j0 = blockIdx.x * 16;
+  const int rows = e.kl - j0 < 16 ? e.kl - j0 : 16;
+  for (int x = threadIdx.x; x < rows * c4 * 2; x += 256) {
+    const bool is_v = x >= rows * c4;
+    const int y = is_v ? x - rows * c4 : x, r = y / c4, c = (y - r * c4) * 4;
+    const long long row = e.k0 + j0 + r;
+    const float* p = (is_v ? a.part_v : a.part_k) + row * w + c;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < a.parts; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(p + (long long)i * a.rows_k * w);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
+    const float f = is_v ? 1.f : a.scale;
+    T* o = is_v ? (T*)a.dV + row * a.dv_rs + c : (T*)a.dK + row * a.dk_rs + c;
+    if (sizeof(T) == 2) *reinterpret_cast<uint2*>(o) = make_uint2(dmt_pack_bf16(s.x * f, s.y * f), dmt_pack_bf16(s.z * f, s.w * f));
+    else *reinterpret_cast<float4*>(o) = make_float4(s.x * f, s.y * f, s.z * f, s.w * f);
   }
-  if (threadIdx.x == 0) out[blockIdx.x] += (float)red[0];
 }
 
 template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t st) {
@@ -403,36 +428,34 @@ template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t
   if (a.cap > 0.f || a.slopes) tile_dq_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
   else tile_dq_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
 }
-template <typename T, int DHP> void launch_dkv(const Args& a, int nt, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B);
-  if (a.cap > 0.f || a.slopes) tile_dkv_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
-  else tile_dkv_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts + (a.slope_part ? a.Hq : 0));
+  if (a.cap > 0.f || a.slopes) tile_dkv_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt, nqt);
+  else tile_dkv_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt, nqt);
 }
 
 template <typename T>
-int launch_bwd(const Args& a, hipStream_t st) {
-  const long long items = a.rows_q * a.Hq;
-  if (items && a.max_q) {
-    rowsum_kernel<T><<<(unsigned)cdiv64(items, 16), 256, 0, st>>>(a);
-    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(row sums)");
-    const int nt = (int)cdiv64(a.max_q, 128);
-    if (a.dh <= 32) launch_dq<T, 32>(a, nt, st);
-    else if (a.dh <= 64) launch_dq<T, 64>(a, nt, st);
-    else if (a.dh <= 80) launch_dq<T, 80>(a, nt, st);
-    else launch_dq<T, 128>(a, nt, st);
+int launch_bwd(Args a, hipStream_t st) {
+  const int nqt = (int)cdiv64(a.max_q, 128), nkt = (int)cdiv64(a.max_k, 128);
+  if (a.rows_q && nqt) {
+    if (a.dh <= 32) launch_dq<T, 32>(a, nqt, st);
+    else if (a.dh <= 64) launch_dq<T, 64>(a, nqt, st);
+    else if (a.dh <= 80) launch_dq<T, 80>(a, nqt, st);
+    else launch_dq<T, 128>(a, nqt, st);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq)");
-    if (a.slope_part) {
-      slopes_kernel<<<a.Hq, 256, 0, st>>>(a.slope_part, (long long)a.B * nt, a.dslopes);
-      DMT_CHECK_LAUNCH("dmt_attn_var_bwd(slopes)");
-    }
+  } else {
+    a.slope_part = nullptr;                               // (no query: nothing to add)
   }
-  if (a.rows_k && a.max_k) {
-    const int nt = (int)cdiv64(a.max_k, 128);
-    if (a.dh <= 32) launch_dkv<T, 32>(a, nt, st);
-    else if (a.dh <= 64) launch_dkv<T, 64>(a, nt, st);
-    else if (a.dh <= 80) launch_dkv<T, 80>(a, nt, st);
-    else launch_dkv<T, 128>(a, nt, st);
+  if (nkt) {
+    if (a.dh <= 32) launch_dkv<T, 32>(a, nkt, nqt, st);
+    else if (a.dh <= 64) launch_dkv<T, 64>(a, nkt, nqt, st);
+    else if (a.dh <= 80) launch_dkv<T, 80>(a, nkt, nqt, st);
+    else launch_dkv<T, 128>(a, nkt, nqt, st);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dkv)");
+    if (a.parts > 1 && a.rows_k) {
+      join_parts_kernel<T><<<dim3((unsigned)cdiv64(a.max_k, 16), a.B), 256, 0, st>>>(a);
+      DMT_CHECK_LAUNCH("dmt_attn_var_bwd(join)");
+    }
   }
   return DMT_OK;
 }
@@ -443,7 +466,5 @@ extern "C" int dmt_attn_var_bwd(const dmt_attn_var_desc* d, void* stream) {
   Args a;
   int rc = dmt_attn_var_args(d, &a, true, "dmt_attn_var_bwd");
   if (rc) return rc < 0 ? rc : DMT_OK;
-  rc = dmt_attn_var_doc_ranges(a, stream);
-  if (rc) return rc;
   return d->dtype == DMT_F32 ? launch_bwd<float>(a, (hipStream_t)stream) : launch_bwd<bf16_t>(a, (hipStream_t)stream);
 }

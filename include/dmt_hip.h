@@ -849,9 +849,12 @@ typedef struct {
   void* dK; int64_t dk_rs;
   void* dV; int64_t dv_rs;
   float* dslopes;                          /* [Hq] or NULL; needs slopes                               */
-  void* ws; uint64_t ws_bytes;             /* documents (both directions) and the backward             */
+  void* doc_ranges;                        /* with documents: dmt_attn_var_doc_bytes() bytes, 16-byte aligned, written by the forward (least and
+                                            * largest id of every 64 rows) and read by the backward of the same call             */
+  void* ws; uint64_t ws_bytes;             /* backward: dmt_attn_var_ws_bytes()                        */
 } dmt_attn_var_desc;
-uint64_t dmt_attn_var_ws_bytes(const dmt_attn_var_desc* d, int32_t backward);
+uint64_t dmt_attn_var_doc_bytes(int32_t B, int32_t max_q, int32_t max_k);
+uint64_t dmt_attn_var_ws_bytes(const dmt_attn_var_desc* d);
 int dmt_attn_var_supported(int32_t dtype, int32_t dh, int32_t Hq, int32_t Hkv);
 int dmt_attn_var_fwd(const dmt_attn_var_desc* d, void* stream);
 int dmt_attn_var_bwd(const dmt_attn_var_desc* d, void* stream);

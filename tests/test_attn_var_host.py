@@ -46,7 +46,7 @@ BAD = [(dict(dtype=2), "needs bf16"), (dict(dh=33), "needs bf16"), (dict(dh=136)
        (dict(B=-1), "negative"), (dict(B=70000), "65535"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(cap=-1.0), "cap"),
        (dict(cap=float("inf")), "cap"), (dict(q_doc=64), "go together"), (dict(q_rs=63), "shorter"), (dict(k_rs=33), "aligned"), (dict(V=1032), "aligned"),
        (dict(Q=None), "NULL"), (dict(k_lens=None), "NULL"), (dict(out=None), "NULL"), (dict(rows_k=2 ** 31), "int32"), (dict(k_rs=1 << 24), "16 MB"),
-       (dict(q_doc=64, k_doc=64, ws=None), "workspace")]
+       (dict(q_doc=64, k_doc=64), "doc_ranges"), (dict(q_doc=64, k_doc=64, doc_ranges=1032), "doc_ranges")]
 
 
 @pytest.mark.parametrize("kw,msg", BAD)
