@@ -40,6 +40,14 @@ struct Args {
   int nqt, nkt;                     // 64-row tiles of max_q, max_k
 };
 
+// The arguments once more, for the part behind a kernel's loop that hardly ever runs: read from the argument segment there and then, so that
+// they do not occupy (and spill) scalar registers in the loop.  Args is the first argument of every kernel that asks.
+__device__ __forceinline__ const Args* args_again() {
+  const void* p = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return (const Args*)p;
+}
+
 // one example's lengths and what its queries may see
 struct Ex {
   int ql, kl, off, pre;
@@ -333,11 +341,14 @@ template <int DHP> struct Tile<bf16_t, DHP> {
   static constexpr int NDT = (DHP + 31) / 32;     // 32-dim tiles of a head
   static constexpr int CH = DHP / 8;              // 16-byte chunks of a row
   static constexpr int CHE = 8;                   // elements of a chunk
-  static constexpr int RS = DHP + 8;              // LDS row stride: 16-byte reads of 8 consecutive rows hit 8 different bank groups
-  static constexpr int rst() { int r = DHP; while (r % 128 != 32 && r % 128 != 96) r += 8; return r; }
-  static constexpr int RST = rst();               // and of a tile read transposed only: 4 rows on disjoint banks
-  static __device__ __forceinline__ Frag natural(const bf16_t* X, int rs, int row, int s, int half) {
-    return *reinterpret_cast<const bf16x8_t*>(X + row * rs + 16 * s + 8 * half);
+  // LDS rows: the 16-byte chunks of a row are permuted by its number, so that both ways of reading it spread over the banks: 16 bytes of 8
+  // consecutive rows (natural), and 4 rows x 2 chunks (transposing; r a multiple of 4).
+  static constexpr int SC = DHP == 80 ? 12 : CH;  // chunks of a row in LDS
+  static constexpr int RS = SC * 8;
+  static __device__ __forceinline__ int swz(int row) { return SC % 8 ? (row >> 2) & 1 : ((row & 3) << 1) | ((row >> 2) & 1); }
+  static __device__ __forceinline__ int at(int row, int ch) { return row * RS + ((ch ^ swz(row)) * 8); }
+  static __device__ __forceinline__ Frag natural(const bf16_t* X, int u, int l31, int s, int half) {     // row 32 u + l31
+    return *reinterpret_cast<const bf16x8_t*>(X + 32 * u * RS + at(l31, 2 * s + half));
   }
   static __device__ __forceinline__ int col(int s, int half) { return 16 * s + 8 * half; }
   static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
@@ -349,18 +360,18 @@ template <int DHP> struct Tile<bf16_t, DHP> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w
-  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int rs, int row0, const f32x16_t& w, int lane) {
-    const int half = lane >> 5, i16 = lane & 15, grp = (lane >> 4) & 1;
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int row0, const f32x16_t& w, int lane) {
+    const int half = lane >> 5, i16 = lane & 15, grp = (lane >> 4) & 1, r = 4 * half + (i16 >> 2);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       union { bf16x8_t v; unsigned d[4]; } b;
 #pragma unroll
       for (int i = 0; i < 4; ++i) b.d[i] = dmt_pack_bf16(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
-      const bf16_t* x = X + (row0 + 16 * u + 4 * half + (i16 >> 2)) * rs + 16 * grp + 4 * (i16 & 3);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
-        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + dt * 32));
-        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + dt * 32 + 8 * rs));
+        const bf16_t* x = X + (row0 + 16 * u) * RS + at(r, 4 * dt + 2 * grp + ((i16 >> 1) & 1)) + 4 * (i16 & 1);
+        const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x));
+        const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + 8 * RS));
         acc[dt] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b.v, acc[dt]);
       }
     }
@@ -373,9 +384,9 @@ template <int DHP> struct Tile<float, DHP> {
   static constexpr int CH = DHP / 4;
   static constexpr int CHE = 4;
   static constexpr int RS = DHP + 4;
-  static constexpr int RST = DHP + 4;
-  static __device__ __forceinline__ Frag natural(const float* X, int rs, int row, int s, int half) {
-    return *reinterpret_cast<const f32x4_t*>(X + row * rs + 8 * s + 4 * half);
+  static __device__ __forceinline__ int at(int row, int ch) { return row * RS + ch * 4; }
+  static __device__ __forceinline__ Frag natural(const float* X, int u, int l31, int s, int half) {
+    return *reinterpret_cast<const f32x4_t*>(X + 32 * u * RS + at(l31, 2 * s + half));
   }
   static __device__ __forceinline__ int col(int s, int half) { return 8 * s + 4 * half; }
   static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
@@ -388,13 +399,13 @@ template <int DHP> struct Tile<float, DHP> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int rs, int row0, const f32x16_t& w, int lane) {
-    const float* x = X + (row0 + 4 * (lane >> 5)) * rs + (lane & 31);
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int row0, const f32x16_t& w, int lane) {
+    const float* x = X + (row0 + 4 * (lane >> 5)) * RS + (lane & 31);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
-        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[(8 * (r >> 2) + (r & 3)) * rs + dt * 32], w[r], acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[(8 * (r >> 2) + (r & 3)) * RS + dt * 32], w[r], acc[dt], 0, 0, 0);
     }
   }
 };
@@ -421,36 +432,78 @@ __device__ __forceinline__ void own_row(typename Tile<T, DHP>::Frag* f, const T*
   }
 }
 
-// The 64-row tiles of two operands on their way into LDS: requested into registers one tile ahead, written when the tile before is done with.
-template <typename T, int DHP> struct Stage {
-  typedef Tile<T, DHP> TL;
+// The 64-row tiles of two operands on their way into LDS.  bf16: straight from memory (buffer_load ... lds: 64 lanes fill 1 KB of consecutive
+// 16-byte chunks, each lane choosing what the row permutation wants there); issued a tile ahead, it costs no registers and no LDS-write
+// instructions.  begin() and end() bracket the use of the tile before; the buffer that begin() names must be free.
+template <typename T, int DHP> struct Stage;
+__device__ __forceinline__ u32x4_t rsrc_words(const void* base, unsigned bytes) {
+  const unsigned long long p = (unsigned long long)(uintptr_t)base;
+  u32x4_t r;
+  r[0] = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)p);
+  r[1] = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(p >> 32)) & 0xffffu;
+  r[2] = (unsigned)__builtin_amdgcn_readfirstlane((int)bytes);
+  r[3] = 0x00027000u;
+  return r;
+}
+__device__ __forceinline__ void load16_lds(const u32x4_t& rsrc, int off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+template <int DHP> struct Stage<bf16_t, DHP> {
+  typedef Tile<bf16_t, DHP> TL;
+  static constexpr int IT = KT * TL::SC / 256;
+  static_assert(KT * TL::SC % 256 == 0, "whole 1 KB pieces");
+  int off_a[IT], off_b[IT];              // byte offsets within a tile
+  unsigned at;                           // LDS byte offset of the wavefront's first piece within a tile
+  __device__ __forceinline__ void init(long long rs_a, long long rs_b, int dh, int tid) {
+    at = (unsigned)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024u;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int c = tid + i * 256, row = c / TL::SC, ch = (c - row * TL::SC) ^ TL::swz(row);
+      const bool in = ch * 8 < dh;
+      off_a[i] = in ? row * (int)(rs_a * 2) + ch * 16 : OUTSIDE;
+      off_b[i] = in ? row * (int)(rs_b * 2) + ch * 16 : OUTSIDE;
+    }
+  }
+  __device__ __forceinline__ void begin(const bf16_t* pa, long long rs_a, const bf16_t* pb, long long rs_b, int rows, int dh, bf16_t* la, bf16_t* lb) {
+    const unsigned da = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)la + at;
+    const unsigned db = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lb + at;
+    const u32x4_t ra = rsrc_words(pa, (unsigned)((rows - 1) * (int)(rs_a * 2) + dh * 2)), rb = rsrc_words(pb, (unsigned)((rows - 1) * (int)(rs_b * 2) + dh * 2));
+#pragma unroll
+    for (int i = 0; i < IT; ++i) load16_lds(ra, off_a[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(da + 4096u * i)));
+#pragma unroll
+    for (int i = 0; i < IT; ++i) load16_lds(rb, off_b[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(db + 4096u * i)));
+  }
+  __device__ __forceinline__ void end(bf16_t*, bf16_t*) const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+};
+// fp32: through registers, one tile in LDS
+template <int DHP> struct Stage<float, DHP> {
+  typedef Tile<float, DHP> TL;
   static constexpr int IT = (KT * TL::CH + 255) / 256;
   u32x4_t a[IT], b[IT];
-  int off_a[IT], off_b[IT], dst[IT];     // byte offsets within a tile; row << 8 | chunk of the destination
+  int off_a[IT], off_b[IT], dst[IT];     // byte offsets within a tile; element in LDS
   __device__ __forceinline__ void init(long long rs_a, long long rs_b, int dh, int tid) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       const int c = tid + i * 256, row = c / TL::CH, ch = c - row * TL::CH;
-      const bool in = row < KT && ch * TL::CHE < dh;
-      off_a[i] = in ? row * (int)(rs_a * (int)sizeof(T)) + ch * 16 : OUTSIDE;
-      off_b[i] = in ? row * (int)(rs_b * (int)sizeof(T)) + ch * 16 : OUTSIDE;
-      dst[i] = row < KT ? (row << 8 | ch) : -1;
+      const bool in = row < KT && ch * 4 < dh;
+      off_a[i] = in ? row * (int)(rs_a * 4) + ch * 16 : OUTSIDE;
+      off_b[i] = in ? row * (int)(rs_b * 4) + ch * 16 : OUTSIDE;
+      dst[i] = row < KT ? TL::at(row, ch) : -1;
     }
   }
-  __device__ __forceinline__ void request(const T* pa, long long rs_a, const T* pb, long long rs_b, int rows, int dh) {
-    const rsrc_t ra = rows_rsrc<T>(pa, rs_a, rows, dh), rb = rows_rsrc<T>(pb, rs_b, rows, dh);
+  __device__ __forceinline__ void begin(const float* pa, long long rs_a, const float* pb, long long rs_b, int rows, int dh, float*, float*) {
+    const rsrc_t ra = rows_rsrc<float>(pa, rs_a, rows, dh), rb = rows_rsrc<float>(pb, rs_b, rows, dh);
 #pragma unroll
     for (int i = 0; i < IT; ++i) a[i] = load16(ra, off_a[i]);
 #pragma unroll
     for (int i = 0; i < IT; ++i) b[i] = load16(rb, off_b[i]);
   }
-  __device__ __forceinline__ void write(T* la, int lds_a, T* lb, int lds_b) const {
+  __device__ __forceinline__ void end(float* la, float* lb) const {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
       if ((KT * TL::CH) % 256 != 0 && dst[i] < 0) continue;
-      const int row = dst[i] >> 8, ch = dst[i] & 255;
-      *reinterpret_cast<u32x4_t*>(la + row * lds_a + ch * TL::CHE) = a[i];
-      *reinterpret_cast<u32x4_t*>(lb + row * lds_b + ch * TL::CHE) = b[i];
+      *reinterpret_cast<u32x4_t*>(la + dst[i]) = a[i];
+      *reinterpret_cast<u32x4_t*>(lb + dst[i]) = b[i];
     }
   }
 };

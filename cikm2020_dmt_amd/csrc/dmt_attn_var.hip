@@ -12,7 +12,7 @@ template <typename T, int DHP, bool SHAPED>
 __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;               // tiles in LDS
-  constexpr int KE = KT * TL::RS, VE = KT * TL::RST + 32;
+  constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS, VE = KT * TL::RS + PAD;      // (fp32: dims past the last row's end are read, not used)
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
   __shared__ __attribute__((aligned(16))) int docs[NB][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
@@ -56,13 +56,14 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   Stage<T, DHP> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
-  const auto request = [&](int t) {
+  const auto begin = [&](int t, int buf) {
     const int k0 = t * KT;
-    st.request(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh);
+    st.begin(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh, lds + buf * (KE + VE),
+             lds + buf * (KE + VE) + KE);
     if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
   };
-  const auto write = [&](int buf) {
-    st.write(lds + buf * (KE + VE), TL::RS, lds + buf * (KE + VE) + KE, TL::RST);
+  const auto end = [&](int buf) {
+    st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
     if (kr && tid < KT) docs[buf][tid] = kd;
   };
   f32x16_t o[TL::NDT];
@@ -71,13 +72,13 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   float m = -INFINITY, l = 0.f;
   int t = next(0), buf = 0;
   if (t < nk) {
-    request(t);
-    write(0);
+    begin(t, 0);
+    end(0);
   }
   __syncthreads();
   while (t < nk) {
     const int tn = next(t + 1), k0 = t * KT;
-    if (tn < nk) request(tn);
+    if (tn < nk) begin(tn, NB == 2 ? buf ^ 1 : 0);
     const T* Kl = lds + buf * (KE + VE);
     const T* Vl = Kl + KE;
     bool work = active && k0 < lim_w, docs_differ = false;
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
       for (int u = 0; u < 2; ++u) {
         s[u] = zero16();
 #pragma unroll
-        for (int x = 0; x < TL::NS; ++x) s[u] = TL::mma(TL::natural(Kl, TL::RS, 32 * u + l31, x, half), q[x], s[u]);
+        for (int x = 0; x < TL::NS; ++x) s[u] = TL::mma(TL::natural(Kl, u, l31, x, half), q[x], s[u]);
       }
       if (SHAPED) {
         if (sh.cap) {
@@ -158,11 +159,11 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
           s[u][r] = exp2_hw(SHAPED ? s[u][r] - mu : __builtin_fmaf(s[u][r], c, -mu));
           l += s[u][r];
         }
-        TL::accumulate(o, Vl, TL::RST, 32 * u, s[u], lane);
+        TL::accumulate(o, Vl, 32 * u, s[u], lane);
       }
     }
     if (NB == 1) __syncthreads();
-    if (tn < nk) write(NB == 2 ? buf ^ 1 : 0);
+    if (tn < nk) end(NB == 2 ? buf ^ 1 : 0);
     __syncthreads();
     if (NB == 2) buf ^= 1;
     t = tn;
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   unsigned long long again = __ballot(in && !(bad == 0.f));
   again |= again >> 32;
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_fwd<T>(a, e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1) row_fwd<T>(*args_again(), e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
 // (least, largest) document id of every 64 rows, of the queries (blockIdx.z = 0) and of the keys: tiles that share no id are skipped, tiles of

@@ -31,7 +31,7 @@ template <typename T, int DHP, bool SHAPED>
 __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
-  constexpr int KE = KT * TL::RS + 32, VE = KT * TL::RS;
+  constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS + PAD, VE = KT * TL::RS;
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
   __shared__ __attribute__((aligned(16))) int docs[NB][KT];
   __shared__ float part[4];
@@ -91,13 +91,14 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   Stage<T, DHP> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
-  const auto request = [&](int t) {
+  const auto begin = [&](int t, int buf) {
     const int k0 = t * KT;
-    st.request(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh);
+    st.begin(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh, lds + buf * (KE + VE),
+             lds + buf * (KE + VE) + KE);
     if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
   };
-  const auto write = [&](int buf) {
-    st.write(lds + buf * (KE + VE), TL::RS, lds + buf * (KE + VE) + KE, TL::RS);
+  const auto end = [&](int buf) {
+    st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
     if (kr && tid < KT) docs[buf][tid] = kd;
   };
   f32x16_t o[TL::NDT];
@@ -106,13 +107,13 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
   int t = next(0), buf = 0;
   if (t < nk) {
-    request(t);
-    write(0);
+    begin(t, 0);
+    end(0);
   }
   __syncthreads();
   while (t < nk) {
     const int tn = next(t + 1), k0 = t * KT;
-    if (tn < nk) request(tn);
+    if (tn < nk) begin(tn, NB == 2 ? buf ^ 1 : 0);
     const T* Kl = lds + buf * (KE + VE);
     const T* Vl = Kl + KE;
     bool work = active && k0 < lim_w, docs_differ = false;
@@ -127,8 +128,8 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
         f32x16_t s = zero16(), dp = zero16(), r2;
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) {
-          s = TL::mma(TL::natural(Kl, TL::RS, 32 * u + l31, x, half), q[x], s);
-          dp = TL::mma(TL::natural(Vl, TL::RS, 32 * u + l31, x, half), g[x], dp);
+          s = TL::mma(TL::natural(Kl, u, l31, x, half), q[x], s);
+          dp = TL::mma(TL::natural(Vl, u, l31, x, half), g[x], dp);
         }
         const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
         if (SHAPED) shaped<-1>(s, r2, sh, d0);
@@ -166,11 +167,11 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
           s[r] *= dp[r] - D;
           if (SHAPED && sh.cap) s[r] *= 4.f * r2[r] * (1.f - r2[r]);
         }
-        TL::accumulate(o, Kl, TL::RS, 32 * u, s, lane);
+        TL::accumulate(o, Kl, 32 * u, s, lane);
       }
     }
     if (NB == 1) __syncthreads();
-    if (tn < nk) write(NB == 2 ? buf ^ 1 : 0);
+    if (tn < nk) end(NB == 2 ? buf ^ 1 : 0);
     __syncthreads();
     if (NB == 2) buf ^= 1;
     t = tn;
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     if (half) sl = 0.f;                                  // (both halves hold the row's)
     sl = wave_sum(sl);
     for (int r = 0; r < 32; ++r)
-      if ((again >> r) & 1) sl += row_dq<T>(a, e, h, iw + r, __shfl(D, r), (float*)lds + wave * ROW_LDS, lane);
+      if ((again >> r) & 1) sl += row_dq<T>(*args_again(), e, h, iw + r, __shfl(D, r), (float*)lds + wave * ROW_LDS, lane);
   }
   if (a.slope_part) {
     if (lane == 0) part[wave] = sl;
@@ -222,18 +223,19 @@ __device__ void sum_slopes(const float* part, long long n, float* out, double* r
 
 // dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
 // tiles of 64: S and dP with lane = key, P and dX packed are the B operands of dV^T += dO^T P and dK^T += Q^T dX.  Nothing crosses wavefronts.
-template <typename T, int DHP, bool SHAPED>
-__global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv_kernel(const Args a, int nt, int nqt) {
+// WHAT: 1 = dK, 2 = dV, 3 = both.
+template <typename T, int DHP, bool SHAPED, int WHAT>
+__global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, int nqt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
-  constexpr int QE = KT * TL::RS + 32;
+  constexpr int QE = KT * TL::RS + (sizeof(T) == 2 ? 0 : 32);
   __shared__ __attribute__((aligned(16))) T lds[NB * 2 * QE];
   __shared__ __attribute__((aligned(16))) int docs[NB][KT];
   __shared__ __attribute__((aligned(16))) float stats[NB][2][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
-  const int id = (int)blockIdx.x - (SHAPED && a.slope_part ? a.Hq : 0);
-  if (SHAPED && id < 0) {                                 // the first workgroups finish the slopes' gradient that the dQ kernel left in parts
+  const int id = (int)blockIdx.x - (SHAPED && (WHAT & 1) && a.slope_part ? a.Hq : 0);
+  if (SHAPED && (WHAT & 1) && id < 0) {                                 // the first workgroups finish the slopes' gradient that the dQ kernel left in parts
     const long long n = (long long)a.B * nqt;
     sum_slopes(a.slope_part + (long long)blockIdx.x * n, n, a.dslopes + blockIdx.x, (double*)lds);
     return;
@@ -248,7 +250,7 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   const bool active = jw < e.kl;
   typename TL::Frag k[TL::NS], v[TL::NS];
   own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, j, half);
-  own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
+  if (WHAT & 1) own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
   // queries that may see some key of the workgroup / wavefront / lane: from `lo` on (rows before it sit above the diagonal, unless the key
   // belongs to the prefix)
   const int lo_wg = a.causal && kt * 128 >= e.pre ? max(0, kt * 128 - e.off) : 0;
@@ -279,10 +281,10 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   st.init(a.q_rs, a.do_rs, a.dh, tid);
   int qd = 0;
   float lse2 = 0.f;
-  const auto request = [&](int n) {
+  const auto begin = [&](int n, int buf) {
     const int h = hk * a.G + g0 + n / per, i0 = (t0 + n % per) * KT;
-    st.request((const T*)a.Q + (e.q0 + i0) * a.q_rs + (long long)h * a.dh, a.q_rs, (const T*)a.dout + (e.q0 + i0) * a.do_rs + (long long)h * a.dh, a.do_rs,
-               min(KT, e.ql - i0), a.dh);
+    st.begin((const T*)a.Q + (e.q0 + i0) * a.q_rs + (long long)h * a.dh, a.q_rs, (const T*)a.dout + (e.q0 + i0) * a.do_rs + (long long)h * a.dh, a.do_rs,
+             min(KT, e.ql - i0), a.dh, lds + buf * 2 * QE, lds + buf * 2 * QE + QE);
     if (tid < 2 * KT) {
       const int i = i0 + (tid & (KT - 1));
       const long long stat = (e.q0 + i) * a.Hq + h;
@@ -295,23 +297,26 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
       }
     }
   };
-  const auto write = [&](int buf) {
-    st.write(lds + buf * 2 * QE, TL::RS, lds + buf * 2 * QE + QE, TL::RS);
+  const auto end = [&](int buf) {
+    st.end(lds + buf * 2 * QE, lds + buf * 2 * QE + QE);
     if (tid < 2 * KT) stats[buf][tid / KT][tid & (KT - 1)] = lse2;
     if (qr && tid < KT) docs[buf][tid] = qd;
   };
-  f32x16_t dk[TL::NDT], dv[TL::NDT];
+  f32x16_t dk[WHAT & 1 ? TL::NDT : 1], dv[WHAT & 2 ? TL::NDT : 1];
 #pragma unroll
-  for (int dt = 0; dt < TL::NDT; ++dt) dk[dt] = dv[dt] = zero16();
+  for (int dt = 0; dt < TL::NDT; ++dt) {
+    if (WHAT & 1) dk[dt] = zero16();
+    if (WHAT & 2) dv[dt] = zero16();
+  }
   int n = next(0), buf = 0;
   if (n < total) {
-    request(n);
-    write(0);
+    begin(n, 0);
+    end(0);
   }
   __syncthreads();
   while (n < total) {
     const int nn = next(n + 1), tq = t0 + n % per, i0 = tq * KT;
-    if (nn < total) request(nn);
+    if (nn < total) begin(nn, NB == 2 ? buf ^ 1 : 0);
     const T* Ql = lds + buf * 2 * QE;
     const T* Gl = Ql + QE;
     const Shape sh = shape_of(a, hk * a.G + g0 + n / per);
@@ -327,8 +332,8 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
         f32x16_t s = zero16(), dp = zero16(), r2;
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) {
-          s = TL::mma(TL::natural(Ql, TL::RS, 32 * u + l31, x, half), k[x], s);
-          dp = TL::mma(TL::natural(Gl, TL::RS, 32 * u + l31, x, half), v[x], dp);
+          s = TL::mma(TL::natural(Ql, u, l31, x, half), k[x], s);
+          if (WHAT & 1) dp = TL::mma(TL::natural(Gl, u, l31, x, half), v[x], dp);
         }
         if (SHAPED) shaped<1>(s, r2, sh, (float)(i0 + 32 * u + 4 * half + e.off - j));
 #pragma unroll
@@ -353,7 +358,8 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
             }
           }
         }
-        TL::accumulate(dv, Gl, TL::RS, 32 * u, s, lane);
+        if (WHAT & 2) TL::accumulate(dv, Gl, 32 * u, s, lane);
+        if (!(WHAT & 1)) continue;
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg) {
           const float4 ds = *reinterpret_cast<const float4*>(&stats[buf][1][32 * u + 8 * gg + 4 * half]);
@@ -364,11 +370,11 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
             if (SHAPED && sh.cap) s[4 * gg + c] *= 4.f * r2[4 * gg + c] * (1.f - r2[4 * gg + c]);
           }
         }
-        TL::accumulate(dk, Ql, TL::RS, 32 * u, s, lane);
+        TL::accumulate(dk, Ql, 32 * u, s, lane);
       }
     }
     if (NB == 1) __syncthreads();
-    if (nn < total) write(NB == 2 ? buf ^ 1 : 0);
+    if (nn < total) end(NB == 2 ? buf ^ 1 : 0);
     __syncthreads();
     if (NB == 2) buf ^= 1;
     n = nn;
@@ -377,27 +383,30 @@ __global__ __launch_bounds__(256, (DHP * sizeof(T) > 160 ? 1 : 2)) void tile_dkv
   const bool in = j < e.kl;
   float bad = 0.f;
 #pragma unroll
-  for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(dk[dt], dt, half, a.dh) + not_finite(dv[dt], dt, half, a.dh);
+  for (int dt = 0; dt < TL::NDT; ++dt) {
+    if (WHAT & 1) bad += not_finite(dk[dt], dt, half, a.dh);
+    if (WHAT & 2) bad += not_finite(dv[dt], dt, half, a.dh);
+  }
   if (in && a.parts > 1) {
     const long long at = (((long long)part * a.rows_k + e.k0 + j) * a.Hkv + hk) * a.dh;
 #pragma unroll
     for (int dt = 0; dt < TL::NDT; ++dt) {
-      store_dims<float>(dk[dt], 1.f, a.part_k + at, dt, half, a.dh);
-      store_dims<float>(dv[dt], 1.f, a.part_v + at, dt, half, a.dh);
+      if (WHAT & 1) store_dims<float>(dk[dt], 1.f, a.part_k + at, dt, half, a.dh);
+      if (WHAT & 2) store_dims<float>(dv[dt], 1.f, a.part_v + at, dt, half, a.dh);
     }
   } else if (in) {
     T* pk = (T*)a.dK + (e.k0 + j) * a.dk_rs + (long long)hk * a.dh;
     T* pv = (T*)a.dV + (e.k0 + j) * a.dv_rs + (long long)hk * a.dh;
 #pragma unroll
     for (int dt = 0; dt < TL::NDT; ++dt) {
-      store_dims<T>(dk[dt], a.scale, pk, dt, half, a.dh);
-      store_dims<T>(dv[dt], 1.f, pv, dt, half, a.dh);
+      if (WHAT & 1) store_dims<T>(dk[dt], a.scale, pk, dt, half, a.dh);
+      if (WHAT & 2) store_dims<T>(dv[dt], 1.f, pv, dt, half, a.dh);
     }
   }
   unsigned long long again = __ballot(in && !(bad == 0.f));
   again |= again >> 32;
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_dkv<T>(a, e, hk, part, jw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1) row_dkv<T>(*args_again(), e, hk, part, jw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
 // dK = scale (sum of its parts), dV = sum of its parts, in their order: 16 key rows of one example a workgroup
@@ -428,10 +437,18 @@ template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t
   if (a.cap > 0.f || a.slopes) tile_dq_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
   else tile_dq_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
 }
+template <typename T, int DHP, bool SHAPED> void launch_dkv_as(const Args& a, int nt, int nqt, hipStream_t st) {
+  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
+  if (DHP * sizeof(T) > 160) {
+    tile_dkv_kernel<T, DHP, SHAPED, 2><<<grid, 256, 0, st>>>(a, nt, nqt);
+    tile_dkv_kernel<T, DHP, SHAPED, 1><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+  } else {
+    tile_dkv_kernel<T, DHP, SHAPED, 3><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+  }
+}
 template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts + (a.slope_part ? a.Hq : 0));
-  if (a.cap > 0.f || a.slopes) tile_dkv_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt, nqt);
-  else tile_dkv_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt, nqt);
+  if (a.cap > 0.f || a.slopes) launch_dkv_as<T, DHP, true>(a, nt, nqt, st);
+  else launch_dkv_as<T, DHP, false>(a, nt, nqt, st);
 }
 
 template <typename T>
