@@ -34,7 +34,7 @@ struct Args {
   float* dslopes;
   float* D;                         // [rows_q, Hq]: rowsum(dout * out)
   float* slope_part;                // [Hq][B * ceil(max_q / 128)]
-  int parts;                        // dK, dV: the heads of a group in so many pieces, summed by a launch of their own
+  int parts, qparts;                // dK, dV: heads of a group x query ranges in `parts` pieces (qparts ranges), summed by a launch of their own
   float* part_k; float* part_v;     // [parts][rows_k][Hkv * dh] when parts > 1
   int2* q_rng; int2* k_rng;         // (least, largest) document id of every 64-row tile: [B][ceil(max / 64)]
   int nqt, nkt;                     // 64-row tiles of max_q, max_k
@@ -241,10 +241,10 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float D, float
   return slope_part(wave_sum(s0), wave_sum(s1), wave_sum(s2), wave_sum(sp));
 }
 
-// dk and dv of one key row: over the query heads of its group (those of one part), then over the queries
-__device__ __forceinline__ int part_head(const Args& a, int part) { return (int)((long long)a.G * part / a.parts); }
+// dk and dv of one key row: over the query heads of its group (those of one part), then over the queries (of one range)
+__device__ __forceinline__ int part_head(const Args& a, int hp) { return (int)((long long)a.G * hp / (a.parts / a.qparts)); }
 template <typename T>
-__device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int j, float* lds, int lane) {
+__device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int i_lo, int i_hi, int j, float* lds, int lane) {
   float* k = lds;
   float* v = lds + MAX_DH;
   float* pl = lds + 2 * MAX_DH;
@@ -257,13 +257,13 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int j, flo
   }
   lds_fence();
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-  for (int h = hk * a.G + part_head(a, part); h < hk * a.G + part_head(a, part + 1); ++h) {
+  for (int h = hk * a.G + part_head(a, part / a.qparts); h < hk * a.G + part_head(a, part / a.qparts + 1); ++h) {
     const Shape s = shape_of(a, h);
     const T* Q = (const T*)a.Q + e.q0 * a.q_rs + (long long)h * dh;
     const T* O = (const T*)a.dout + e.q0 * a.do_rs + (long long)h * dh;
-    for (int i0 = 0; i0 < e.ql; i0 += 64) {
+    for (int i0 = i_lo; i0 < i_hi; i0 += 64) {
       const int i = i0 + lane;
-      const bool ok = i < e.ql && may_see(a, e, i, j, a.q_doc ? a.q_doc[e.q0 + i] : 0);
+      const bool ok = i < i_hi && may_see(a, e, i, j, a.q_doc ? a.q_doc[e.q0 + i] : 0);
       const unsigned long long vis = __ballot(ok);
       if (!vis) continue;
       float p = 0.f, dx = 0.f;
@@ -505,6 +505,47 @@ template <int DHP> struct Stage<float, DHP> {
       *reinterpret_cast<u32x4_t*>(la + dst[i]) = a[i];
       *reinterpret_cast<u32x4_t*>(lb + dst[i]) = b[i];
     }
+  }
+};
+
+// The tiles lo .. hi - 1 that a workgroup has to visit.  With documents the ranges of 64 tiles are looked at together, a lane a tile: a walk that
+// asked for one range after the other spent most of a workgroup's life waiting for them.
+template <bool DOCS> struct Walk;
+template <> struct Walk<false> {         // every tile, nothing masked
+  int hi;
+  __device__ __forceinline__ int next(int t, int& flags) {
+    flags = 1;
+    return t < hi ? t : hi;
+  }
+};
+template <> struct Walk<true> {
+  const int2* rng;
+  int lo, hi, free_wg, free_w;           // tiles before free_wg (free_w) hold rows that no document hides from the workgroup (wavefront)
+  int glo, ghi, wlo, whi;                // the ids of the workgroup's and of the wavefront's own rows
+  int chunk;
+  unsigned long long vis, visw, same;
+  __device__ __forceinline__ void look(int c) {
+    const int t = c * 64 + (threadIdx.x & 63);
+    const bool in = t >= lo && t < hi;
+    const int2 r = in ? rng[t] : make_int2(1, 0);
+    vis = __ballot(in && (t < free_wg || (r.x <= ghi && r.y >= glo)));
+    visw = __ballot(in && (t < free_w || (r.x <= whi && r.y >= wlo)));
+    same = __ballot(in && r.x == r.y && wlo == whi && r.x == wlo);
+    chunk = c;
+  }
+  // the first tile to visit from t on, or hi; flags: 1 = the wavefront has to look at it, 2 = documents may hide some of it
+  __device__ __forceinline__ int next(int t, int& flags) {
+    while (t < hi) {
+      if ((t >> 6) != chunk) look(t >> 6);
+      const unsigned long long m = vis >> (t & 63);
+      if (m) {
+        t += __ffsll((long long)m) - 1;
+        flags = (int)((visw >> (t & 63)) & 1) | ((int)((same >> (t & 63)) & 1) ^ 1) << 1;
+        return t;
+      }
+      t = (t | 63) + 1;
+    }
+    return hi;
   }
 };
 

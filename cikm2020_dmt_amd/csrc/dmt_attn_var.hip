@@ -8,13 +8,13 @@ namespace {
 // One workgroup of 4 wavefronts owns 128 queries of a head (a wavefront 32) and walks over the keys in tiles of 64, one tile in LDS, the next
 // one on its way through registers.  One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
 // are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
-template <typename T, int DHP, bool SHAPED>
+template <typename T, int DHP, bool SHAPED, bool DOCS>
 __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;               // tiles in LDS
   constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS, VE = KT * TL::RS + PAD;      // (fp32: dims past the last row's end are read, not used)
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
-  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  __shared__ __attribute__((aligned(16))) int docs[DOCS ? NB : 1][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
   int head, qt;
@@ -35,24 +35,22 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
   const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
   const int nk = (lim_wg + KT - 1) / KT;
-  int qlo = 0, qhi = 0, wlo = 0, whi = 0, qd = 0;
-  const int2* kr = nullptr;
-  if (a.q_doc) {
+  int qd = 0;
+  Walk<DOCS> wk;
+  wk.hi = nk;
+  if constexpr (DOCS) {
+    wk.lo = 0;
     const int2* qr = a.q_rng + (long long)b * a.nqt;
-    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0;
-    qlo = min(r0.x, r1.x);
-    qhi = max(r0.y, r1.y);
-    const int2 rw = wave < 2 ? r0 : r1;
-    wlo = rw.x;
-    whi = rw.y;
+    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0, rw = wave < 2 ? r0 : r1;
+    wk.rng = a.k_rng + (long long)b * a.nkt;
+    wk.free_wg = wk.free_w = (e.pre + KT - 1) / KT;
+    wk.glo = min(r0.x, r1.x);
+    wk.ghi = max(r0.y, r1.y);
+    wk.wlo = rw.x;
+    wk.whi = rw.y;
+    wk.chunk = -1;
     qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
-    kr = a.k_rng + (long long)b * a.nkt;
   }
-  const auto next = [&](int t) {
-    if (kr)
-      while (t < nk && t * KT >= e.pre && (kr[t].x > qhi || kr[t].y < qlo)) ++t;
-    return t;
-  };
   Stage<T, DHP> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
@@ -60,32 +58,29 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     const int k0 = t * KT;
     st.begin(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh, lds + buf * (KE + VE),
              lds + buf * (KE + VE) + KE);
-    if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
+    if (DOCS && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
   };
   const auto end = [&](int buf) {
     st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
-    if (kr && tid < KT) docs[buf][tid] = kd;
+    if (DOCS && tid < KT) docs[buf][tid] = kd;
   };
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
   float m = -INFINITY, l = 0.f;
-  int t = next(0), buf = 0;
+  int flags = 0, buf = 0, t = wk.next(0, flags);
   if (t < nk) {
     begin(t, 0);
     end(0);
   }
   __syncthreads();
   while (t < nk) {
-    const int tn = next(t + 1), k0 = t * KT;
+    int nflags = 0;
+    const int tn = wk.next(t + 1, nflags), k0 = t * KT;
     if (tn < nk) begin(tn, NB == 2 ? buf ^ 1 : 0);
     const T* Kl = lds + buf * (KE + VE);
     const T* Vl = Kl + KE;
-    bool work = active && k0 < lim_w, docs_differ = false;
-    if (kr && k0 + KT > e.pre) {
-      if (k0 >= e.pre && (kr[t].x > whi || kr[t].y < wlo)) work = false;
-      docs_differ = !(kr[t].x == kr[t].y && wlo == whi && wlo == kr[t].x);
-    }
+    const bool work = active && k0 < lim_w && (flags & 1), docs_differ = DOCS && (flags & 2) && k0 + KT > e.pre;
     if (work) {
       f32x16_t s[2];
 #pragma unroll
@@ -115,7 +110,18 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
         }
       }
       // masked places become -inf: only in the tiles that the lengths, the diagonal or a document boundary cross
-      if (docs_differ) {
+      const bool cut = k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off);
+      if (docs_differ && !cut && k0 >= e.pre) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 d = *reinterpret_cast<const int4*>(&docs[buf][32 * u + 8 * g + 4 * half]);
+            const int dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[u][4 * g + c] = dd[c] == qd ? s[u][4 * g + c] : -INFINITY;
+          }
+      } else if (docs_differ) {
         const int pre = e.pre - k0 - 4 * half, lm = lim0 - k0 - 4 * half;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -129,7 +135,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
               s[u][4 * g + c] = (key < pre || (key < lm && dd[c] == qd)) ? s[u][4 * g + c] : -INFINITY;
             }
           }
-      } else if (k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off)) {
+      } else if (cut) {
         const int lm = lim - k0 - 4 * half;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -167,6 +173,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     __syncthreads();
     if (NB == 2) buf ^= 1;
     t = tn;
+    flags = nflags;
   }
   if (!active) return;
   l += other_half(l);
@@ -208,8 +215,11 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const Args a) {
 template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
   const int nt = (int)cdiv64(a.max_q, 128);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  if (a.cap > 0.f || a.slopes) tile_fwd_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
-  else tile_fwd_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+  const bool shaped = a.cap > 0.f || a.slopes;
+  if (shaped && a.q_doc) tile_fwd_kernel<T, DHP, true, true><<<grid, 256, 0, st>>>(a, nt);
+  else if (shaped) tile_fwd_kernel<T, DHP, true, false><<<grid, 256, 0, st>>>(a, nt);
+  else if (a.q_doc) tile_fwd_kernel<T, DHP, false, true><<<grid, 256, 0, st>>>(a, nt);
+  else tile_fwd_kernel<T, DHP, false, false><<<grid, 256, 0, st>>>(a, nt);
 }
 template <typename T> int launch_fwd(const Args& a, hipStream_t st) {
   if (a.dh <= 32) launch_tile<T, 32>(a, st);
@@ -231,13 +241,17 @@ extern "C" int dmt_attn_var_supported(int32_t dtype, int32_t dh, int32_t Hq, int
 }
 
 namespace {
-// dK, dV: the query heads of a group run one after the other in a workgroup, unless that leaves fewer than four workgroups a compute unit: then
-// they are cut into pieces that run side by side and leave fp32 sums to be added in their order.
-constexpr int64_t WANT_WG = 1024;
-int parts_of(const dmt_attn_var_desc* d) {
-  const int64_t G = d->Hq / d->Hkv, base = (int64_t)d->B * d->Hkv * cdiv64(d->max_k, 128);
-  const int64_t p = base > 0 ? cdiv64(WANT_WG, base) : 1;
-  return (int)(p < G ? p : G);
+// dK, dV: a workgroup walks over the query heads of its group and over the queries.  When that leaves fewer than four workgroups a compute unit
+// the walk is cut into pieces that run side by side and leave fp32 sums to be added in their order: first by head, then by ranges of at least
+// 256 queries.
+int parts_of(const dmt_attn_var_desc* d, int* qparts) {
+  const int64_t G = d->Hq / d->Hkv, base = (int64_t)d->B * d->Hkv * cdiv64(d->max_k, 128), want = 1024;
+  const int64_t p = base > 0 ? cdiv64(want, base) : 1, hp = p < G ? p : G;
+  int64_t qp = base > 0 ? cdiv64(want, base * hp) : 1;
+  if (qp > d->max_q / 256) qp = d->max_q / 256;
+  if (qp < 1) qp = 1;
+  *qparts = (int)qp;
+  return (int)(hp * qp);
 }
 struct WsLayout { uint64_t D, sp, pk, pv, total; };
 WsLayout ws_layout(const dmt_attn_var_desc* d) {
@@ -247,7 +261,8 @@ WsLayout ws_layout(const dmt_attn_var_desc* d) {
   at += up16(4 * (uint64_t)d->rows_q * (uint64_t)d->Hq);
   w.sp = at;
   if (d->dslopes) at += up16(4 * (uint64_t)d->Hq * (uint64_t)d->B * (uint64_t)cdiv64(d->max_q, 128));
-  const int parts = parts_of(d);
+  int qparts;
+  const int parts = parts_of(d, &qparts);
   const uint64_t part = parts > 1 ? up16(4 * (uint64_t)parts * (uint64_t)d->rows_k * (uint64_t)d->Hkv * (uint64_t)d->dh) : 0;
   w.pk = at;
   at += part;
@@ -324,7 +339,8 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   a->k_rng = d->q_doc ? (int2*)((char*)d->doc_ranges + up16(8 * (uint64_t)d->B * (uint64_t)a->nqt)) : nullptr;
   a->D = backward ? (float*)(ws + w.D) : nullptr;
   a->slope_part = backward && d->dslopes ? (float*)(ws + w.sp) : nullptr;
-  a->parts = backward ? parts_of(d) : 1;
+  a->parts = a->qparts = 1;
+  if (backward) a->parts = parts_of(d, &a->qparts);
   a->part_k = backward ? (float*)(ws + w.pk) : nullptr;
   a->part_v = backward ? (float*)(ws + w.pv) : nullptr;
   return DMT_OK;

@@ -27,13 +27,13 @@ __device__ __forceinline__ void shaped(f32x16_t& s, f32x16_t& r2, const Shape& s
 }
 
 // dQ (and D): one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
-template <typename T, int DHP, bool SHAPED>
+template <typename T, int DHP, bool SHAPED, bool DOCS>
 __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
   constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS + PAD, VE = KT * TL::RS;
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
-  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  __shared__ __attribute__((aligned(16))) int docs[DOCS ? NB : 1][KT];
   __shared__ float part[4];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
@@ -70,24 +70,22 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
   const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
   const int nk = (lim_wg + KT - 1) / KT;
-  int qlo = 0, qhi = 0, wlo = 0, whi = 0, qd = 0;
-  const int2* kr = nullptr;
-  if (a.q_doc) {
+  int qd = 0;
+  Walk<DOCS> wk;
+  wk.hi = nk;
+  if constexpr (DOCS) {
+    wk.lo = 0;
     const int2* qr = a.q_rng + (long long)b * a.nqt;
-    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0;
-    qlo = min(r0.x, r1.x);
-    qhi = max(r0.y, r1.y);
-    const int2 rw = wave < 2 ? r0 : r1;
-    wlo = rw.x;
-    whi = rw.y;
+    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0, rw = wave < 2 ? r0 : r1;
+    wk.rng = a.k_rng + (long long)b * a.nkt;
+    wk.free_wg = wk.free_w = (e.pre + KT - 1) / KT;
+    wk.glo = min(r0.x, r1.x);
+    wk.ghi = max(r0.y, r1.y);
+    wk.wlo = rw.x;
+    wk.whi = rw.y;
+    wk.chunk = -1;
     qd = in ? a.q_doc[e.q0 + i] : 0;
-    kr = a.k_rng + (long long)b * a.nkt;
   }
-  const auto next = [&](int t) {
-    if (kr)
-      while (t < nk && t * KT >= e.pre && (kr[t].x > qhi || kr[t].y < qlo)) ++t;
-    return t;
-  };
   Stage<T, DHP> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
@@ -95,32 +93,29 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     const int k0 = t * KT;
     st.begin(K + (long long)k0 * a.k_rs, a.k_rs, V + (long long)k0 * a.v_rs, a.v_rs, min(KT, e.kl - k0), a.dh, lds + buf * (KE + VE),
              lds + buf * (KE + VE) + KE);
-    if (kr && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
+    if (DOCS && tid < KT) kd = k0 + tid < e.kl ? a.k_doc[e.k0 + k0 + tid] : 0;
   };
   const auto end = [&](int buf) {
     st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
-    if (kr && tid < KT) docs[buf][tid] = kd;
+    if (DOCS && tid < KT) docs[buf][tid] = kd;
   };
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
-  int t = next(0), buf = 0;
+  int flags = 0, buf = 0, t = wk.next(0, flags);
   if (t < nk) {
     begin(t, 0);
     end(0);
   }
   __syncthreads();
   while (t < nk) {
-    const int tn = next(t + 1), k0 = t * KT;
+    int nflags = 0;
+    const int tn = wk.next(t + 1, nflags), k0 = t * KT;
     if (tn < nk) begin(tn, NB == 2 ? buf ^ 1 : 0);
     const T* Kl = lds + buf * (KE + VE);
     const T* Vl = Kl + KE;
-    bool work = active && k0 < lim_w, docs_differ = false;
-    if (kr && k0 + KT > e.pre) {
-      if (k0 >= e.pre && (kr[t].x > whi || kr[t].y < wlo)) work = false;
-      docs_differ = !(kr[t].x == kr[t].y && wlo == whi && wlo == kr[t].x);
-    }
+    const bool work = active && k0 < lim_w && (flags & 1), docs_differ = DOCS && (flags & 2) && k0 + KT > e.pre;
     if (work) {
       const bool cut = k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off);
 #pragma unroll
@@ -175,6 +170,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     __syncthreads();
     if (NB == 2) buf ^= 1;
     t = tn;
+    flags = nflags;
   }
   float sl = 0.f;
   if (active) {
@@ -223,14 +219,16 @@ __device__ void sum_slopes(const float* part, long long n, float* out, double* r
 
 // dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
 // tiles of 64: S and dP with lane = key, P and dX packed are the B operands of dV^T += dO^T P and dK^T += Q^T dX.  Nothing crosses wavefronts.
-// WHAT: 1 = dK, 2 = dV, 3 = both.
-template <typename T, int DHP, bool SHAPED, int WHAT>
+// WHAT: 1 = dK, 2 = dV, 3 = both.  Both accumulators and both operands' rows fit the 256 registers of two wavefronts a SIMD up to 80 dims (64 in
+// fp32); wider heads take a kernel each -- one more product of scores, but at 4096 causal keys, 16 heads of 128 dims 225 + 164 us against 443 us
+// for one kernel with one wavefront a SIMD (accumulators moved between register files) and 1033 us with spills.
+template <typename T, int DHP, bool SHAPED, bool DOCS, int WHAT>
 __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, int nqt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
   constexpr int QE = KT * TL::RS + (sizeof(T) == 2 ? 0 : 32);
   __shared__ __attribute__((aligned(16))) T lds[NB * 2 * QE];
-  __shared__ __attribute__((aligned(16))) int docs[NB][KT];
+  __shared__ __attribute__((aligned(16))) int docs[DOCS ? NB : 1][KT];
   __shared__ __attribute__((aligned(16))) float stats[NB][2][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
@@ -243,7 +241,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   int head, kt;
   place(id, a.B * a.Hkv * a.parts, nt, false, head, kt);
   const int part = head % a.parts, b = head / (a.parts * a.Hkv), hk = head / a.parts - b * a.Hkv;
-  const int g0 = part_head(a, part), ng = part_head(a, part + 1) - g0;
+  const int g0 = part_head(a, part / a.qparts), ng = part_head(a, part / a.qparts + 1) - g0;
   const Ex e = example(a, b);
   if (kt * 128 >= e.kl) return;
   const int jw = kt * 128 + wave * 32, j = jw + l31;
@@ -256,33 +254,31 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   const int lo_wg = a.causal && kt * 128 >= e.pre ? max(0, kt * 128 - e.off) : 0;
   const int lo_w = a.causal && jw >= e.pre ? max(0, jw - e.off) : 0;
   const int lo_l = j >= e.kl ? 0x7fffffff : (a.causal && j >= e.pre ? max(0, j - e.off) : 0);
-  const int t0 = lo_wg / KT, nq = (e.ql + KT - 1) / KT, per = nq > t0 ? nq - t0 : 0, total = per * ng;
-  const bool free_keys = jw < e.pre;                      // some key of the wavefront is in the prefix: no document hides it
-  int klo = 0, khi = 0, wlo = 0, whi = 0, kd_l = 0;
-  const int2* qr = nullptr;
-  if (a.q_doc) {
+  const int nq = (e.ql + KT - 1) / KT, tl = lo_wg / KT, span = nq > tl ? nq - tl : 0, qp = part % a.qparts;
+  const int t0 = tl + (int)((long long)span * qp / a.qparts), t1 = tl + (int)((long long)span * (qp + 1) / a.qparts);
+  int kd_l = 0;
+  Walk<DOCS> wk;
+  wk.hi = t1;
+  if constexpr (DOCS) {
+    wk.lo = t0;
     const int2* kr = a.k_rng + (long long)b * a.nkt;
-    const int2 r0 = kr[kt * 2], r1 = kt * 2 + 1 < a.nkt ? kr[kt * 2 + 1] : r0;
-    klo = min(r0.x, r1.x);
-    khi = max(r0.y, r1.y);
-    const int2 rw = wave < 2 ? r0 : r1;
-    wlo = rw.x;
-    whi = rw.y;
+    const int2 r0 = kr[kt * 2], r1 = kt * 2 + 1 < a.nkt ? kr[kt * 2 + 1] : r0, rw = wave < 2 ? r0 : r1;
+    wk.rng = a.q_rng + (long long)b * a.nqt;
+    wk.free_wg = kt * 128 < e.pre ? t1 : 0;              // (a key of the prefix: no document hides it from any query)
+    wk.free_w = jw < e.pre ? t1 : 0;
+    wk.glo = min(r0.x, r1.x);
+    wk.ghi = max(r0.y, r1.y);
+    wk.wlo = rw.x;
+    wk.whi = rw.y;
+    wk.chunk = -1;
     kd_l = j < e.kl ? a.k_doc[e.k0 + j] : 0;
-    qr = a.q_rng + (long long)b * a.nqt;
   }
-  // step n of the walk: head n / per of the group, tile t0 + n % per
-  const auto next = [&](int n) {
-    if (qr && kt * 128 >= e.pre)
-      while (n < total && (qr[t0 + n % per].x > khi || qr[t0 + n % per].y < klo)) ++n;
-    return n;
-  };
   Stage<T, DHP> st;
   st.init(a.q_rs, a.do_rs, a.dh, tid);
   int qd = 0;
   float lse2 = 0.f;
-  const auto begin = [&](int n, int buf) {
-    const int h = hk * a.G + g0 + n / per, i0 = (t0 + n % per) * KT;
+  const auto begin = [&](int g, int t, int buf) {
+    const int h = hk * a.G + g0 + g, i0 = t * KT;
     st.begin((const T*)a.Q + (e.q0 + i0) * a.q_rs + (long long)h * a.dh, a.q_rs, (const T*)a.dout + (e.q0 + i0) * a.do_rs + (long long)h * a.dh, a.do_rs,
              min(KT, e.ql - i0), a.dh, lds + buf * 2 * QE, lds + buf * 2 * QE + QE);
     if (tid < 2 * KT) {
@@ -291,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
       if (tid < KT) {
         const float x = i < e.ql ? a.lse[stat] : -INFINITY;
         lse2 = x != -INFINITY ? x * LOG2E : INFINITY;     // (rows that see nothing, rows past the end: weight 0)
-        if (qr) qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
+        if (DOCS) qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
       } else {
         lse2 = i < e.ql ? a.D[stat] : 0.f;
       }
@@ -300,7 +296,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   const auto end = [&](int buf) {
     st.end(lds + buf * 2 * QE, lds + buf * 2 * QE + QE);
     if (tid < 2 * KT) stats[buf][tid / KT][tid & (KT - 1)] = lse2;
-    if (qr && tid < KT) docs[buf][tid] = qd;
+    if (DOCS && tid < KT) docs[buf][tid] = qd;
   };
   f32x16_t dk[WHAT & 1 ? TL::NDT : 1], dv[WHAT & 2 ? TL::NDT : 1];
 #pragma unroll
@@ -308,23 +304,28 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
     if (WHAT & 1) dk[dt] = zero16();
     if (WHAT & 2) dv[dt] = zero16();
   }
-  int n = next(0), buf = 0;
-  if (n < total) {
-    begin(n, 0);
+  // the walk: the heads of the part one after the other, each over the tiles to visit
+  int flags = 0, buf = 0, g = 0, t = wk.next(t0, flags);
+  if (t >= t1) g = ng;
+  const int first = t, first_flags = flags;
+  if (g < ng) {
+    begin(0, t, 0);
     end(0);
   }
   __syncthreads();
-  while (n < total) {
-    const int nn = next(n + 1), tq = t0 + n % per, i0 = tq * KT;
-    if (nn < total) begin(nn, NB == 2 ? buf ^ 1 : 0);
+  while (g < ng) {
+    int nflags = 0, gn = g, tn = wk.next(t + 1, nflags);
+    if (tn >= t1) {
+      ++gn;
+      tn = first;
+      nflags = first_flags;
+    }
+    const int i0 = t * KT;
+    if (gn < ng) begin(gn, tn, NB == 2 ? buf ^ 1 : 0);
     const T* Ql = lds + buf * 2 * QE;
     const T* Gl = Ql + QE;
-    const Shape sh = shape_of(a, hk * a.G + g0 + n / per);
-    bool work = active && i0 + KT > lo_w, docs_differ = false;
-    if (qr) {
-      if (!free_keys && (qr[tq].x > whi || qr[tq].y < wlo)) work = false;
-      docs_differ = jw + 32 > e.pre && !(qr[tq].x == qr[tq].y && wlo == whi && wlo == qr[tq].x);
-    }
+    const Shape sh = shape_of(a, hk * a.G + g0 + g);
+    const bool work = active && i0 + KT > lo_w && (flags & 1), docs_differ = DOCS && (flags & 2) && jw + 32 > e.pre;
     if (work) {
       const bool cut = jw + 32 > e.kl || (a.causal && jw + 32 > e.pre && i0 + e.off < jw + 31);
 #pragma unroll
@@ -374,10 +375,12 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
       }
     }
     if (NB == 1) __syncthreads();
-    if (nn < total) end(NB == 2 ? buf ^ 1 : 0);
+    if (gn < ng) end(NB == 2 ? buf ^ 1 : 0);
     __syncthreads();
     if (NB == 2) buf ^= 1;
-    n = nn;
+    g = gn;
+    t = tn;
+    flags = nflags;
   }
   if (!active) return;
   const bool in = j < e.kl;
@@ -406,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   unsigned long long again = __ballot(in && !(bad == 0.f));
   again |= again >> 32;
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_dkv<T>(*args_again(), e, hk, part, jw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1) row_dkv<T>(*args_again(), e, hk, part, t0 * KT, min(e.ql, t1 * KT), jw + r, (float*)lds + wave * ROW_LDS, lane);
 }
 
 // dK = scale (sum of its parts), dV = sum of its parts, in their order: 16 key rows of one example a workgroup
@@ -434,21 +437,27 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
 
 template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  if (a.cap > 0.f || a.slopes) tile_dq_kernel<T, DHP, true><<<grid, 256, 0, st>>>(a, nt);
-  else tile_dq_kernel<T, DHP, false><<<grid, 256, 0, st>>>(a, nt);
+  const bool shaped = a.cap > 0.f || a.slopes;
+  if (shaped && a.q_doc) tile_dq_kernel<T, DHP, true, true><<<grid, 256, 0, st>>>(a, nt);
+  else if (shaped) tile_dq_kernel<T, DHP, true, false><<<grid, 256, 0, st>>>(a, nt);
+  else if (a.q_doc) tile_dq_kernel<T, DHP, false, true><<<grid, 256, 0, st>>>(a, nt);
+  else tile_dq_kernel<T, DHP, false, false><<<grid, 256, 0, st>>>(a, nt);
 }
-template <typename T, int DHP, bool SHAPED> void launch_dkv_as(const Args& a, int nt, int nqt, hipStream_t st) {
+template <typename T, int DHP, bool SHAPED, bool DOCS> void launch_dkv_as(const Args& a, int nt, int nqt, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
-  if (DHP * sizeof(T) > 160) {
-    tile_dkv_kernel<T, DHP, SHAPED, 2><<<grid, 256, 0, st>>>(a, nt, nqt);
-    tile_dkv_kernel<T, DHP, SHAPED, 1><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+  if constexpr (DHP > (sizeof(T) == 2 ? 80 : 64)) {
+    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 2><<<grid, 256, 0, st>>>(a, nt, nqt);
+    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 1><<<grid + more, 256, 0, st>>>(a, nt, nqt);
   } else {
-    tile_dkv_kernel<T, DHP, SHAPED, 3><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 3><<<grid + more, 256, 0, st>>>(a, nt, nqt);
   }
 }
 template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
-  if (a.cap > 0.f || a.slopes) launch_dkv_as<T, DHP, true>(a, nt, nqt, st);
-  else launch_dkv_as<T, DHP, false>(a, nt, nqt, st);
+  const bool shaped = a.cap > 0.f || a.slopes;
+  if (shaped && a.q_doc) launch_dkv_as<T, DHP, true, true>(a, nt, nqt, st);
+  else if (shaped) launch_dkv_as<T, DHP, true, false>(a, nt, nqt, st);
+  else if (a.q_doc) launch_dkv_as<T, DHP, false, true>(a, nt, nqt, st);
+  else launch_dkv_as<T, DHP, false, false>(a, nt, nqt, st);
 }
 
 template <typename T>
