@@ -49,26 +49,38 @@ struct PlanArgs {
 };
 __device__ __forceinline__ int free_count(const PlanArgs& a) { return a.n_free[0] < a.free_cap ? a.n_free[0] : a.free_cap; }
 
-__device__ __forceinline__ long long wg_scan(long long v, long long* red, int tid, long long& total) {
-  // inclusive sum over the workgroup
+// Inclusive sums of two values over the workgroup: a Kogge-Stone scan by DPP within a wavefront, the wavefronts' sums through LDS (each wavefront
+// scans the 16 of them itself: one barrier).
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast:15 into rows 1, 3; row_bcast:31 into rows 2, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+struct Pair { int a, b, ta, tb; };     // inclusive sums, totals
+__device__ __forceinline__ Pair wg_scan(int a, int b, int (*red)[2][PLAN_NT / 64], int& turn, int tid) {
   const int lane = tid & 63, wave = tid >> 6;
-  long long x = v;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const long long y = __shfl_up(x, s);
-    if (lane >= s) x += y;
+  Pair p;
+  p.a = wave_scan(a);
+  p.b = wave_scan(b);
+  int (*rd)[PLAN_NT / 64] = red[turn];
+  turn ^= 1;                           // (two sets of slots: one barrier a scan)
+  if (lane == 63) {
+    rd[0][wave] = p.a;
+    rd[1][wave] = p.b;
   }
   __syncthreads();
-  if (lane == 63) red[wave] = x;
-  __syncthreads();
-  long long base = 0, all = 0;
-  for (int w = 0; w < PLAN_NT / 64; ++w) {
-    const long long r = red[w];
-    if (w < wave) base += r;
-    all += r;
+  const int l16 = lane & 15, sa = wave_scan(lane < 16 ? rd[0][l16] : 0), sb = wave_scan(lane < 16 ? rd[1][l16] : 0);
+  p.ta = __builtin_amdgcn_readlane(sa, 15);
+  p.tb = __builtin_amdgcn_readlane(sb, 15);
+  if (wave > 0) {
+    p.a += __builtin_amdgcn_readlane(sa, wave - 1);
+    p.b += __builtin_amdgcn_readlane(sb, wave - 1);
   }
-  total = all;
-  return x + base;
+  return p;
 }
 
 __device__ void plan_rows(const PlanArgs& a, int t, int step, int total, int runs) {
@@ -105,48 +117,59 @@ __device__ void plan_rows(const PlanArgs& a, int t, int step, int total, int run
   }
 }
 
+// (The row counts are scanned in two halves of 16 bits: 1024 of them cannot pass 31 bits then.  Blocks and runs of requests that fit are bounded by
+// the rows, fewer than 2^30.)
 __global__ __launch_bounds__(PLAN_NT) void plan_kernel(const PlanArgs a, int small) {
-  __shared__ long long red[PLAN_NT / 64];
+  __shared__ int red[2][2][PLAN_NT / 64];
   const int tid = threadIdx.x;
-  long long row_base = 0, need_base = 0, run_base = 0, taken = 0, refused = 0, tot;
-  const long long n_free = free_count(a);
+  int turn = 0;
+  long long row_base = 0, need_base = 0;
+  int run_base = 0, taken = 0, refused = 0;
+  const int n_free = free_count(a);
   for (int r0 = 0; r0 < a.n; r0 += PLAN_NT) {
     const int r = r0 + tid;
     const bool in = r < a.n;
     const int len = in ? a.lens[r] : 0, nw = in ? a.new_lens[r] : 0;
-    const long long rows = nw > 0 ? nw : 0;
-    const long long row_end = row_base + wg_scan(rows, red, tid, tot);
-    row_base += tot;
+    const int rows = nw > 0 ? nw : 0;
+    long long row_end;
+    Pair p;
+    {
+      p = wg_scan(rows & 0xffff, rows >> 16, red, turn, tid);
+      row_end = row_base + p.a + ((long long)p.b << 16);
+      row_base += p.ta + ((long long)p.tb << 16);
+    }
     const bool fits = in && nw >= 0 && len >= 0 && (long long)len + nw <= (long long)a.width * BS && row_end <= a.rows;
-    const long long need = fits ? ((long long)len + nw + BS - 1) / BS - ((long long)len + BS - 1) / BS : 0;
-    const long long need_end = need_base + wg_scan(need, red, tid, tot);
-    need_base += tot;
+    // (fits: len + nw <= 64 width < 2^37, so blocks < 2^31 / 64 when it matters; rows <= a.rows < 2^30)
+    const int blocks_end = fits ? (int)(((long long)len + nw + BS - 1) / BS) : 0, have = fits ? (int)(((long long)len + BS - 1) / BS) : 0;
+    const int need = blocks_end - have;
+    p = wg_scan(need, 0, red, turn, tid);
+    const long long need_end = need_base + p.a;
+    need_base += p.ta;
     const bool ok = fits && (need == 0 || need_end <= n_free);
-    const long long runs = ok && nw > 0 ? ((long long)len + nw + BS - 1) / BS - len / BS : 0;
-    const long long run_end = run_base + wg_scan(runs, red, tid, tot);
-    run_base += tot;
-    wg_scan(ok ? need : 0, red, tid, tot);
-    taken += tot;
-    wg_scan(in && !ok ? 1 : 0, red, tid, tot);
-    refused += tot;
+    const int runs = ok && nw > 0 ? blocks_end - len / BS : 0;
+    p = wg_scan(runs, (ok ? need : 0), red, turn, tid);
+    const int run_first = run_base + p.a - runs;
+    run_base += p.ta;
+    taken += p.tb;
+    refused += __syncthreads_count(in && !ok);
     if (in) {
       const long long row_first = row_end - rows;
       a.row_off[r] = (int)(row_first < 0x7fffffffll ? row_first : 0x7fffffffll);
       if (r == a.n - 1) a.row_off[a.n] = (int)(row_end < 0x7fffffffll ? row_end : 0x7fffffffll);
       a.lens_out[r] = ok ? len + nw : len;
-      a.req[r] = make_int2(ok ? (int)(need_end - need) : -1, (int)(run_end - runs));
+      a.req[r] = make_int2(ok ? (int)(need_end - need) : -1, run_first);
     }
   }
   if (tid == 0) {
     if (a.n == 0) a.row_off[0] = 0;
-    a.state[0] = (int)(n_free - taken);
-    a.state[1] = (int)refused;
-    a.totals[0] = (int)run_base;
+    a.state[0] = n_free - taken;
+    a.state[1] = refused;
+    a.totals[0] = run_base;
   }
   if (small) {
     __threadfence_block();
     __syncthreads();
-    plan_rows(a, tid, PLAN_NT, row_base < 0x7fffffffll ? (int)row_base : 0x7fffffff, (int)run_base);
+    plan_rows(a, tid, PLAN_NT, row_base < 0x7fffffffll ? (int)row_base : 0x7fffffff, run_base);
   }
 }
 
@@ -156,19 +179,21 @@ __global__ __launch_bounds__(256) void plan_rows_kernel(const PlanArgs a) {
 
 __global__ __launch_bounds__(PLAN_NT) void release_kernel(int n, const int* done, int* lens, const int* table, int width, int* free_ids, int* n_free,
                                                           int cap) {
-  __shared__ long long red[PLAN_NT / 64];
+  __shared__ int red[2][2][PLAN_NT / 64];
   const int tid = threadIdx.x;
-  long long base = n_free[0], tot;
+  int turn = 0;
+  long long base = n_free[0];
   for (int r0 = 0; r0 < n; r0 += PLAN_NT) {
     const int r = r0 + tid;
     const bool in = r < n && done[r] != 0 && lens[r] > 0;
-    long long mine = in ? ((long long)lens[r] + BS - 1) / BS : 0;
-    if (mine > width) mine = width;
-    const long long end = base + wg_scan(mine, red, tid, tot);
-    base += tot;
+    long long held = in ? ((long long)lens[r] + BS - 1) / BS : 0;
+    const int mine = (int)(held > width ? width : held);
+    const Pair p = wg_scan(mine & 0xffff, mine >> 16, red, turn, tid);
+    const long long end = base + p.a + ((long long)p.b << 16);
+    base += p.ta + ((long long)p.tb << 16);
     if (in) {
       long long at = end - mine;
-      for (int j = 0; j < (int)mine; ++j, ++at)
+      for (int j = 0; j < mine; ++j, ++at)
         if (at >= 0 && at < cap) free_ids[at] = table[(long long)r * width + j];
       lens[r] = 0;
     }
@@ -184,11 +209,13 @@ struct Cache {
   float* ks; float* vs;
 };
 
-// One workgroup owns a (run, head): its rows are held in registers between the maximum and the rounding.
+// One workgroup owns a (run, head): its rows are held in registers between the maximum and the rounding.  What bounds it is the rows' bytes; the
+// bytes of V pass through LDS because they lie across the tokens (68 bytes a dim there: the 16 chunks of a row would meet in one bank at 64).
+constexpr int VLD = BS + 4;
 __global__ __launch_bounds__(256) void append_kernel(const Cache c, int rows, const bf16_t* kr, long long k_rs, const bf16_t* vr, long long v_rs,
                                                      const int* slots, const int* run_row, const int* run_len) {
   __shared__ float red[2][4];
-  __shared__ __attribute__((aligned(16))) unsigned char vt[MAX_DH * BS];
+  __shared__ __attribute__((aligned(16))) unsigned char vt[MAX_DH * VLD];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = blockIdx.y, dh = c.dh, ch = dh / 8;
   const int row0 = run_row[blockIdx.x];
   int len = run_len[blockIdx.x];
@@ -249,12 +276,21 @@ __global__ __launch_bounds__(256) void append_kernel(const Cache c, int rows, co
     }
   }
   // V: the block passes through LDS (its bytes lie across the tokens)
-  for (int x = tid * 16; x < dh * BS; x += 4096) *reinterpret_cast<uint4*>(vt + x) = *reinterpret_cast<const uint4*>(vb + x);
-  __syncthreads();
+  if (len < BS) {
+    for (int x = tid * 16; x < dh * BS; x += 4096) {
+      const uint4 w = *reinterpret_cast<const uint4*>(vb + x);
+      unsigned* d = reinterpret_cast<unsigned*>(vt + (x / BS) * VLD + x % BS);
+      d[0] = w.x;
+      d[1] = w.y;
+      d[2] = w.z;
+      d[3] = w.w;
+    }
+    __syncthreads();
+  }
   if (v_grow) {
     const float f = vs0 * vi;
     for (int x = tid; x < dh * first; x += 256) {
-      const int dd = x / first, at = dd * BS + place_of(x - dd * first);
+      const int dd = x / first, at = dd * VLD + place_of(x - dd * first);
       vt[at] = (unsigned char)f32_to_f8x2(f8_to_f32(vt[at]) * f, 0.f);
     }
     __syncthreads();
@@ -271,44 +307,62 @@ __global__ __launch_bounds__(256) void append_kernel(const Cache c, int rows, co
       for (int e = 0; e < 4; ++e) {
         o[e >> 1] |= f32_to_f8x2(__uint_as_float(kw[e] << 16) * ki, __uint_as_float(kw[e] & 0xffff0000u) * ki) << (16 * (e & 1));
         const unsigned y = f32_to_f8x2(__uint_as_float(vw[e] << 16) * vi, __uint_as_float(vw[e] & 0xffff0000u) * vi);
-        vt[(q * 8 + 2 * e) * BS + pl] = (unsigned char)y;
-        vt[(q * 8 + 2 * e + 1) * BS + pl] = (unsigned char)(y >> 8);
+        vt[(q * 8 + 2 * e) * VLD + pl] = (unsigned char)y;
+        vt[(q * 8 + 2 * e + 1) * VLD + pl] = (unsigned char)(y >> 8);
       }
       *reinterpret_cast<uint2*>(kb + (long long)(first + t) * dh + q * 8) = make_uint2(o[0], o[1]);
     }
   }
   __syncthreads();
-  for (int x = tid * 16; x < dh * BS; x += 4096) *reinterpret_cast<uint4*>(vb + x) = *reinterpret_cast<const uint4*>(vt + x);
+  for (int x = tid * 16; x < dh * BS; x += 4096) {
+    const unsigned* d = reinterpret_cast<const unsigned*>(vt + (x / BS) * VLD + x % BS);
+    *reinterpret_cast<uint4*>(vb + x) = make_uint4(d[0], d[1], d[2], d[3]);
+  }
 }
 
-// A workgroup reads 64 listed slots of one head: K a lane per 8 dims, V a lane per slot (the tokens of a block share its 64-byte rows).
+// A workgroup reads 64 listed slots of one head.  V lies across the tokens: when the slots are a whole block in order (how a caller looks at a
+// block) its bytes come in 16-byte loads, 4 x 4 tokens of one dim each, and are turned around in LDS; else a lane per slot gathers bytes.
 __global__ __launch_bounds__(256) void read_kernel(const Cache c, int n, const int* slots, bf16_t* kr, long long k_rs, bf16_t* vr, long long v_rs) {
   __shared__ __attribute__((aligned(16))) bf16_t tile[64 * (MAX_DH + 8)];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = blockIdx.y, dh = c.dh, ch = dh / 8, ld = dh + 8;
   const int i0 = blockIdx.x * 64;
   const int cnt = n - i0 < 64 ? n - i0 : 64;
-  for (int x = tid; x < cnt * ch; x += 256) {
-    const int i = x / ch, q = x - i * ch, slot = slots[i0 + i], block = slot / BS;
-    uint4 o = make_uint4(0u, 0u, 0u, 0u);
-    if (slot >= 0 && block < c.n_blocks) {
-      const long long bh = (long long)block * c.Hkv + hk;
-      const uint2 w = *reinterpret_cast<const uint2*>(c.k + (bh * BS + slot % BS) * dh + q * 8);
-      const float s = c.ks[bh];
-      unsigned* ow = reinterpret_cast<unsigned*>(&o);
+  const int slot = lane < cnt ? slots[i0 + lane] : -1, block = slot >= 0 ? slot / BS : -1;
+  const bool ok = slot >= 0 && block < c.n_blocks;
+  const long long bh = ok ? (long long)block * c.Hkv + hk : 0;
+  const int slot0 = __builtin_amdgcn_readfirstlane(slot);
+  const bool whole = slot0 % BS == 0 && __all(ok && slot == slot0 + lane);
+  const float vs = ok ? c.vs[bh] : 0.f;
+  if (whole) {
+    const uint8_t* src = c.v + bh * BS * dh;
+    for (int x = tid; x < dh * 4; x += 256) {
+      const int j = x >> 2, b = x & 3;
+      const uint4 w = *reinterpret_cast<const uint4*>(src + j * BS + 16 * b);
+      const unsigned d[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned h = (e < 2 ? w.x : w.y) >> (16 * (e & 1));
-        ow[e] = dmt_pack_bf16(f8_to_f32(h & 255) * s, f8_to_f32((h >> 8) & 255) * s);
-      }
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[(16 * q + 4 * b + e) * ld + j] = f2bf(f8_to_f32((d[q] >> (8 * e)) & 255) * vs);
+    }
+  } else {
+    const uint8_t* src = c.v + bh * BS * dh + (ok ? place_of(slot % BS) : 0);
+    for (int j = wave; j < dh; j += 4) tile[lane * ld + j] = ok ? f2bf(f8_to_f32(src[(long long)j * BS]) * vs) : (bf16_t)0;
+  }
+  for (int x = tid; x < cnt * ch; x += 256) {
+    const int i = x / ch, q = x - i * ch, sl = slots[i0 + i], bl = sl >= 0 ? sl / BS : -1;
+    uint4 o = make_uint4(0u, 0u, 0u, 0u);
+    if (sl >= 0 && bl < c.n_blocks) {
+      const long long b2 = (long long)bl * c.Hkv + hk;
+      const uint2 w = *reinterpret_cast<const uint2*>(c.k + (b2 * BS + sl % BS) * dh + q * 8);
+      const float s = c.ks[b2];
+      const unsigned lo = w.x, hi = w.y;
+      o.x = dmt_pack_bf16(f8_to_f32(lo & 255) * s, f8_to_f32((lo >> 8) & 255) * s);
+      o.y = dmt_pack_bf16(f8_to_f32((lo >> 16) & 255) * s, f8_to_f32(lo >> 24) * s);
+      o.z = dmt_pack_bf16(f8_to_f32(hi & 255) * s, f8_to_f32((hi >> 8) & 255) * s);
+      o.w = dmt_pack_bf16(f8_to_f32((hi >> 16) & 255) * s, f8_to_f32(hi >> 24) * s);
     }
     *reinterpret_cast<uint4*>(kr + (long long)(i0 + i) * k_rs + (long long)hk * dh + q * 8) = o;
   }
-  const int slot = lane < cnt ? slots[i0 + lane] : -1, block = slot / BS;
-  const bool ok = slot >= 0 && block < c.n_blocks;
-  const long long bh = ok ? (long long)block * c.Hkv + hk : 0;
-  const float s = ok ? c.vs[bh] : 0.f;
-  const uint8_t* src = c.v + bh * BS * dh + (ok ? place_of(slot % BS) : 0);
-  for (int j = wave; j < dh; j += 4) tile[lane * ld + j] = ok ? f2bf(f8_to_f32(src[(long long)j * BS]) * s) : (bf16_t)0;
   __syncthreads();
   for (int x = tid; x < cnt * ch; x += 256) {
     const int i = x / ch, q = x - i * ch;
