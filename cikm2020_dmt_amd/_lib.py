@@ -142,7 +142,7 @@ class AttnVarDesc(C.Structure):
                 ("rows_q", c_i64), ("rows_k", c_i64), ("Q", c_vp), ("q_rs", c_i64), ("K", c_vp), ("k_rs", c_i64), ("V", c_vp), ("v_rs", c_i64),
                 ("q_off", c_vp), ("q_lens", c_vp), ("k_off", c_vp), ("k_lens", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32),
                 ("slopes", c_vp), ("prefix", c_vp), ("q_doc", c_vp), ("k_doc", c_vp), ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp),
-                ("dout", c_vp), ("do_rs", c_i64), ("dQ", c_vp), ("dq_rs", c_i64), ("dK", c_vp), ("dk_rs", c_i64),
+                ("out_lo", c_vp), ("dout", c_vp), ("do_rs", c_i64), ("dQ", c_vp), ("dq_rs", c_i64), ("dK", c_vp), ("dk_rs", c_i64),
                 ("dV", c_vp), ("dv_rs", c_i64), ("dslopes", c_vp), ("doc_ranges", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
 
 
@@ -348,4 +348,6 @@ def check(rc: int, what: str = ""):
 
 
 def call(name: str, *args):
-    check(getattr(load(), name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc != 0:
+        check(rc, name)

@@ -27,6 +27,7 @@ struct Args {
   const int* q_doc; const int* k_doc;
   void* out; long long o_rs;
   float* lse;
+  void* out_lo;
   const void* dout; long long do_rs;
   void* dQ; long long dq_rs;
   void* dK; long long dk_rs;
@@ -173,6 +174,7 @@ __device__ void row_fwd(const Args& a, const Ex& e, int h, int i, float* lds, in
     if (c < dh) {
       const float o = (u ? o1 : o0) * inv;
       stf<T>(O + c, o);
+      if (sizeof(T) == 2 && a.out_lo) stf<T>((T*)a.out_lo + (row * a.Hq + h) * dh + c, o - bf2f(f2bf(o)));
     }
   }
   if (a.lse && lane == 0) a.lse[row * a.Hq + h] = (m == -INFINITY && l == 0.f) ? -INFINITY : (m + __log2f(l)) * LN2;

@@ -187,6 +187,18 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     T* O = (T*)a.out + row * a.o_rs + (long long)h * a.dh;
 #pragma unroll
     for (int dt = 0; dt < TL::NDT; ++dt) store_dims<T>(o[dt], inv, O, dt, half, a.dh);
+    if (sizeof(T) == 2 && a.out_lo) {
+      T* L = (T*)a.out_lo + (row * a.Hq + h) * a.dh;
+#pragma unroll
+      for (int dt = 0; dt < TL::NDT; ++dt) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = o[dt][r] * inv;
+          o[dt][r] = x - bf2f(f2bf(x));
+        }
+        store_dims<T>(o[dt], 1.f, L, dt, half, a.dh);
+      }
+    }
     if (a.lse && half == 0) a.lse[row * a.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
   }
   unsigned long long again = __ballot(in && !(bad == 0.f));
@@ -314,6 +326,7 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
                   "%s: bad gradient row stride", what);
     DMT_CHECK_ARG(al16(d->dout, d->do_rs, es) && al16(d->dQ, d->dq_rs, es) && al16(d->dK, d->dk_rs, es) && al16(d->dV, d->dv_rs, es),
                   "%s: gradient rows must be 16-byte aligned", what);
+    DMT_CHECK_ARG((uintptr_t)d->out_lo % 16 == 0, "%s: out_lo must be 16-byte aligned", what);
     DMT_CHECK_ARG(!d->dslopes || d->slopes, "%s: dslopes without slopes", what);
   }
   DMT_CHECK_ARG(!d->q_doc || (d->doc_ranges && ((uintptr_t)d->doc_ranges % 16) == 0), "%s: documents need doc_ranges (16-byte aligned)", what);
@@ -330,7 +343,7 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   a->q_off = d->q_off; a->q_lens = d->q_lens; a->k_off = d->k_off; a->k_lens = d->k_lens;
   a->scale = d->scale; a->cap = d->cap; a->causal = d->causal != 0; a->slopes = d->slopes; a->prefix = d->prefix;
   a->q_doc = d->q_doc; a->k_doc = d->k_doc;
-  a->out = d->out; a->o_rs = d->o_rs; a->lse = d->lse;
+  a->out = d->out; a->o_rs = d->o_rs; a->lse = d->lse; a->out_lo = d->dtype == DMT_BF16 ? d->out_lo : nullptr;
   a->dout = d->dout; a->do_rs = d->do_rs; a->dQ = d->dQ; a->dq_rs = d->dq_rs; a->dK = d->dK; a->dk_rs = d->dk_rs; a->dV = d->dV; a->dv_rs = d->dv_rs;
   a->dslopes = d->dslopes;
   a->nqt = (int)cdiv64(d->max_q, 64);

@@ -62,6 +62,12 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, i, half);
 #pragma unroll
     for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
+    if (sizeof(T) == 2 && a.out_lo) {
+      const long long ls = (long long)a.Hq * a.dh;
+      own_row<T, DHP>(ov, (const T*)a.out_lo + e.q0 * ls + (long long)h * a.dh, ls, e.ql, a.dh, i, half);
+#pragma unroll
+      for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
+    }
     D += other_half(D);
     if (in && half == 0) a.D[stat] = D;
   }

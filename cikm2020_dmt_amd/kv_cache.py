@@ -17,10 +17,19 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .ops import BF16, F32, p, stream_ptr
+from .ops import BF16, F32, _cur_device, _raw_stream, p
 
 BLOCK = L.DMT_KV_BLOCK
 F8 = torch.float8_e4m3fn
+
+
+def _call(device, name, *args):
+    """one entry point on the device's current stream (with that device current)"""
+    if _cur_device() == device.index:
+        L.call(name, *args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            L.call(name, *args, _raw_stream(_cur_device()))
 
 
 class KVCache:
@@ -42,15 +51,14 @@ class KVCache:
             raise ValueError("the cache lives on one GPU")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_blocks, self.Hkv, self.dh, self.device = n, Hkv, dh, k.device
+        self._ws_bytes = {}
+        self._args = (Hkv, dh, n, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
 
     @classmethod
     def empty(cls, n_blocks, Hkv, dh, device="cuda"):
         z = lambda *s: torch.zeros(s, dtype=torch.uint8, device=device).view(F8)  # noqa: E731
         return cls(z(n_blocks, Hkv, BLOCK, dh), z(n_blocks, Hkv, dh, BLOCK), torch.ones((n_blocks, Hkv), device=device),
                    torch.ones((n_blocks, Hkv), device=device))
-
-    def _args(self):
-        return (self.Hkv, self.dh, self.n_blocks, p(self.k), p(self.v), p(self.k_scale), p(self.v_scale))
 
 
 class KVPlan(NamedTuple):
@@ -66,7 +74,7 @@ class KVPlan(NamedTuple):
 
 
 def _i32(t, shape, what, device):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError("%s must be a contiguous int32 tensor %s on %s, got %s %s on %s" % (what, list(shape), device, t.dtype, list(t.shape), t.device))
 
 
@@ -86,19 +94,19 @@ def kv_plan(lens, new_lens, table, free, n_free, rows) -> KVPlan:
     if not 0 <= rows < 2 ** 30:
         raise ValueError("rows must lie in 0 .. 2^30 - 1, got %d" % rows)
     runs = min(rows, rows // BLOCK + 2 * n)
-    need = int(L.load().dmt_kv_plan_ws_bytes(n))
+    need = 16 + 8 * n                                                            # dmt_kv_plan_ws_bytes
     sizes = (n + 1, n, rows, runs, runs, 1, 1)
     buf = torch.empty(need // 4 + sum(sizes), dtype=torch.int32, device=dev)     # one allocation: the step is a matter of microseconds
     base = buf.data_ptr()
-    out = torch.split(buf, (need // 4,) + sizes)[1:]
-    at, o = [], base + need
-    for s in sizes:
-        at.append(o)
-        o += 4 * s
-    with torch.cuda.device(dev):
-        L.call("dmt_kv_plan", n, rows, p(lens), p(new_lens), p(table), width, p(free), free.numel(), p(n_free), at[0], at[1], at[2], at[3], at[4],
-               at[5], base, need, stream_ptr())
-    return KVPlan(*out)
+    out = torch.split_with_sizes(buf, (need // 4,) + sizes)
+    a0 = base + need
+    a1 = a0 + 4 * (n + 1)
+    a2 = a1 + 4 * n
+    a3 = a2 + 4 * rows
+    a4 = a3 + 4 * runs
+    _call(dev, "dmt_kv_plan", n, rows, lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(), width, free.data_ptr(), free.shape[0],
+          n_free.data_ptr(), a0, a1, a2, a3, a4, a4 + 4 * runs, base, need)
+    return KVPlan(*out[1:])
 
 
 def kv_release(done, lens, table, free, n_free):
@@ -109,12 +117,11 @@ def kv_release(done, lens, table, free, n_free):
     _i32(table, (n, table.shape[1]), "table", dev)
     _i32(free, (free.numel(),), "free", dev)
     _i32(n_free, (1,), "n_free", dev)
-    with torch.cuda.device(dev):
-        L.call("dmt_kv_release", n, p(done), p(lens), p(table), table.shape[1], p(free), p(n_free), free.numel(), stream_ptr())
+    _call(dev, "dmt_kv_release", n, p(done), p(lens), p(table), table.shape[1], p(free), p(n_free), free.numel())
 
 
 def _rows(t, what, width, device):
-    if t.dim() != 2 or t.dtype != BF16 or t.shape[1] != width or t.device != device or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dim() != 2 or t.dtype is not BF16 or t.shape[1] != width or t.device != device or t.stride(1) != 1:
         raise ValueError("%s must be bf16 rows [., %d] with unit inner stride on %s, got %s %s on %s" % (what, width, device, t.dtype, list(t.shape), t.device))
     rs = t.stride(0) if t.shape[0] > 1 else width
     if t.data_ptr() % 16 or rs % 8 or rs < width:
@@ -132,18 +139,17 @@ def kv_append(cache: KVCache, k_rows, v_rows, plan: KVPlan):
     runs = plan.run_row.shape[0]
     for t, s, what in ((plan.slots, rows, "slots"), (plan.run_row, runs, "run_row"), (plan.run_len, runs, "run_len")):
         _i32(t, (s,), what, dev)
-    with torch.cuda.device(dev):
-        L.call("dmt_kv_append", *cache._args(), rows, p(k_rows), krs, p(v_rows), vrs, p(plan.slots), p(plan.run_row), p(plan.run_len), runs,
-               stream_ptr())
+    _call(dev, "dmt_kv_append", *cache._args, rows, k_rows.data_ptr(), krs, v_rows.data_ptr(), vrs, plan.slots.data_ptr(),
+          plan.run_row.data_ptr(), plan.run_len.data_ptr(), runs)
 
 
 def kv_read(cache: KVCache, slots):
     """(k_rows, v_rows) bf16 [n, Hkv * dh]: the values that stand in `slots` (int32 [n]), exactly; zeros for a slot outside the pool."""
     n, w = slots.shape[0], cache.Hkv * cache.dh
     _i32(slots, (n,), "slots", cache.device)
-    k, v = (torch.empty((n, w), dtype=BF16, device=cache.device) for _ in range(2))
-    with torch.cuda.device(cache.device):
-        L.call("dmt_kv_read", *cache._args(), n, p(slots), p(k), w, p(v), w, stream_ptr())
+    k = torch.empty((n, w), dtype=BF16, device=cache.device)
+    v = torch.empty_like(k)
+    _call(cache.device, "dmt_kv_read", *cache._args, n, slots.data_ptr(), k.data_ptr(), w, v.data_ptr(), w)
     return k, v
 
 
@@ -169,23 +175,26 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
         raise ValueError("scale must be positive and finite, cap 0 or positive and finite: got %r, %r" % (scale, cap))
     if max_q < 0 or (max_len is not None and max_len < 0):
         raise ValueError("max_q and max_len must not be negative")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty((q.shape[0], w), dtype=BF16, device=dev)
     elif out.shape != q.shape:
         raise ValueError("out must be %s" % list(q.shape))
-    o_rs = _rows(out, "out", w, dev)
+    o_rs = _rows(out, "out", w, dev) if given else w
     lse = torch.empty((q.shape[0], H), dtype=F32, device=dev) if want_lse else None
-    d = L.KvAttnDesc()
-    d.n, d.Hq, d.Hkv, d.dh, d.n_blocks = n, H, cache.Hkv, cache.dh, cache.n_blocks
-    d.max_q, d.width, d.rows = int(max_q), table.shape[1], q.shape[0]
-    d.max_len = min(int(max_len) if max_len is not None else 0x7FFFFFFF, table.shape[1] * BLOCK)
-    d.k, d.v, d.k_scale, d.v_scale = cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr()
-    d.Q, d.q_rs, d.table, d.lens, d.row_off = q.data_ptr(), q_rs, table.data_ptr(), lens.data_ptr(), row_off.data_ptr()
-    d.scale, d.cap, d.causal, d.slopes = scale, float(cap), 1 if causal else 0, p(slopes)
-    d.out, d.o_rs, d.lse = out.data_ptr(), o_rs, p(lse)
-    need = int(L.load().dmt_kv_attn_ws_bytes(C.byref(d)))
+    most = table.shape[1] * BLOCK
+    max_len = most if max_len is None else min(int(max_len), most)
+    key = (n, H, int(max_q), max_len)
+    need = cache._ws_bytes.get(key)
+    if need is None:                   # (a function of the sizes alone)
+        d = L.KvAttnDesc()
+        d.n, d.Hq, d.Hkv, d.dh, d.max_q, d.max_len = n, H, cache.Hkv, cache.dh, int(max_q), max_len
+        need = cache._ws_bytes[key] = int(L.load().dmt_kv_attn_ws_bytes(C.byref(d)))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    d.ws, d.ws_bytes = p(ws), need
-    with torch.cuda.device(dev):
-        L.call("dmt_kv_attn", C.byref(d), stream_ptr())
+    a = cache._args
+    d = L.KvAttnDesc(n, H, a[0], a[1], a[2], int(max_q), max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
+                     table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0,
+                     None if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, None if lse is None else lse.data_ptr(),
+                     None if ws is None else ws.data_ptr(), need)
+    _call(dev, "dmt_kv_attn", C.byref(d))
     return (out, lse) if want_lse else out

@@ -1256,7 +1256,7 @@ def _aligned_rows(t):
     return t.contiguous()
 
 
-def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, cfg):
+def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg):
     H, Hkv, scale, cap, causal, max_q, max_k = cfg
     d = L.AttnVarDesc()
     d.dtype, d.B, d.Hq, d.Hkv, d.dh, d.max_q, d.max_k = dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k
@@ -1267,7 +1267,7 @@ def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, c
     d.q_lens, d.q_off, d.k_lens, d.k_off = (x.data_ptr() for x in lens)
     d.scale, d.cap, d.causal = scale, cap, 1 if causal else 0
     d.slopes, d.prefix, d.q_doc, d.k_doc = (x.data_ptr() if x is not None else None for x in (slopes, prefix, q_doc, k_doc))
-    d.out, d.o_rs, d.lse, d.doc_ranges = out.data_ptr(), out.shape[1], p(lse), p(rng)
+    d.out, d.o_rs, d.lse, d.out_lo, d.doc_ranges = out.data_ptr(), out.shape[1], p(lse), p(lo), p(rng)
     return d
 
 
@@ -1290,10 +1290,11 @@ class AttnVarFn(torch.autograd.Function):
         lse = torch.full((rows, H), -float("inf"), device=q.device) if fill[0] else torch.empty((rows, H), dtype=F32, device=q.device)
         need_sl = slopes is not None and ctx.needs_input_grad[3]
         lens = (q_lens, q_off, k_lens, k_off)
+        lo = torch.empty_like(out) if q.dtype != F32 and any(ctx.needs_input_grad[:4]) else None
         rng = _var_doc_ranges(q_doc, q_lens.shape[0], cfg[5], cfg[6])
-        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, cfg)
+        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg)
         L.call("dmt_attn_var_fwd", C.byref(desc), stream_ptr())
-        ctx.save_for_backward(q, k, v, slopes, prefix, q_doc, k_doc, rng, *lens, out, lse)
+        ctx.save_for_backward(q, k, v, slopes, prefix, q_doc, k_doc, rng, *lens, out, lse, lo)
         ctx.cfg, ctx.fill, ctx.need_sl, ctx.k_shared = cfg, fill, need_sl, k_shared
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -1301,13 +1302,13 @@ class AttnVarFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dlse):
-        q, k, v, slopes, prefix, q_doc, k_doc, rng, q_lens, q_off, k_lens, k_off, out, lse = ctx.saved_tensors
+        q, k, v, slopes, prefix, q_doc, k_doc, rng, q_lens, q_off, k_lens, k_off, out, lse, lo = ctx.saved_tensors
         if dout is None:
             return (None,) * 14
         if ctx.k_shared:
             raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
         dout = _aligned_rows(dout)
-        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, (q_lens, q_off, k_lens, k_off), out, lse, ctx.cfg)
+        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, (q_lens, q_off, k_lens, k_off), out, lse, lo, ctx.cfg)
         nq, nk = (torch.zeros if f else torch.empty for f in ctx.fill)
         dq = nq(q.shape, dtype=q.dtype, device=q.device)
         dk, dv = nk(k.shape, dtype=k.dtype, device=k.device), nk(v.shape, dtype=v.dtype, device=v.device)

@@ -844,6 +844,9 @@ typedef struct {
   const int32_t* q_doc; const int32_t* k_doc;   /* one id for each row of Q / K, or both NULL          */
   void* out; int64_t o_rs;
   float* lse;                              /* [rows_q, Hq] or NULL (forward); required in the backward */
+  void* out_lo;                            /* [rows_q, Hq * dh] contiguous or NULL (bf16): what the rounding of out took away.  A caller that will
+                                            * run the backward gives it to both: rowsum(dout out) meets dP in a difference, and with the rounded
+                                            * output alone dQ and dK are half again as far off where few keys share a row's weight  */
   const void* dout; int64_t do_rs;         /* backward from here on (out, lse: the forward's) */
   void* dQ; int64_t dq_rs;
   void* dK; int64_t dk_rs;

@@ -113,7 +113,7 @@ def test_rows_of_no_example_stay(cuda):
     cfg = (2, 1, 0.2, 0.0, True, 65, 65)
     out, lse = torch.full_like(q, 7.0), torch.full((q.shape[0], 2), 7.0, device=cuda)
     lens = (seqs.q_lens, seqs.q_off, seqs.k_lens, seqs.k_off)
-    d = ops._attn_var_desc(q, k, v, None, None, None, None, None, lens, out, lse, cfg)
+    d = ops._attn_var_desc(q, k, v, None, None, None, None, None, lens, out, lse, None, cfg)
     L.check(L.load().dmt_attn_var_fwd(d, ops.stream_ptr()))
     dq, dk, dv = torch.full_like(q, 7.0), torch.full_like(k, 7.0), torch.full_like(v, 7.0)
     d.dout, d.do_rs, d.dQ, d.dq_rs, d.dK, d.dk_rs, d.dV, d.dv_rs = (do.data_ptr(), 64, dq.data_ptr(), 64, dk.data_ptr(), 32, dv.data_ptr(), 32)
