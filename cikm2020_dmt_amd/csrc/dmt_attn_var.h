@@ -591,4 +591,19 @@ __device__ __forceinline__ void place(int id, int heads, int nt, bool last_first
 
 }  // namespace attn_var
 
+// the kernels' variants: scores as they are (0), with slopes alone (1), capped and perhaps with slopes (2); documents or none
+template <int V> struct Const { static constexpr int value = V; };
+template <typename F> void with_shape(const attn_var::Args& a, F f) {
+  const int shape = a.cap > 0.f ? 2 : (a.slopes ? 1 : 0);
+  if (a.q_doc) {
+    if (shape == 0) f(Const<0>(), Const<1>());
+    else if (shape == 1) f(Const<1>(), Const<1>());
+    else f(Const<2>(), Const<1>());
+  } else {
+    if (shape == 0) f(Const<0>(), Const<0>());
+    else if (shape == 1) f(Const<1>(), Const<0>());
+    else f(Const<2>(), Const<0>());
+  }
+}
+
 int dmt_attn_var_args(const dmt_attn_var_desc* d, attn_var::Args* a, bool backward, const char* what);

@@ -8,7 +8,7 @@ namespace {
 // One workgroup of 4 wavefronts owns 128 queries of a head (a wavefront 32) and walks over the keys in tiles of 64, one tile in LDS, the next
 // one on its way through registers.  One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
 // are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
-template <typename T, int DHP, bool SHAPED, bool DOCS>
+template <typename T, int DHP, int SHAPE, bool DOCS>
 __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;               // tiles in LDS
@@ -27,8 +27,6 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
   const Shape sh = shape_of(a, h);
-  typename TL::Frag q[TL::NS];
-  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
   // what the workgroup, the wavefront and the lane's row may see
   const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
@@ -64,15 +62,15 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
     if (DOCS && tid < KT) docs[buf][tid] = kd;
   };
+  int flags = 0, buf = 0, t = wk.next(0, flags);
+  if (t < nk) begin(t, 0);                                 // (its latency and that of the row's own loads pass together)
+  typename TL::Frag q[TL::NS];
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
   float m = -INFINITY, l = 0.f;
-  int flags = 0, buf = 0, t = wk.next(0, flags);
-  if (t < nk) {
-    begin(t, 0);
-    end(0);
-  }
+  if (t < nk) end(0);
   __syncthreads();
   while (t < nk) {
     int nflags = 0;
@@ -89,8 +87,8 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) s[u] = TL::mma(TL::natural(Kl, u, l31, x, half), q[x], s[u]);
       }
-      if (SHAPED) {
-        if (sh.cap) {
+      if (SHAPE) {
+        if (SHAPE == 2) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -101,7 +99,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[u][r] *= sh.c1;
         }
-        if (sh.slope) {
+        if (SHAPE == 1 || sh.slope) {
           const float d0 = (float)(i + e.off - k0 - 4 * half);
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
 #pragma unroll
       for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
       mx = fmaxf(mx, other_half(mx));
-      const float c = SHAPED ? 1.f : sh.c1;
+      const float c = SHAPE ? 1.f : sh.c1;
       const float mt = mx * c;
       if (__any(mt > m + 8.f)) {
         const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.f : exp2_hw(m - mn);
@@ -162,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[u][r] = exp2_hw(SHAPED ? s[u][r] - mu : __builtin_fmaf(s[u][r], c, -mu));
+          s[u][r] = exp2_hw(SHAPE ? s[u][r] - mu : __builtin_fmaf(s[u][r], c, -mu));
           l += s[u][r];
         }
         TL::accumulate(o, Vl, 32 * u, s[u], lane);
@@ -227,11 +225,7 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const Args a) {
 template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
   const int nt = (int)cdiv64(a.max_q, 128);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  const bool shaped = a.cap > 0.f || a.slopes;
-  if (shaped && a.q_doc) tile_fwd_kernel<T, DHP, true, true><<<grid, 256, 0, st>>>(a, nt);
-  else if (shaped) tile_fwd_kernel<T, DHP, true, false><<<grid, 256, 0, st>>>(a, nt);
-  else if (a.q_doc) tile_fwd_kernel<T, DHP, false, true><<<grid, 256, 0, st>>>(a, nt);
-  else tile_fwd_kernel<T, DHP, false, false><<<grid, 256, 0, st>>>(a, nt);
+  with_shape(a, [&](auto shape, auto docs) { tile_fwd_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value><<<grid, 256, 0, st>>>(a, nt); });
 }
 template <typename T> int launch_fwd(const Args& a, hipStream_t st) {
   if (a.dh <= 32) launch_tile<T, 32>(a, st);

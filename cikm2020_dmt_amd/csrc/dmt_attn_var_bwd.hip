@@ -6,28 +6,26 @@ using namespace attn_var;
 
 namespace {
 
-// The scores of one 32 x 32 tile, in place: z2 (the row's statistic is subtracted by the caller).  d0: distance of register row 0 and the lane's
-// column; STEP: what a register row adds to it.
-template <int STEP>
-__device__ __forceinline__ void shaped(f32x16_t& s, f32x16_t& r2, const Shape& sh, float d0) {
-  if (sh.cap) {
+// The scores of one 32 x 32 tile, in place: z2 minus the row statistic (kept in rows or, stat[], in registers).  d0: distance of register row 0
+// and the lane's column; STEP: what a register row adds to it.  r2: what the cap's derivative needs.
+template <int SHAPE, int STEP, typename STAT>
+__device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& r2, const Shape& sh, float d0, STAT stat) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
+  for (int r = 0; r < 16; ++r) {
+    float z;
+    if (SHAPE == 2) {
       r2[r] = cap_r(sh, s[r]);
-      s[r] = __builtin_fmaf(-2.f * sh.cap2, r2[r], sh.cap2);
+      z = __builtin_fmaf(-2.f * sh.cap2, r2[r], sh.cap2 - stat(r));
+    } else {
+      z = __builtin_fmaf(s[r], sh.c1, -stat(r));
     }
-  } else {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= sh.c1;
-  }
-  if (sh.slope) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), s[r]);
+    if (SHAPE == 1 || (SHAPE == 2 && sh.slope)) z = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), z);
+    s[r] = exp2_hw(z);
   }
 }
 
 // dQ (and D): one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
-template <typename T, int DHP, bool SHAPED, bool DOCS>
+template <typename T, int DHP, int SHAPE, bool DOCS>
 __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
@@ -50,27 +48,6 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
   const Shape sh = shape_of(a, h);
-  typename TL::Frag q[TL::NS], g[TL::NS];
-  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
-  own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, i, half);
-  const long long stat = (e.q0 + (in ? i : 0)) * a.Hq + h;
-  // (a row that sees nothing: lse = -inf; its weights 2^(z - inf) are 0)
-  const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY;
-  float D = 0.f;                                         // rowsum(dout * out), for this kernel and the next
-  {
-    typename TL::Frag ov[TL::NS];
-    own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, i, half);
-#pragma unroll
-    for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
-    if (sizeof(T) == 2 && a.out_lo) {
-      const long long ls = (long long)a.Hq * a.dh;
-      own_row<T, DHP>(ov, (const T*)a.out_lo + e.q0 * ls + (long long)h * a.dh, ls, e.ql, a.dh, i, half);
-#pragma unroll
-      for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
-    }
-    D += other_half(D);
-    if (in && half == 0) a.D[stat] = D;
-  }
   const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
@@ -105,15 +82,34 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     st.end(lds + buf * (KE + VE), lds + buf * (KE + VE) + KE);
     if (DOCS && tid < KT) docs[buf][tid] = kd;
   };
+  int flags = 0, buf = 0, t = wk.next(0, flags);
+  if (t < nk) begin(t, 0);                               // (its latency and that of the rows' own loads pass together)
+  typename TL::Frag q[TL::NS], g[TL::NS];
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
+  own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, i, half);
+  const long long stat = (e.q0 + (in ? i : 0)) * a.Hq + h;
+  // (a row that sees nothing: lse = -inf; its weights 2^(z - inf) are 0)
+  const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY;
+  float D = 0.f;                                         // rowsum(dout * out), for this kernel and the next
+  {
+    typename TL::Frag ov[TL::NS];
+    own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, i, half);
+#pragma unroll
+    for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
+    if (sizeof(T) == 2 && a.out_lo) {
+      const long long ls = (long long)a.Hq * a.dh;
+      own_row<T, DHP>(ov, (const T*)a.out_lo + e.q0 * ls + (long long)h * a.dh, ls, e.ql, a.dh, i, half);
+#pragma unroll
+      for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
+    }
+    D += other_half(D);
+    if (in && half == 0) a.D[stat] = D;
+  }
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
-  int flags = 0, buf = 0, t = wk.next(0, flags);
-  if (t < nk) {
-    begin(t, 0);
-    end(0);
-  }
+  if (t < nk) end(0);
   __syncthreads();
   while (t < nk) {
     int nflags = 0;
@@ -133,9 +129,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
           dp = TL::mma(TL::natural(Vl, u, l31, x, half), g[x], dp);
         }
         const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
-        if (SHAPED) shaped<-1>(s, r2, sh, d0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = exp2_hw(SHAPED ? s[r] - lse2 : __builtin_fmaf(s[r], sh.c1, -lse2));
+        weights<SHAPE, -1>(s, r2, sh, d0, [&](int) { return lse2; });
         if (docs_differ || cut) {
           // (a masked place gives weight and gradient 0 whatever stands there)
           const int pre = e.pre - k0 - 32 * u - 4 * half, lm = (docs_differ ? lim0 : lim) - k0 - 32 * u - 4 * half;
@@ -153,7 +147,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
             }
           }
         }
-        if (SHAPED && a.slope_part) {
+        if (SHAPE && a.slope_part) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const float ad = fabsf(d0 - (float)reg_row(r, 0)), pd = s[r] * dp[r];
@@ -166,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] *= dp[r] - D;
-          if (SHAPED && sh.cap) s[r] *= 4.f * r2[r] * (1.f - r2[r]);
+          if (SHAPE == 2) s[r] *= 4.f * r2[r] * (1.f - r2[r]);
         }
         TL::accumulate(o, Kl, 32 * u, s, lane);
       }
@@ -180,7 +174,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   }
   float sl = 0.f;
   if (active) {
-    if (SHAPED && a.slope_part) {
+    if (SHAPE && a.slope_part) {
       s0 += other_half(s0);
       s1 += other_half(s1);
       s2 += other_half(s2);
@@ -228,7 +222,7 @@ __device__ void sum_slopes(const float* part, long long n, float* out, double* r
 // WHAT: 1 = dK, 2 = dV, 3 = both.  Both accumulators and both operands' rows fit the 256 registers of two wavefronts a SIMD up to 80 dims (64 in
 // fp32); wider heads take a kernel each -- one more product of scores, but at 4096 causal keys, 16 heads of 128 dims 225 + 164 us against 443 us
 // for one kernel with one wavefront a SIMD (accumulators moved between register files) and 1033 us with spills.
-template <typename T, int DHP, bool SHAPED, bool DOCS, int WHAT>
+template <typename T, int DHP, int SHAPE, bool DOCS, int WHAT>
 __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, int nqt) {
   typedef Tile<T, DHP> TL;
   constexpr int NB = sizeof(T) == 2 ? 2 : 1;
@@ -238,8 +232,8 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   __shared__ __attribute__((aligned(16))) float stats[NB][2][KT];
   static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
-  const int id = (int)blockIdx.x - (SHAPED && (WHAT & 1) && a.slope_part ? a.Hq : 0);
-  if (SHAPED && (WHAT & 1) && id < 0) {                                 // the first workgroups finish the slopes' gradient that the dQ kernel left in parts
+  const int id = (int)blockIdx.x - (SHAPE && (WHAT & 1) && a.slope_part ? a.Hq : 0);
+  if (SHAPE && (WHAT & 1) && id < 0) {                                 // the first workgroups finish the slopes' gradient that the dQ kernel left in parts
     const long long n = (long long)a.B * nqt;
     sum_slopes(a.slope_part + (long long)blockIdx.x * n, n, a.dslopes + blockIdx.x, (double*)lds);
     return;
@@ -252,9 +246,6 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   if (kt * 128 >= e.kl) return;
   const int jw = kt * 128 + wave * 32, j = jw + l31;
   const bool active = jw < e.kl;
-  typename TL::Frag k[TL::NS], v[TL::NS];
-  own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, j, half);
-  if (WHAT & 1) own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
   // queries that may see some key of the workgroup / wavefront / lane: from `lo` on (rows before it sit above the diagonal, unless the key
   // belongs to the prefix)
   const int lo_wg = a.causal && kt * 128 >= e.pre ? max(0, kt * 128 - e.off) : 0;
@@ -314,10 +305,11 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   int flags = 0, buf = 0, g = 0, t = wk.next(t0, flags);
   if (t >= t1) g = ng;
   const int first = t, first_flags = flags;
-  if (g < ng) {
-    begin(0, t, 0);
-    end(0);
-  }
+  if (g < ng) begin(0, t, 0);
+  typename TL::Frag k[TL::NS], v[TL::NS];
+  own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, j, half);
+  if (WHAT & 1) own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
+  if (g < ng) end(0);
   __syncthreads();
   while (g < ng) {
     int nflags = 0, gn = g, tn = wk.next(t + 1, nflags);
@@ -342,14 +334,10 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
           s = TL::mma(TL::natural(Ql, u, l31, x, half), k[x], s);
           if (WHAT & 1) dp = TL::mma(TL::natural(Gl, u, l31, x, half), v[x], dp);
         }
-        if (SHAPED) shaped<1>(s, r2, sh, (float)(i0 + 32 * u + 4 * half + e.off - j));
+        f32x4_t ls[4];
 #pragma unroll
-        for (int gg = 0; gg < 4; ++gg) {
-          const float4 ls = *reinterpret_cast<const float4*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
-          const float lv[4] = {ls.x, ls.y, ls.z, ls.w};
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[4 * gg + c] = exp2_hw(SHAPED ? s[4 * gg + c] - lv[c] : __builtin_fmaf(s[4 * gg + c], sh.c1, -lv[c]));
-        }
+        for (int gg = 0; gg < 4; ++gg) ls[gg] = *reinterpret_cast<const f32x4_t*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
+        weights<SHAPE, 1>(s, r2, sh, (float)(i0 + 32 * u + 4 * half + e.off - j), [&](int r) { return ls[r >> 2][r & 3]; });
         if (docs_differ || cut) {
           const int lo = lo_l - i0 - 32 * u - 4 * half;
 #pragma unroll
@@ -374,7 +362,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             s[4 * gg + c] *= dp[4 * gg + c] - D[c];
-            if (SHAPED && sh.cap) s[4 * gg + c] *= 4.f * r2[4 * gg + c] * (1.f - r2[4 * gg + c]);
+            if (SHAPE == 2) s[4 * gg + c] *= 4.f * r2[4 * gg + c] * (1.f - r2[4 * gg + c]);
           }
         }
         TL::accumulate(dk, Ql, 32 * u, s, lane);
@@ -443,27 +431,20 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
 
 template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  const bool shaped = a.cap > 0.f || a.slopes;
-  if (shaped && a.q_doc) tile_dq_kernel<T, DHP, true, true><<<grid, 256, 0, st>>>(a, nt);
-  else if (shaped) tile_dq_kernel<T, DHP, true, false><<<grid, 256, 0, st>>>(a, nt);
-  else if (a.q_doc) tile_dq_kernel<T, DHP, false, true><<<grid, 256, 0, st>>>(a, nt);
-  else tile_dq_kernel<T, DHP, false, false><<<grid, 256, 0, st>>>(a, nt);
-}
-template <typename T, int DHP, bool SHAPED, bool DOCS> void launch_dkv_as(const Args& a, int nt, int nqt, hipStream_t st) {
-  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
-  if constexpr (DHP > (sizeof(T) == 2 ? 80 : 64)) {
-    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 2><<<grid, 256, 0, st>>>(a, nt, nqt);
-    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 1><<<grid + more, 256, 0, st>>>(a, nt, nqt);
-  } else {
-    tile_dkv_kernel<T, DHP, SHAPED, DOCS, 3><<<grid + more, 256, 0, st>>>(a, nt, nqt);
-  }
+  with_shape(a, [&](auto shape, auto docs) { tile_dq_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value><<<grid, 256, 0, st>>>(a, nt); });
 }
 template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
-  const bool shaped = a.cap > 0.f || a.slopes;
-  if (shaped && a.q_doc) launch_dkv_as<T, DHP, true, true>(a, nt, nqt, st);
-  else if (shaped) launch_dkv_as<T, DHP, true, false>(a, nt, nqt, st);
-  else if (a.q_doc) launch_dkv_as<T, DHP, false, true>(a, nt, nqt, st);
-  else launch_dkv_as<T, DHP, false, false>(a, nt, nqt, st);
+  const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
+  with_shape(a, [&](auto shape, auto docs) {
+    constexpr int S = decltype(shape)::value;
+    constexpr bool D = decltype(docs)::value;
+    if constexpr (DHP > (sizeof(T) == 2 ? 80 : 64)) {
+      tile_dkv_kernel<T, DHP, S, D, 2><<<grid, 256, 0, st>>>(a, nt, nqt);
+      tile_dkv_kernel<T, DHP, S, D, 1><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+    } else {
+      tile_dkv_kernel<T, DHP, S, D, 3><<<grid + more, 256, 0, st>>>(a, nt, nqt);
+    }
+  });
 }
 
 template <typename T>
