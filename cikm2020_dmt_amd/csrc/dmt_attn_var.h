@@ -34,7 +34,7 @@ struct Args {
   void* dV; long long dv_rs;
   float* dslopes;
   float* D;                         // [rows_q, Hq]: rowsum(dout * out)
-  float* slope_part;                // [Hq][B * ceil(max_q / 128)]
+  float* slope_part;                // [Hq][B * tiles of the dQ kernel]
   int parts, qparts;                // dK, dV: heads of a group x query ranges in `parts` pieces (qparts ranges), summed by a launch of their own
   float* part_k; float* part_v;     // [parts][rows_k][Hkv * dh] when parts > 1
   int2* q_rng; int2* k_rng;         // (least, largest) document id of every 64-row tile: [B][ceil(max / 64)]
@@ -336,6 +336,12 @@ __device__ __forceinline__ float other_half(float x) {
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
+// The wait that the result of a product needs before plain instructions read it (11 cycles after a 32x32x16, 18 after a 32x32x2), stated here: the
+// compiler counts it, but where a branch forks behind the product and joins before the read it has counted the longer way only, and the last
+// register of a tile was read before it was written.  To be used behind every product whose result meets a branch.
+__device__ __forceinline__ void settle(f32x16_t& a) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a)); }
+__device__ __forceinline__ void settle(f32x16_t& a, f32x16_t& b) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b)); }
+
 template <typename T, int DHP> struct Tile;
 template <int DHP> struct Tile<bf16_t, DHP> {
   typedef bf16x8_t Frag;
@@ -437,7 +443,7 @@ __device__ __forceinline__ void own_row(typename Tile<T, DHP>::Frag* f, const T*
 // The 64-row tiles of two operands on their way into LDS.  bf16: straight from memory (buffer_load ... lds: 64 lanes fill 1 KB of consecutive
 // 16-byte chunks, each lane choosing what the row permutation wants there); issued a tile ahead, it costs no registers and no LDS-write
 // instructions.  begin() and end() bracket the use of the tile before; the buffer that begin() names must be free.
-template <typename T, int DHP> struct Stage;
+template <typename T, int DHP, int NW> struct Stage;        // NW wavefronts
 __device__ __forceinline__ u32x4_t rsrc_words(const void* base, unsigned bytes) {
   const unsigned long long p = (unsigned long long)(uintptr_t)base;
   u32x4_t r;
@@ -450,17 +456,17 @@ __device__ __forceinline__ u32x4_t rsrc_words(const void* base, unsigned bytes) 
 __device__ __forceinline__ void load16_lds(const u32x4_t& rsrc, int off, unsigned lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 }
-template <int DHP> struct Stage<bf16_t, DHP> {
+template <int DHP, int NW> struct Stage<bf16_t, DHP, NW> {
   typedef Tile<bf16_t, DHP> TL;
-  static constexpr int IT = KT * TL::SC / 256;
-  static_assert(KT * TL::SC % 256 == 0, "whole 1 KB pieces");
+  static constexpr int NT = 64 * NW, IT = KT * TL::SC / NT;
+  static_assert(KT * TL::SC % NT == 0, "whole 1 KB pieces");
   int off_a[IT], off_b[IT];              // byte offsets within a tile
   unsigned at;                           // LDS byte offset of the wavefront's first piece within a tile
   __device__ __forceinline__ void init(long long rs_a, long long rs_b, int dh, int tid) {
     at = (unsigned)__builtin_amdgcn_readfirstlane(tid >> 6) * 1024u;
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int c = tid + i * 256, row = c / TL::SC, ch = (c - row * TL::SC) ^ TL::swz(row);
+      const int c = tid + i * NT, row = c / TL::SC, ch = (c - row * TL::SC) ^ TL::swz(row);
       const bool in = ch * 8 < dh;
       off_a[i] = in ? row * (int)(rs_a * 2) + ch * 16 : OUTSIDE;
       off_b[i] = in ? row * (int)(rs_b * 2) + ch * 16 : OUTSIDE;
@@ -471,22 +477,22 @@ template <int DHP> struct Stage<bf16_t, DHP> {
     const unsigned db = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lb + at;
     const u32x4_t ra = rsrc_words(pa, (unsigned)((rows - 1) * (int)(rs_a * 2) + dh * 2)), rb = rsrc_words(pb, (unsigned)((rows - 1) * (int)(rs_b * 2) + dh * 2));
 #pragma unroll
-    for (int i = 0; i < IT; ++i) load16_lds(ra, off_a[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(da + 4096u * i)));
+    for (int i = 0; i < IT; ++i) load16_lds(ra, off_a[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(da + 1024u * NW * i)));
 #pragma unroll
-    for (int i = 0; i < IT; ++i) load16_lds(rb, off_b[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(db + 4096u * i)));
+    for (int i = 0; i < IT; ++i) load16_lds(rb, off_b[i], (unsigned)__builtin_amdgcn_readfirstlane((int)(db + 1024u * NW * i)));
   }
   __device__ __forceinline__ void end(bf16_t*, bf16_t*) const { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 };
 // fp32: through registers, one tile in LDS
-template <int DHP> struct Stage<float, DHP> {
+template <int DHP, int NW> struct Stage<float, DHP, NW> {
   typedef Tile<float, DHP> TL;
-  static constexpr int IT = (KT * TL::CH + 255) / 256;
+  static constexpr int NT = 64 * NW, IT = (KT * TL::CH + NT - 1) / NT;
   u32x4_t a[IT], b[IT];
   int off_a[IT], off_b[IT], dst[IT];     // byte offsets within a tile; element in LDS
   __device__ __forceinline__ void init(long long rs_a, long long rs_b, int dh, int tid) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      const int c = tid + i * 256, row = c / TL::CH, ch = c - row * TL::CH;
+      const int c = tid + i * NT, row = c / TL::CH, ch = c - row * TL::CH;
       const bool in = row < KT && ch * 4 < dh;
       off_a[i] = in ? row * (int)(rs_a * 4) + ch * 16 : OUTSIDE;
       off_b[i] = in ? row * (int)(rs_b * 4) + ch * 16 : OUTSIDE;
@@ -503,7 +509,7 @@ template <int DHP> struct Stage<float, DHP> {
   __device__ __forceinline__ void end(float* la, float* lb) const {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if ((KT * TL::CH) % 256 != 0 && dst[i] < 0) continue;
+      if ((KT * TL::CH) % NT != 0 && dst[i] < 0) continue;
       *reinterpret_cast<u32x4_t*>(la + dst[i]) = a[i];
       *reinterpret_cast<u32x4_t*>(lb + dst[i]) = b[i];
     }
@@ -574,7 +580,7 @@ __device__ __forceinline__ float not_finite(const f32x16_t& o, int dt, int half,
   return t;
 }
 
-// which 128 rows of which head a workgroup takes: workgroups go round the 8 dies, each with an L2 of its own, so a die gets whole heads (the
+// which rows of which head a workgroup takes: workgroups go round the 8 dies, each with an L2 of its own, so a die gets whole heads (the
 // heads that share keys side by side); the tiles with the longest rows of a causal mask start first.
 __device__ __forceinline__ void place(int id, int heads, int nt, bool last_first, int& head, int& tile) {
   int t;
@@ -590,6 +596,14 @@ __device__ __forceinline__ void place(int id, int heads, int nt, bool last_first
 }
 
 }  // namespace attn_var
+
+// Query rows of a workgroup of the forward and dQ kernels: 128 (the four wavefronts share each tile of keys), but 64 where that leaves two
+// workgroups a compute unit or fewer, so that uneven rows even out (4 histories of 2048 in sessions, 8 heads of 64: forward 33 against 37 us, dQ 43
+// against 48; 256 histories of up to 200, 4 heads of 80, would lose: 47 against 38 and 52 against 48).  Heads wider than 80 keep 128: their tiles
+// of keys fill the LDS of half a compute unit either way.
+inline int rows_of(const attn_var::Args& a, int dhp) {
+  return dhp <= 80 && (long long)a.B * a.Hq * cdiv64(a.max_q, 128) <= 512 ? 64 : 128;
+}
 
 // the kernels' variants: scores as they are (0), with slopes alone (1), capped and perhaps with slopes (2); documents or none
 template <int V> struct Const { static constexpr int value = V; };

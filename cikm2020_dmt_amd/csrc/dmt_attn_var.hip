@@ -8,27 +8,27 @@ namespace {
 // One workgroup of 4 wavefronts owns 128 queries of a head (a wavefront 32) and walks over the keys in tiles of 64, one tile in LDS, the next
 // one on its way through registers.  One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
 // are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
-template <typename T, int DHP, int SHAPE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) {
+template <typename T, int DHP, int SHAPE, bool DOCS, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
-  constexpr int NB = sizeof(T) == 2 ? 2 : 1;               // tiles in LDS
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1, ROWS = 32 * NW;               // tiles in LDS
   constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS, VE = KT * TL::RS + PAD;      // (fp32: dims past the last row's end are read, not used)
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
   __shared__ __attribute__((aligned(16))) int docs[DOCS ? NB : 1][KT];
-  static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
+  static_assert(sizeof(lds) >= NW * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
   int head, qt;
   place(blockIdx.x, a.B * a.Hq, nt, a.causal, head, qt);
   const int b = head / a.Hq, h = head - b * a.Hq, hk = h / a.G;
   const Ex e = example(a, b);
-  if (qt * 128 >= e.ql) return;
-  const int iw = qt * 128 + wave * 32, i = iw + l31;
+  if (qt * ROWS >= e.ql) return;
+  const int iw = qt * ROWS + wave * 32, i = iw + l31;
   const bool active = iw < e.ql;
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
   const Shape sh = shape_of(a, h);
   // what the workgroup, the wavefront and the lane's row may see
-  const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
+  const int last = (qt * ROWS + ROWS < e.ql ? qt * ROWS + ROWS : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
   const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
@@ -39,7 +39,8 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
   if constexpr (DOCS) {
     wk.lo = 0;
     const int2* qr = a.q_rng + (long long)b * a.nqt;
-    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0, rw = wave < 2 ? r0 : r1;
+    const int t0 = qt * ROWS / 64, t1 = NW > 2 && t0 + 1 < a.nqt ? t0 + 1 : t0;
+    const int2 r0 = qr[t0], r1 = qr[t1], rw = wave < 2 ? r0 : r1;
     wk.rng = a.k_rng + (long long)b * a.nkt;
     wk.free_wg = wk.free_w = (e.pre + KT - 1) / KT;
     wk.glo = min(r0.x, r1.x);
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     wk.chunk = -1;
     qd = i < e.ql ? a.q_doc[e.q0 + i] : 0;
   }
-  Stage<T, DHP> st;
+  Stage<T, DHP, NW> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
   const auto begin = [&](int t, int buf) {
@@ -87,6 +88,7 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) s[u] = TL::mma(TL::natural(Kl, u, l31, x, half), q[x], s[u]);
       }
+      settle(s[0], s[1]);
       if (SHAPE) {
         if (SHAPE == 2) {
 #pragma unroll
@@ -174,6 +176,8 @@ __global__ __launch_bounds__(256, 2) void tile_fwd_kernel(const Args a, int nt) 
     flags = nflags;
   }
   if (!active) return;
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) settle(o[dt]);
   l += other_half(l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float bad = l * 0.f;
@@ -222,10 +226,16 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const Args a) {
   if (lane == 0) (keys ? a.k_rng : a.q_rng)[(long long)b * nt + t] = make_int2(lo, hi);
 }
 
-template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
-  const int nt = (int)cdiv64(a.max_q, 128);
+template <typename T, int DHP, int NW> void launch_tile_as(const Args& a, hipStream_t st) {
+  const int nt = (int)cdiv64(a.max_q, 32 * NW);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  with_shape(a, [&](auto shape, auto docs) { tile_fwd_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value><<<grid, 256, 0, st>>>(a, nt); });
+  with_shape(a, [&](auto shape, auto docs) { tile_fwd_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
+}
+template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
+  if constexpr (DHP <= 80) {
+    if (rows_of(a, DHP) == 64) return launch_tile_as<T, DHP, 2>(a, st);
+  }
+  launch_tile_as<T, DHP, 4>(a, st);
 }
 template <typename T> int launch_fwd(const Args& a, hipStream_t st) {
   if (a.dh <= 32) launch_tile<T, 32>(a, st);
@@ -266,7 +276,7 @@ WsLayout ws_layout(const dmt_attn_var_desc* d) {
   w.D = at;
   at += up16(4 * (uint64_t)d->rows_q * (uint64_t)d->Hq);
   w.sp = at;
-  if (d->dslopes) at += up16(4 * (uint64_t)d->Hq * (uint64_t)d->B * (uint64_t)cdiv64(d->max_q, 128));
+  if (d->dslopes) at += up16(4 * (uint64_t)d->Hq * (uint64_t)d->B * (uint64_t)cdiv64(d->max_q, 64));
   int qparts;
   const int parts = parts_of(d, &qparts);
   const uint64_t part = parts > 1 ? up16(4 * (uint64_t)parts * (uint64_t)d->rows_k * (uint64_t)d->Hkv * (uint64_t)d->dh) : 0;
@@ -294,7 +304,7 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   DMT_CHECK_ARG(dmt_attn_var_supported(d->dtype, d->dh, d->Hq, d->Hkv),
                 "%s: needs bf16 (dh %% 8 == 0) or fp32 (dh %% 4 == 0), dh <= 128 and Hq a multiple of Hkv: got dtype %d, dh %d, Hq %d, Hkv %d", what,
                 d->dtype, d->dh, d->Hq, d->Hkv);
-  DMT_CHECK_ARG((int64_t)d->B * d->Hq * (cdiv64(d->max_q > d->max_k ? d->max_q : d->max_k, 128) + 1) < (1ll << 31), "%s: B * Hq * max length / 128 passes 2^31", what);
+  DMT_CHECK_ARG((int64_t)d->B * d->Hq * (cdiv64(d->max_q > d->max_k ? d->max_q : d->max_k, 64) + 1) < (1ll << 31), "%s: B * Hq * max length / 64 passes 2^31", what);
   DMT_CHECK_ARG(d->B <= 65535 && d->Hq <= 65535, "%s: B and Hq <= 65535", what);
   DMT_CHECK_ARG(d->rows_q < (1ll << 31) && d->rows_k < (1ll << 31), "%s: row numbers are int32", what);
   DMT_CHECK_ARG(d->scale > 0.f && d->scale < 3.4e38f, "%s: scale must be positive and finite", what);

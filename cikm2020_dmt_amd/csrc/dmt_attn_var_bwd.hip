@@ -25,30 +25,30 @@ __device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& r2, const Shape& 
 }
 
 // dQ (and D): one workgroup owns 128 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of dQ^T += K^T dX.
-template <typename T, int DHP, int SHAPE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
+template <typename T, int DHP, int SHAPE, bool DOCS, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
-  constexpr int NB = sizeof(T) == 2 ? 2 : 1;
+  constexpr int NB = sizeof(T) == 2 ? 2 : 1, ROWS = 32 * NW;
   constexpr int PAD = sizeof(T) == 2 ? 0 : 32, KE = KT * TL::RS + PAD, VE = KT * TL::RS;
   __shared__ __attribute__((aligned(16))) T lds[NB * (KE + VE)];
   __shared__ __attribute__((aligned(16))) int docs[DOCS ? NB : 1][KT];
-  __shared__ float part[4];
-  static_assert(sizeof(lds) >= 4 * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
+  __shared__ float part[NW];
+  static_assert(sizeof(lds) >= NW * ROW_LDS * sizeof(float), "the row form works in the tiles' memory");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, l31 = lane & 31;
   int head, qt;
   place(blockIdx.x, a.B * a.Hq, nt, a.causal, head, qt);
   const int b = head / a.Hq, h = head - b * a.Hq, hk = h / a.G;
   const Ex e = example(a, b);
-  if (qt * 128 >= e.ql) {
+  if (qt * ROWS >= e.ql) {
     if (a.slope_part && tid == 0) a.slope_part[((long long)h * a.B + b) * nt + qt] = 0.f;
     return;
   }
-  const int iw = qt * 128 + wave * 32, i = iw + l31;
+  const int iw = qt * ROWS + wave * 32, i = iw + l31;
   const bool active = iw < e.ql, in = i < e.ql;
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
   const Shape sh = shape_of(a, h);
-  const int last = (qt * 128 + 128 < e.ql ? qt * 128 + 128 : e.ql) - 1;
+  const int last = (qt * ROWS + ROWS < e.ql ? qt * ROWS + ROWS : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
   const int lim0 = a.causal ? min(e.kl, i + e.off + 1) : e.kl, lim = max(lim0, e.pre);
@@ -59,7 +59,8 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   if constexpr (DOCS) {
     wk.lo = 0;
     const int2* qr = a.q_rng + (long long)b * a.nqt;
-    const int2 r0 = qr[qt * 2], r1 = qt * 2 + 1 < a.nqt ? qr[qt * 2 + 1] : r0, rw = wave < 2 ? r0 : r1;
+    const int t0 = qt * ROWS / 64, t1 = NW > 2 && t0 + 1 < a.nqt ? t0 + 1 : t0;
+    const int2 r0 = qr[t0], r1 = qr[t1], rw = wave < 2 ? r0 : r1;
     wk.rng = a.k_rng + (long long)b * a.nkt;
     wk.free_wg = wk.free_w = (e.pre + KT - 1) / KT;
     wk.glo = min(r0.x, r1.x);
@@ -69,7 +70,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
     wk.chunk = -1;
     qd = in ? a.q_doc[e.q0 + i] : 0;
   }
-  Stage<T, DHP> st;
+  Stage<T, DHP, NW> st;
   st.init(a.k_rs, a.v_rs, a.dh, tid);
   int kd = 0;
   const auto begin = [&](int t, int buf) {
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
           dp = TL::mma(TL::natural(Vl, u, l31, x, half), g[x], dp);
         }
         const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
+        settle(s, dp);
         weights<SHAPE, -1>(s, r2, sh, d0, [&](int) { return lse2; });
         if (docs_differ || cut) {
           // (a masked place gives weight and gradient 0 whatever stands there)
@@ -174,6 +176,8 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   }
   float sl = 0.f;
   if (active) {
+#pragma unroll
+    for (int dt = 0; dt < TL::NDT; ++dt) settle(o[dt]);
     if (SHAPE && a.slope_part) {
       s0 += other_half(s0);
       s1 += other_half(s1);
@@ -200,7 +204,7 @@ __global__ __launch_bounds__(256, 2) void tile_dq_kernel(const Args a, int nt) {
   if (a.slope_part) {
     if (lane == 0) part[wave] = sl;
     __syncthreads();
-    if (tid == 0) a.slope_part[((long long)h * a.B + b) * nt + qt] = (part[0] + part[1]) + (part[2] + part[3]);
+    if (tid == 0) a.slope_part[((long long)h * a.B + b) * nt + qt] = NW == 4 ? (part[0] + part[1]) + (part[2] + part[NW - 1]) : part[0] + part[1];
   }
 }
 
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
     wk.chunk = -1;
     kd_l = j < e.kl ? a.k_doc[e.k0 + j] : 0;
   }
-  Stage<T, DHP> st;
+  Stage<T, DHP, 4> st;
   st.init(a.q_rs, a.do_rs, a.dh, tid);
   int qd = 0;
   float lse2 = 0.f;
@@ -334,6 +338,8 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
           s = TL::mma(TL::natural(Ql, u, l31, x, half), k[x], s);
           if (WHAT & 1) dp = TL::mma(TL::natural(Gl, u, l31, x, half), v[x], dp);
         }
+        if (WHAT & 1) settle(s, dp);
+        else settle(s);
         f32x4_t ls[4];
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg) ls[gg] = *reinterpret_cast<const f32x4_t*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
@@ -378,6 +384,11 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   }
   if (!active) return;
   const bool in = j < e.kl;
+#pragma unroll
+  for (int dt = 0; dt < TL::NDT; ++dt) {
+    if (WHAT & 1) settle(dk[dt]);
+    if (WHAT & 2) settle(dv[dt]);
+  }
   float bad = 0.f;
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) {
@@ -429,9 +440,16 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
   }
 }
 
-template <typename T, int DHP> void launch_dq(const Args& a, int nt, hipStream_t st) {
+template <typename T, int DHP, int NW> void launch_dq_as(const Args& a, hipStream_t st) {
+  const int nt = (int)cdiv64(a.max_q, 32 * NW);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  with_shape(a, [&](auto shape, auto docs) { tile_dq_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value><<<grid, 256, 0, st>>>(a, nt); });
+  with_shape(a, [&](auto shape, auto docs) { tile_dq_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
+}
+template <typename T, int DHP> void launch_dq(const Args& a, hipStream_t st) {
+  if constexpr (DHP <= 80) {
+    if (rows_of(a, DHP) == 64) return launch_dq_as<T, DHP, 2>(a, st);
+  }
+  launch_dq_as<T, DHP, 4>(a, st);
 }
 template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
@@ -449,12 +467,13 @@ template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, h
 
 template <typename T>
 int launch_bwd(Args a, hipStream_t st) {
-  const int nqt = (int)cdiv64(a.max_q, 128), nkt = (int)cdiv64(a.max_k, 128);
+  const int dhp = a.dh <= 32 ? 32 : (a.dh <= 64 ? 64 : (a.dh <= 80 ? 80 : 128));
+  const int nqt = (int)cdiv64(a.max_q, rows_of(a, dhp)), nkt = (int)cdiv64(a.max_k, 128);
   if (a.rows_q && nqt) {
-    if (a.dh <= 32) launch_dq<T, 32>(a, nqt, st);
-    else if (a.dh <= 64) launch_dq<T, 64>(a, nqt, st);
-    else if (a.dh <= 80) launch_dq<T, 80>(a, nqt, st);
-    else launch_dq<T, 128>(a, nqt, st);
+    if (a.dh <= 32) launch_dq<T, 32>(a, st);
+    else if (a.dh <= 64) launch_dq<T, 64>(a, st);
+    else if (a.dh <= 80) launch_dq<T, 80>(a, st);
+    else launch_dq<T, 128>(a, st);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq)");
   } else {
     a.slope_part = nullptr;                               // (no query: nothing to add)

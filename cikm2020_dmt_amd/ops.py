@@ -1256,19 +1256,24 @@ def _aligned_rows(t):
     return t.contiguous()
 
 
-def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg):
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg, grads=None):
+    """grads: (dout, dq, dk, dv, dslopes) in the backward"""
     H, Hkv, scale, cap, causal, max_q, max_k = cfg
-    d = L.AttnVarDesc()
-    d.dtype, d.B, d.Hq, d.Hkv, d.dh, d.max_q, d.max_k = dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k
-    d.rows_q, d.rows_k = q.shape[0], k.shape[0]
-    d.Q, d.q_rs = q.data_ptr(), _rows2(q, "q", H, q.dtype)
-    d.K, d.k_rs = k.data_ptr(), _rows2(k, "k", Hkv, q.dtype)
-    d.V, d.v_rs = v.data_ptr(), _rows2(v, "v", Hkv, q.dtype)
-    d.q_lens, d.q_off, d.k_lens, d.k_off = (x.data_ptr() for x in lens)
-    d.scale, d.cap, d.causal = scale, cap, 1 if causal else 0
-    d.slopes, d.prefix, d.q_doc, d.k_doc = (x.data_ptr() if x is not None else None for x in (slopes, prefix, q_doc, k_doc))
-    d.out, d.o_rs, d.lse, d.out_lo, d.doc_ranges = out.data_ptr(), out.shape[1], p(lse), p(lo), p(rng)
-    return d
+    dout, dq, dk, dv, dsl = grads or (None,) * 5
+    g = (0,) * 8 if grads is None else (dout.data_ptr(), _row_stride(dout), dq.data_ptr(), dq.shape[1], dk.data_ptr(), dk.shape[1], dv.data_ptr(),
+                                        dv.shape[1])
+    return L.AttnVarDesc(dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k, q.shape[0], k.shape[0], q.data_ptr(), _row_stride(q),
+                         k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), lens[1].data_ptr(), lens[0].data_ptr(), lens[3].data_ptr(),
+                         lens[2].data_ptr(), scale, cap, 1 if causal else 0, _ptr(slopes), _ptr(prefix), _ptr(q_doc), _ptr(k_doc), out.data_ptr(),
+                         out.shape[1], _ptr(lse), _ptr(lo), g[0], g[1], g[2], g[3], g[4], g[5], g[6], g[7], _ptr(dsl), _ptr(rng), None, 0)
 
 
 def _var_doc_ranges(q_doc, B, max_q, max_k):
@@ -1308,15 +1313,12 @@ class AttnVarFn(torch.autograd.Function):
         if ctx.k_shared:
             raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
         dout = _aligned_rows(dout)
-        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, (q_lens, q_off, k_lens, k_off), out, lse, lo, ctx.cfg)
-        nq, nk = (torch.zeros if f else torch.empty for f in ctx.fill)
-        dq = nq(q.shape, dtype=q.dtype, device=q.device)
-        dk, dv = nk(k.shape, dtype=k.dtype, device=k.device), nk(v.shape, dtype=v.dtype, device=v.device)
+        nq, nk = (torch.zeros_like if f else torch.empty_like for f in ctx.fill)
+        fmt = dict(memory_format=torch.contiguous_format)
+        dq, dk, dv = nq(q, **fmt), nk(k, **fmt), nk(v, **fmt)
         dsl = torch.zeros_like(slopes) if ctx.need_sl else None
-        desc.dout, desc.do_rs = dout.data_ptr(), dout.stride(0) if dout.shape[0] > 1 else dout.shape[1]
-        desc.dQ, desc.dq_rs, desc.dK, desc.dk_rs, desc.dV, desc.dv_rs = (dq.data_ptr(), dq.shape[1], dk.data_ptr(), dk.shape[1], dv.data_ptr(),
-                                                                         dv.shape[1])
-        desc.dslopes = p(dsl)
+        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, (q_lens, q_off, k_lens, k_off), out, lse, lo, ctx.cfg,
+                              (dout, dq, dk, dv, dsl))
         need = int(L.load().dmt_attn_var_ws_bytes(C.byref(desc)))
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         desc.ws, desc.ws_bytes = ws.data_ptr(), need
@@ -1364,9 +1366,13 @@ def attn_var(q, k, v, seqs: AttnSeqs, H, Hkv=None, *, scale=None, cap=0.0, slope
     q_doc, k_doc = (None, None) if docs is None else (_ids(docs[0], q.shape[0], "docs[0]", q.device), _ids(docs[1], k.shape[0], "docs[1]", q.device))
     fill = (seqs.zero_fill, seqs.zero_fill) if seqs.zero_fill is not None else (seqs.total_q != q.shape[0], seqs.total_k != k.shape[0] or seqs.k_shared)
     cfg = (H, Hkv, scale, float(cap), bool(causal), seqs.max_q, seqs.max_k)
-    with torch.cuda.device(q.device):
-        out, lse = AttnVarFn.apply(_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), slopes, prefix, q_doc, k_doc, seqs.q_lens, seqs.q_off,
-                                   seqs.k_lens, seqs.k_off, cfg, fill, seqs.k_shared)
+    args = (_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), slopes, prefix, q_doc, k_doc, seqs.q_lens, seqs.q_off, seqs.k_lens, seqs.k_off, cfg,
+            fill, seqs.k_shared)
+    if _cur_device() == q.device.index:
+        out, lse = AttnVarFn.apply(*args)
+    else:
+        with torch.cuda.device(q.device):
+            out, lse = AttnVarFn.apply(*args)
     return (out, lse) if want_lse else out
 
 
