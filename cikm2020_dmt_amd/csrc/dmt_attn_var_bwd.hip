@@ -208,7 +208,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
   }
 }
 
-// dslopes[h] += sum of its parts, in their order (64 bits: the terms cancel)
+// dslopes[h] = sum of its parts, in their order (64 bits: the terms cancel)
 __device__ void sum_slopes(const float* part, long long n, float* out, double* red) {
   double s = 0.0;
   for (long long i = threadIdx.x; i < n; i += 256) s += (double)part[i];
@@ -218,7 +218,12 @@ __device__ void sum_slopes(const float* part, long long n, float* out, double* r
     if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *out += (float)red[0];
+  if (threadIdx.x == 0) *out = (float)red[0];
+}
+
+__global__ __launch_bounds__(256) void slopes_kernel(const Args a, long long n) {
+  __shared__ double red[256];
+  sum_slopes(a.slope_part + (long long)blockIdx.x * n, n, a.dslopes + blockIdx.x, red);
 }
 
 // dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
@@ -475,8 +480,11 @@ int launch_bwd(Args a, hipStream_t st) {
     else if (a.dh <= 80) launch_dq<T, 80>(a, st);
     else launch_dq<T, 128>(a, st);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq)");
-  } else {
-    a.slope_part = nullptr;                               // (no query: nothing to add)
+  }
+  if (a.slope_part && (!nkt || !a.rows_q || !nqt)) {      // (no dK / dV kernel to finish them, or no query at all: n = 0)
+    slopes_kernel<<<a.Hq, 256, 0, st>>>(a, a.rows_q && nqt ? (long long)a.B * nqt : 0);
+    DMT_CHECK_LAUNCH("dmt_attn_var_bwd(slopes)");
+    a.slope_part = nullptr;
   }
   if (nkt) {
     if (a.dh <= 32) launch_dkv<T, 32>(a, nkt, nqt, st);

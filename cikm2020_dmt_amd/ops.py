@@ -1299,7 +1299,8 @@ class AttnVarFn(torch.autograd.Function):
         rng = _var_doc_ranges(q_doc, q_lens.shape[0], cfg[5], cfg[6])
         desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg)
         L.call("dmt_attn_var_fwd", C.byref(desc), stream_ptr())
-        ctx.save_for_backward(q, k, v, slopes, prefix, q_doc, k_doc, rng, *lens, out, lse, lo)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, lo)
+        ctx.ints = (prefix, q_doc, k_doc, rng), lens
         ctx.cfg, ctx.fill, ctx.need_sl, ctx.k_shared = cfg, fill, need_sl, k_shared
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -1307,18 +1308,18 @@ class AttnVarFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dlse):
-        q, k, v, slopes, prefix, q_doc, k_doc, rng, q_lens, q_off, k_lens, k_off, out, lse, lo = ctx.saved_tensors
+        q, k, v, slopes, out, lse, lo = ctx.saved_tensors
+        masks, lens = ctx.ints
         if dout is None:
             return (None,) * 14
         if ctx.k_shared:
             raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
         dout = _aligned_rows(dout)
-        nq, nk = (torch.zeros_like if f else torch.empty_like for f in ctx.fill)
-        fmt = dict(memory_format=torch.contiguous_format)
-        dq, dk, dv = nq(q, **fmt), nk(k, **fmt), nk(v, **fmt)
-        dsl = torch.zeros_like(slopes) if ctx.need_sl else None
-        desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, (q_lens, q_off, k_lens, k_off), out, lse, lo, ctx.cfg,
-                              (dout, dq, dk, dv, dsl))
+        nq, nk = (torch.zeros if f else torch.empty for f in ctx.fill)
+        dq = nq(q.shape, dtype=q.dtype, device=q.device)
+        dk, dv = nk(k.shape, dtype=k.dtype, device=k.device), nk(v.shape, dtype=v.dtype, device=v.device)
+        dsl = torch.empty_like(slopes) if ctx.need_sl else None
+        desc = _attn_var_desc(q, k, v, slopes, *masks, lens, out, lse, lo, ctx.cfg, (dout, dq, dk, dv, dsl))
         need = int(L.load().dmt_attn_var_ws_bytes(C.byref(desc)))
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
         desc.ws, desc.ws_bytes = ws.data_ptr(), need

@@ -312,3 +312,14 @@ def test_many_histories_give_the_same_results_again(cuda, dh, kw):
     lse = torch.logsumexp(z, -1).transpose(1, 2)[ok]
     assert (first[0].float() - want).abs().max() <= 2.0 ** -8 * 2 * float(v.abs().max())      # two roundings of values of at most max |v|
     assert (first[1] - lse).abs().max() <= 1e-4
+
+
+def test_slopes_without_queries_or_keys(cuda):
+    """gradients where there is nothing to see: zeros, and nothing left unwritten"""
+    sl = torch.tensor([0.3, 0.1], device=cuda)
+    for ql, kl in (([0, 0], [5, 3]), ([4, 2], [0, 0]), ([0], [0])):
+        lv = [torch.randn((n, 2 * 32), device=cuda).to(BF).requires_grad_(True) for n in (sum(ql), sum(kl), sum(kl))] + [sl.clone().requires_grad_(True)]
+        out = ops.attn_var(*lv[:3], ops.AttnSeqs(ql, kl, device=cuda), 2, slopes=lv[3])
+        assert (out == 0).all()
+        for g, x in zip(torch.autograd.grad(out, lv, torch.ones_like(out)), lv):
+            assert g.shape == x.shape and (g == 0).all()
