@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libdmt_hip.so")
@@ -151,6 +152,18 @@ class KvAttnDesc(C.Structure):
                 ("width", c_i32), ("rows", c_i64), ("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("Q", c_vp), ("q_rs", c_i64),
                 ("table", c_vp), ("lens", c_vp), ("row_off", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32), ("slopes", c_vp),
                 ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
+
+
+def _packer(desc):
+    """struct.Struct of a descriptor's fields in their order: filling one by name costs three times as much (it is done in every call)"""
+    code = {c_i32: "i", c_i64: "q", c_f32: "f", c_vp: "P", C.c_uint64: "Q"}
+    st = struct.Struct("@" + "".join(code[t] for _, t in desc._fields_))
+    assert st.size <= C.sizeof(desc) < st.size + 8, desc.__name__
+    pad = b"\0" * (C.sizeof(desc) - st.size)
+    return lambda *values: desc.from_buffer_copy(st.pack(*values) + pad)
+
+
+attn_var_desc, kv_attn_desc = _packer(AttnVarDesc), _packer(KvAttnDesc)      # NULL pointers are 0 here
 
 
 _SIGS = {

@@ -96,7 +96,7 @@ def kv_plan(lens, new_lens, table, free, n_free, rows) -> KVPlan:
     runs = min(rows, rows // BLOCK + 2 * n)
     need = 16 + 8 * n                                                            # dmt_kv_plan_ws_bytes
     sizes = (n + 1, n, rows, runs, runs, 1, 1)
-    buf = torch.empty(need // 4 + sum(sizes), dtype=torch.int32, device=dev)     # one allocation: the step is a matter of microseconds
+    buf = lens.new_empty(need // 4 + sum(sizes))     # one allocation: the step is a matter of microseconds
     base = buf.data_ptr()
     out = torch.split_with_sizes(buf, (need // 4,) + sizes)
     a0 = base + need
@@ -177,7 +177,7 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
         raise ValueError("max_q and max_len must not be negative")
     given = out is not None
     if not given:
-        out = torch.empty((q.shape[0], w), dtype=BF16, device=dev)
+        out = q.new_empty((q.shape[0], w))
     elif out.shape != q.shape:
         raise ValueError("out must be %s" % list(q.shape))
     o_rs = _rows(out, "out", w, dev) if given else w
@@ -190,11 +190,11 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
         d = L.KvAttnDesc()
         d.n, d.Hq, d.Hkv, d.dh, d.max_q, d.max_len = n, H, cache.Hkv, cache.dh, int(max_q), max_len
         need = cache._ws_bytes[key] = int(L.load().dmt_kv_attn_ws_bytes(C.byref(d)))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = cache._args
-    d = L.KvAttnDesc(n, H, a[0], a[1], a[2], int(max_q), max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
-                     table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0,
-                     None if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, None if lse is None else lse.data_ptr(),
-                     None if ws is None else ws.data_ptr(), need)
+    d = L.kv_attn_desc(n, H, a[0], a[1], a[2], int(max_q), max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
+                       table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0,
+                       0 if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, 0 if lse is None else lse.data_ptr(),
+                       0 if ws is None else ws.data_ptr(), need)
     _call(dev, "dmt_kv_attn", C.byref(d))
     return (out, lse) if want_lse else out

@@ -1257,7 +1257,7 @@ def _aligned_rows(t):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _row_stride(t):
@@ -1270,10 +1270,10 @@ def _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, l
     dout, dq, dk, dv, dsl = grads or (None,) * 5
     g = (0,) * 8 if grads is None else (dout.data_ptr(), _row_stride(dout), dq.data_ptr(), dq.shape[1], dk.data_ptr(), dk.shape[1], dv.data_ptr(),
                                         dv.shape[1])
-    return L.AttnVarDesc(dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k, q.shape[0], k.shape[0], q.data_ptr(), _row_stride(q),
-                         k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), lens[1].data_ptr(), lens[0].data_ptr(), lens[3].data_ptr(),
-                         lens[2].data_ptr(), scale, cap, 1 if causal else 0, _ptr(slopes), _ptr(prefix), _ptr(q_doc), _ptr(k_doc), out.data_ptr(),
-                         out.shape[1], _ptr(lse), _ptr(lo), g[0], g[1], g[2], g[3], g[4], g[5], g[6], g[7], _ptr(dsl), _ptr(rng), None, 0)
+    return L.attn_var_desc(dt_code(q.dtype), lens[0].shape[0], H, Hkv, q.shape[1] // H, max_q, max_k, q.shape[0], k.shape[0], q.data_ptr(), _row_stride(q),
+                           k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), lens[1].data_ptr(), lens[0].data_ptr(), lens[3].data_ptr(),
+                           lens[2].data_ptr(), scale, cap, 1 if causal else 0, _ptr(slopes), _ptr(prefix), _ptr(q_doc), _ptr(k_doc), out.data_ptr(),
+                           out.shape[1], _ptr(lse), _ptr(lo), g[0], g[1], g[2], g[3], g[4], g[5], g[6], g[7], _ptr(dsl), _ptr(rng), 0, 0)
 
 
 def _var_doc_ranges(q_doc, B, max_q, max_k):
@@ -1290,9 +1290,8 @@ class AttnVarFn(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes, prefix, q_doc, k_doc, q_lens, q_off, k_lens, k_off, cfg, fill, k_shared):
         H, Hkv = cfg[:2]
         rows, d = q.shape
-        new = torch.zeros if fill[0] else torch.empty
-        out = new((rows, d), dtype=q.dtype, device=q.device)
-        lse = torch.full((rows, H), -float("inf"), device=q.device) if fill[0] else torch.empty((rows, H), dtype=F32, device=q.device)
+        out = q.new_zeros((rows, d)) if fill[0] else q.new_empty((rows, d))
+        lse = torch.full((rows, H), -float("inf"), device=q.device) if fill[0] else q.new_empty((rows, H), dtype=F32)
         need_sl = slopes is not None and ctx.needs_input_grad[3]
         lens = (q_lens, q_off, k_lens, k_off)
         lo = torch.empty_like(out) if q.dtype != F32 and any(ctx.needs_input_grad[:4]) else None
@@ -1315,13 +1314,12 @@ class AttnVarFn(torch.autograd.Function):
         if ctx.k_shared:
             raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
         dout = _aligned_rows(dout)
-        nq, nk = (torch.zeros if f else torch.empty for f in ctx.fill)
-        dq = nq(q.shape, dtype=q.dtype, device=q.device)
-        dk, dv = nk(k.shape, dtype=k.dtype, device=k.device), nk(v.shape, dtype=v.dtype, device=v.device)
+        dq = q.new_zeros(q.shape) if ctx.fill[0] else q.new_empty(q.shape)
+        dk, dv = (k.new_zeros(k.shape), v.new_zeros(v.shape)) if ctx.fill[1] else (k.new_empty(k.shape), v.new_empty(v.shape))
         dsl = torch.empty_like(slopes) if ctx.need_sl else None
         desc = _attn_var_desc(q, k, v, slopes, *masks, lens, out, lse, lo, ctx.cfg, (dout, dq, dk, dv, dsl))
         need = int(L.load().dmt_attn_var_ws_bytes(C.byref(desc)))
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
+        ws = q.new_empty(need, dtype=torch.uint8)
         desc.ws, desc.ws_bytes = ws.data_ptr(), need
         L.call("dmt_attn_var_bwd", C.byref(desc), stream_ptr())
         return (dq, dk, dv, dsl) + (None,) * 10
