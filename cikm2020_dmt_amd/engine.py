@@ -780,6 +780,27 @@ class DMTEngine:
             y = self.ff(s, blk + ffs)
         return y
 
+    def memory_kv(self, mem, i, j):
+        """(K | V) rows [.., 2 d] that decoder block j of sequence i projects from its memory: what serving.HistoryCache keeps."""
+        d = self.spec["d_model"]
+        a = trans_prefix(i) + "num_blocks_%d/vanilla_attention/" % j
+        wl, bl, w = self._lf(a + "qkv_kernel"), self._lf(a + "qkv_bias"), self._w(a + "qkv_kernel")
+        return ops.linear(mem, wl[:, d:], bl[d:], self._wslice(w, d, 3 * d))
+
+    def decode_cached(self, y, i, attend):
+        """decode_prepared for candidate rows y [B, d] whose memories are held elsewhere: attend(j, q) -> [B, d] attends block j's queries to
+        them (serving.HistoryCache.attend).  Inference only (no dropout)."""
+        d = self.spec["d_model"]
+        ffs = "positionwise_feedforward/" if self.spec.get("tie_ffn", True) else "positionwise_feedforward_dec/"
+        for j in range(int(self.spec.get("num_blocks_decode", 1))):
+            blk = trans_prefix(i) + "num_blocks_%d/" % j
+            a = blk + "vanilla_attention/"
+            wl, bl, w = self._lf(a + "qkv_kernel"), self._lf(a + "qkv_bias"), self._w(a + "qkv_kernel")
+            s = attend(j, ops.linear(y, wl[:, :d], bl[:d], self._wslice(w, 0, d))) + y
+            s = ops.layer_norm(s.unsqueeze(1), self._lf(a + "ln/gamma"), self._lf(a + "ln/beta"))
+            y = self.ff(s, blk + ffs).squeeze(1)
+        return y
+
     def interest_blocks(self, us, tars_scaled):
         """The d_model-wide blocks of interest_state: user_stat per sequence, each followed by the RAW target embedding when
         is_trans_out_concat_item (mmoe_transformer_unbias.py:212-219; the gather hands out the decoder's copy, scaled by sqrt(d_model):

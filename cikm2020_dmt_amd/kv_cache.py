@@ -187,6 +187,8 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
     key = (n, H, int(max_q), max_len)
     need = cache._ws_bytes.get(key)
     if need is None:                   # (a function of the sizes alone)
+        if len(cache._ws_bytes) >= 4096:
+            cache._ws_bytes.clear()
         d = L.KvAttnDesc()
         d.n, d.Hq, d.Hkv, d.dh, d.max_q, d.max_len = n, H, cache.Hkv, cache.dh, int(max_q), max_len
         need = cache._ws_bytes[key] = int(L.load().dmt_kv_attn_ws_bytes(C.byref(d)))

@@ -7,7 +7,8 @@ the request are tiled across the candidate batch and the ordinary predict graph 
 The reference re-encodes the user's behaviour sequences for every candidate row.  Here the three sequence encoders (self-
 attention + FFN over [T, d]) and the K | V projections of their memories run ONCE per request; every candidate only pays for
 its own embedding lookups, the single-query decoder attention against the shared memory (zero batch stride), MMoE and the
-towers.  Same numbers as Inference.inference(tiled batch, is_predict=True) -- checked in tests/test_gpu_serving.py.
+towers.  CandidateScorer.keep_histories holds the projected memories of many users between requests (HistoryCache, 8 bits), so
+that candidates of several users are scored in one batch with no encoder in it.  Same numbers as Inference.inference(tiled batch, is_predict=True) -- checked in tests/test_gpu_serving.py.
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ import numpy as np
 import torch
 
 from .engine import AssembleFn, DeviceBatch, DMTEngine, FeatureColumn
+from .kv_cache import BLOCK, KVCache, kv_append, kv_attn, kv_plan, kv_release
 
 
 def normalisation_constants(mean: Sequence[float], std: Sequence[float]):
@@ -33,6 +35,44 @@ def normalise_dense(raw: torch.Tensor, const_vec: torch.Tensor, std: torch.Tenso
     x = torch.clamp(raw.float(), min=0.0)      # (the upper bound sys.float_info.max is no bound for float32)
     y = x * std / (torch.square(std + 1e-7) * 3.0) - const_vec
     return torch.clamp(y, min=-0.99, max=0.99)
+
+
+class HistoryCache:
+    """K / V of many users' histories in 8 bits between requests (kv_cache.py): `n_users` places, each holding up to max_len rows in 64-row
+    blocks of one pool per layer; all layers share the block table.  Rows are appended for any set of users at a time, queries of any set of
+    users attend in one launch, a user's place is given up and its blocks return to the pool -- all on the GPU, in stream order."""
+
+    def __init__(self, n_users, n_blocks, max_len, num_heads, head_dim, layers=1, device="cuda"):
+        if n_users <= 0 or n_blocks <= 0 or max_len <= 0 or layers <= 0:
+            raise ValueError("HistoryCache needs at least one user, block, row and layer")
+        self.layers = [KVCache.empty(n_blocks, num_heads, head_dim, device) for _ in range(layers)]
+        i32 = dict(dtype=torch.int32, device=self.layers[0].device)
+        width = -(-max_len // BLOCK)
+        self.n_users, self.max_len = int(n_users), width * BLOCK                 # (whole blocks)
+        self.table = torch.full((n_users, width), -1, **i32)
+        self.lens = torch.zeros((n_users,), **i32)
+        self.free = torch.arange(n_blocks, **i32)
+        self.n_free = torch.full((1,), n_blocks, **i32)
+
+    def append(self, rows, new_lens):
+        """rows: one (k_rows, v_rows) pair per layer, bf16 [R, num_heads * head_dim], the users' new rows in the order of their places; new_lens:
+        int32 [n_users] (0: nothing).  Returns the KVPlan: plan.refused counts users whose rows found no room (their histories stay)."""
+        if len(rows) != len(self.layers):
+            raise ValueError("%d layers, got rows for %d" % (len(self.layers), len(rows)))
+        plan = kv_plan(self.lens, new_lens, self.table, self.free, self.n_free, rows[0][0].shape[0])
+        for cache, (k, v) in zip(self.layers, rows):
+            kv_append(cache, k, v, plan)
+        self.lens, self.n_free = plan.lens, plan.n_free
+        return plan
+
+    def attend(self, layer, q, row_off, num_heads, max_q, **kw):
+        """kv_attn of one layer: user r's query rows are row_off[r] .. row_off[r + 1] of q"""
+        return kv_attn(self.layers[layer], q, self.table, self.lens, row_off, num_heads, max_q, **kw)
+
+    def drop(self, done):
+        """done: int32 [n_users], non-zero: forget that user"""
+        self.lens, self.n_free = self.lens.clone(), self.n_free.clone()          # (a plan of an earlier step keeps its own)
+        kv_release(done, self.lens, self.table, self.free, self.n_free)
 
 
 class CandidateScorer:
@@ -87,14 +127,17 @@ class CandidateScorer:
         feats = {f: FeatureColumn(c.idx[:1], c.wts[:1] if c.wts is not None else None, c.lens[:1], c.T) for f, c in batch.feats.items()}
         return DeviceBatch(1, feats, batch.dense[:1])
 
+    def _fresh_tables(self):
+        if self.optimizer is not None and self.optimizer.global_step != self._flushed_at:
+            self.optimizer.flush_tables()
+            self._flushed_at = self.optimizer.global_step
+
     # ------------------------------------------------------------------ scoring
     @torch.no_grad()
     def logits(self, batch: DeviceBatch):
         """(click_logit, order_logit) [B, 1] for B candidate rows of one user; user-side columns are read from row 0."""
         eng, spec = self.engine, self.spec
-        if self.optimizer is not None and self.optimizer.global_step != self._flushed_at:
-            self.optimizer.flush_tables()
-            self._flushed_at = self.optimizer.global_step
+        self._fresh_tables()
         saved_seed, eng.dropout_step_seed = eng.dropout_step_seed, None        # predict graph: is_train=False
         try:
             b1 = self._row0(batch)
@@ -111,6 +154,90 @@ class CandidateScorer:
                 us.append(eng.decode_shared(eng.decoder_query(tar_i).unsqueeze(1), mem1, k_lens, i).squeeze(1))
             z = AssembleFn.apply(zbuf, eng.plan.interest_off, spec["d_model"], *eng.interest_blocks(us, tars_scaled))
             tasks = eng.expert_gate(z, z_is_engine_buffer=True)          # (z is gather_pooled's zero-initialised zbuf)
+            return tuple(eng.build_tower(m, nm) for m, nm in zip(tasks, ("click", "order")))
+        finally:
+            eng.dropout_step_seed = saved_seed
+
+    # ------------------------------------------------------------------ histories kept between requests
+    def keep_histories(self, n_users, n_blocks):
+        """Make room for the encoded histories of n_users users (n_blocks blocks of 64 rows a sequence): remember() encodes a user once,
+        logits_of() then scores candidates of many users in one batch without running an encoder.  For bf16 engines with a head size that
+        is a multiple of 16 (the E64 widths); the decoder's K / V are held in 8 bits, so its attention is that of the rounded rows."""
+        eng, spec = self.engine, self.spec
+        if eng.store.compute_dtype != torch.bfloat16:
+            raise ValueError("histories are kept for bf16 engines")
+        if spec.get("is_trans_input_by_mlp"):
+            raise ValueError("histories are not kept for is_trans_input_by_mlp models")
+        H, layers = spec["num_heads"], int(spec.get("num_blocks_decode", 1))
+        self.histories = [HistoryCache(n_users, n_blocks, spec["maxlen_k"], H, spec["d_model"] // H, layers, eng.store.device)
+                          for _ in spec["attention_embed_pairs"]]
+
+    def _places(self, users, B):
+        if not hasattr(self, "histories"):
+            raise RuntimeError("keep_histories() first")
+        users, n = np.asarray(users, dtype=np.int64), self.histories[0].n_users
+        if users.shape != (B,) or B == 0:
+            raise ValueError("one place for each row of the batch")
+        if users.min() < 0 or users.max() >= n:
+            raise ValueError("places lie in 0 .. %d" % (n - 1))
+        return users, n
+
+    @torch.no_grad()
+    def remember(self, users, batch: DeviceBatch):
+        """Encode row r of `batch` as the history of place users[r] (distinct places; what stood there is replaced).  Returns the number of
+        (user, sequence) histories that found no room: those are empty then, and attention over an empty history gives zeros.  A history
+        is as old as the weights that encoded it: after training steps, remember it again."""
+        eng, spec = self.engine, self.spec
+        users, n = self._places(users, batch.B)
+        if len(np.unique(users)) != len(users):
+            raise ValueError("the places of one call must be distinct")
+        self._fresh_tables()
+        dev, d = eng.store.device, spec["d_model"]
+        order = np.argsort(users)                                # rows go in in the order of the places
+        done = np.zeros(n, dtype=np.int32)
+        done[users] = 1
+        # (dense rows: without host lengths no sequence is packed)
+        dense = DeviceBatch(batch.B, {f: FeatureColumn(c.idx, c.wts, c.lens, c.T) for f, c in batch.feats.items()}, batch.dense)
+        saved_seed, eng.dropout_step_seed = eng.dropout_step_seed, None
+        try:
+            X, _tar, _z = eng.gather(dense)
+            refused = 0
+            for i, h in enumerate(self.histories):
+                lens, T = eng.seq_lens(dense, i), X[i].shape[1]
+                new = np.zeros(n, dtype=np.int32)
+                new[users] = np.minimum(lens.cpu().numpy(), T)
+                at = torch.as_tensor(np.concatenate([r * T + np.arange(new[users[r]]) for r in order])).to(dev)
+                mem = eng.encode_prepared(X[i], lens, i)
+                rows = []
+                for j in range(len(h.layers)):
+                    kv = eng.memory_kv(mem, i, j).reshape(-1, 2 * d)[at]
+                    rows.append((kv[:, :d], kv[:, d:]))
+                h.drop(torch.as_tensor(done).to(dev))
+                refused += int(h.append(rows, torch.as_tensor(new).to(dev)).refused)
+            return refused
+        finally:
+            eng.dropout_step_seed = saved_seed
+
+    @torch.no_grad()
+    def logits_of(self, users, batch: DeviceBatch):
+        """(click_logit, order_logit) [B, 1] for candidate rows of remembered users: users[r] is the place of row r's user, in ascending
+        order (rows of one user side by side).  The sequence columns of `batch` are not read by the attention."""
+        eng, spec = self.engine, self.spec
+        users, n = self._places(users, batch.B)
+        if (np.diff(users) < 0).any():
+            raise ValueError("the places must stand in ascending order")
+        self._fresh_tables()
+        count = np.bincount(users, minlength=n)
+        row_off = torch.as_tensor(np.concatenate([[0], np.cumsum(count)]).astype(np.int32)).to(eng.store.device)
+        saved_seed, eng.dropout_step_seed = eng.dropout_step_seed, None
+        try:
+            tar, zbuf = eng.gather_pooled(batch)
+            us = []
+            for i, h in enumerate(self.histories):
+                attend = lambda j, q, h=h: h.attend(j, q, row_off, spec["num_heads"], int(count.max()), causal=False)  # noqa: E731
+                us.append(eng.decode_cached(eng.decoder_query(tar), i, attend))
+            z = AssembleFn.apply(zbuf, eng.plan.interest_off, spec["d_model"], *eng.interest_blocks(us, [tar] * len(us)))
+            tasks = eng.expert_gate(z, z_is_engine_buffer=True)
             return tuple(eng.build_tower(m, nm) for m, nm in zip(tasks, ("click", "order")))
         finally:
             eng.dropout_step_seed = saved_seed

@@ -1,0 +1,127 @@
+"""Serving from kept histories: CandidateScorer.remember / logits_of against the same decoder over the values that the cache holds, and
+HistoryCache's bookkeeping."""
+import numpy as np
+import pytest
+import torch
+
+from cikm2020_dmt_amd import kv_cache as KV
+from cikm2020_dmt_amd import ops
+from cikm2020_dmt_amd import spec as S
+from cikm2020_dmt_amd.data_feed.synthetic import make_batch
+from cikm2020_dmt_amd.engine import AssembleFn, trans_prefix
+from cikm2020_dmt_amd.serving import CandidateScorer, HistoryCache
+from cikm2020_dmt_amd.train import Trainer
+
+pytestmark = pytest.mark.gpu
+ROWS = {"Sku": 3000, "Brand": 800, "Shopid": 900, "Cid3": 300, "Cid2": 50}
+
+
+def _trainer(cuda, dtype=torch.bfloat16, **opt):
+    sp = dict(S.scaled_spec(S.e64_spec(), ROWS), **opt)
+    return sp, Trainer(sp, device=cuda, compute_dtype=dtype, init=True, dropout=False)
+
+
+def _expected(sc, users, batch):
+    """logits_of with the attention of the tiled request path over the rows that the cache holds for each candidate's user"""
+    eng, spec = sc.engine, sc.spec
+    d, H = spec["d_model"], spec["num_heads"]
+    with torch.no_grad():
+        tar, zbuf = eng.gather_pooled(batch)
+        us = []
+        for i, h in enumerate(sc.histories):
+            y = eng.decoder_query(tar).unsqueeze(1)
+            L = h.lens[torch.as_tensor(users, device=h.lens.device)].contiguous()
+            T = int(L.max())
+            for j, cache in enumerate(h.layers):
+                blk = trans_prefix(i) + "num_blocks_%d/" % j
+                a = blk + "vanilla_attention/"
+                wl, bl, w = eng._lf(a + "qkv_kernel"), eng._lf(a + "qkv_bias"), eng._w(a + "qkv_kernel")
+                q = ops.linear(y, wl[:, :d], bl[:d], eng._wslice(w, 0, d))
+                pos = torch.arange(T, device=tar.device)
+                slots = h.table[torch.as_tensor(users, device=tar.device)][:, pos // 64] * 64 + pos % 64
+                k, v = KV.kv_read(cache, slots.to(torch.int32).reshape(-1).contiguous())
+                kv = torch.cat([k, v], 1).reshape(len(users), T, 2 * d)
+                s = ops.AttnFn.apply(q, kv, y, None, L, H, d, False, 0, 1.0, eng.kopts)
+                s = ops.layer_norm(s, eng._lf(a + "ln/gamma"), eng._lf(a + "ln/beta"))
+                y = eng.ff(s, blk + "positionwise_feedforward/")
+            us.append(y.squeeze(1))
+        z = AssembleFn.apply(zbuf, eng.plan.interest_off, d, *eng.interest_blocks(us, [tar] * len(us)))
+        tasks = eng.expert_gate(z, z_is_engine_buffer=True)
+        return [eng.build_tower(m, nm) for m, nm in zip(tasks, ("click", "order"))]
+
+
+def _one_user_rows(sp, tr, seed, n):
+    inputs, mask, label = make_batch(sp, n, seed=seed, lengths="ragged", weights="random")
+    return tr.make_batch(inputs, mask, label)
+
+
+@pytest.mark.parametrize("opt", [dict(), dict(num_blocks_decode=2)])
+def test_candidates_of_remembered_users(cuda, opt):
+    """several users at once, replaced and extended histories, users without candidates; tolerance: the bf16 one of the request path"""
+    sp, tr = _trainer(cuda, **opt)
+    sc = CandidateScorer(tr.engine)
+    sc.keep_histories(9, 40)
+    assert sc.remember([4, 0, 7, 2], _one_user_rows(sp, tr, 3, 4)) == 0
+    assert sc.remember([7, 8], _one_user_rows(sp, tr, 4, 2)) == 0                # 7 again: replaced
+    users = [0] * 5 + [2] * 1 + [7] * 33 + [8] * 2
+    batch = _one_user_rows(sp, tr, 9, len(users))
+    got, want = sc.logits_of(users, batch), _expected(sc, users, batch)
+    for g, w in zip(got, want):
+        assert torch.allclose(g.float(), w.float(), atol=4e-2, rtol=4e-2)
+    for h in sc.histories:                                                        # every block is in one table or free
+        held = [b for t, L in zip(h.table.tolist(), h.lens.tolist()) for b in t[:-(-L // 64)]]
+        assert sorted(held + h.free[:int(h.n_free)].tolist()) == list(range(40))
+
+
+def test_histories_follow_the_encoder(cuda):
+    """the cached K / V are the decoder's projections of the encoded rows, each within half a step of e4m3 at its block's scale (2^-4 of the
+    value, 2^-10 of the scale below the normal range)"""
+    sp, tr = _trainer(cuda)
+    eng, d = tr.engine, sp["d_model"]
+    sc = CandidateScorer(eng)
+    sc.keep_histories(3, 12)
+    batch = _one_user_rows(sp, tr, 5, 3)
+    users = [2, 0, 1]
+    assert sc.remember(users, batch) == 0
+    eng.packed_rows = False                                                       # [B, T, d] below
+    with torch.no_grad():
+        X, _t, _z = eng.gather(batch)
+        for i, pairs in enumerate(sp["attention_embed_pairs"]):
+            lens = batch.feats[pairs[-1][0]].lens
+            kv = eng.memory_kv(eng.encode_prepared(X[i], lens, i), i, 0).float()
+            h = sc.histories[i]
+            for r, u in enumerate(users):
+                L = int(lens[r])
+                assert int(h.lens[u]) == L
+                pos = torch.arange(L, device=cuda)
+                slots = (h.table[u][pos // 64] * 64 + pos % 64).to(torch.int32)
+                k, v = KV.kv_read(h.layers[0], slots)
+                for got, want, sc_ in ((k, kv[r, :L, :d], h.layers[0].k_scale), (v, kv[r, :L, d:], h.layers[0].v_scale)):
+                    step = sc_[(slots // 64).long()].repeat_interleave(d // sp["num_heads"], 1)
+                    assert ((got.float() - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * step).all()
+
+
+def test_no_room_and_refusals(cuda):
+    sp, tr = _trainer(cuda)
+    sc = CandidateScorer(tr.engine)
+    sc.keep_histories(4, 2)
+    assert sc.remember([0, 1, 2, 3], _one_user_rows(sp, tr, 5, 4)) == 6          # 2 blocks a sequence, 4 users of one block each, 3 sequences
+    batch = _one_user_rows(sp, tr, 5, 2)
+    with pytest.raises(RuntimeError, match="keep_histories"):
+        CandidateScorer(tr.engine).logits_of([0, 0], batch)
+    for bad in ([0, 0], [0], [0, 4], [-1, 0]):
+        with pytest.raises(ValueError):
+            sc.remember(bad, batch)
+    for bad in ([1, 0], [0], [0, 4]):
+        with pytest.raises(ValueError):
+            sc.logits_of(bad, batch)
+    with pytest.raises(ValueError, match="bf16"):
+        CandidateScorer(_trainer(cuda, torch.float32)[1].engine).keep_histories(4, 2)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        CandidateScorer(Trainer(S.scaled_spec(S.default_spec(), ROWS), device=cuda, compute_dtype=torch.bfloat16, dropout=False).engine).keep_histories(4, 2)
+    with pytest.raises(ValueError):
+        HistoryCache(0, 4, 64, 2, 32)
+    h = HistoryCache(2, 4, 64, 2, 32, layers=2)
+    x = torch.zeros((1, 64), dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(ValueError, match="2 layers"):
+        h.append([(x, x)], torch.tensor([1, 0], dtype=torch.int32, device=cuda))
