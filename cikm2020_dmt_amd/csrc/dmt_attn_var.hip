@@ -340,6 +340,7 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
     DMT_CHECK_ARG(w.total == 0 || (d->ws && ((uintptr_t)d->ws % 16) == 0 && d->ws_bytes >= w.total), "%s: workspace of %llu bytes needed", what,
                   (unsigned long long)w.total);
   }
+  DMT_CHECK_ARG(d->rows_q == 0 || (d->out != d->Q && d->out != d->K && d->out != d->V), "%s: out must not be an operand", what);
   char* ws = (char*)d->ws;
   a->B = d->B; a->Hq = d->Hq; a->Hkv = d->Hkv; a->dh = d->dh; a->G = d->Hq / d->Hkv;
   a->max_q = d->max_q; a->max_k = d->max_k; a->rows_q = d->rows_q; a->rows_k = d->rows_k;

@@ -904,6 +904,7 @@ extern "C" int dmt_kv_plan(int32_t n, int32_t rows, const int32_t* lens, const i
   DMT_CHECK_ARG(rows == 0 || (slots && run_row && run_len), "dmt_kv_plan: NULL slots / run_row / run_len");
   DMT_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= dmt_kv_plan_ws_bytes(n), "dmt_kv_plan: workspace of %llu bytes needed",
                 (unsigned long long)dmt_kv_plan_ws_bytes(n));
+  DMT_CHECK_ARG(state != n_free && (n == 0 || lens_out != lens), "dmt_kv_plan: lens_out and state are written before lens and n_free were read");
   PlanArgs a;
   a.n = n; a.rows = rows; a.width = width;
   const long long mr = (long long)rows / BS + 2ll * n;
@@ -969,8 +970,14 @@ static uint64_t kv_ws(const dmt_kv_attn_desc* d, Split* s, int* nq, uint64_t* ml
   return s->pieces > 1 ? cols * ((uint64_t)d->dh * 4 + 8) : 0;
 }
 
+// (split_of and kv_ws count in 64 bits: n Hkv and the tiles of columns stay below 2^31 each and together)
+static bool launch_fits(const dmt_kv_attn_desc* d) {
+  const int64_t cols = (int64_t)d->max_q * (d->Hq / d->Hkv), heads = (int64_t)d->n * d->Hkv;
+  return cols < (1ll << 31) && heads < (1ll << 31) && heads * cdiv64(cols, cols <= 32 ? 16 : 32) < (1ll << 31);
+}
+
 extern "C" uint64_t dmt_kv_attn_ws_bytes(const dmt_kv_attn_desc* d) {
-  if (!d || d->n <= 0 || d->Hkv <= 0 || d->Hq < d->Hkv || d->max_q <= 0 || d->max_len <= 0 || d->dh <= 0) return 0;
+  if (!d || d->n <= 0 || d->Hkv <= 0 || d->Hq < d->Hkv || d->max_q <= 0 || d->max_len <= 0 || d->dh <= 0 || !launch_fits(d)) return 0;
   Split s;
   int nq;
   uint64_t ml;
@@ -994,13 +1001,15 @@ extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
   a.n = d->n; a.Hq = d->Hq; a.G = d->Hq / d->Hkv; a.max_q = d->max_q; a.max_len = d->max_len; a.width = d->width; a.causal = d->causal != 0;
   a.rows = d->rows; a.Q = (const bf16_t*)d->Q; a.q_rs = d->q_rs; a.table = d->table; a.lens = d->lens; a.row_off = d->row_off;
   a.scale = d->scale; a.cap = d->cap; a.slopes = d->slopes; a.out = (bf16_t*)d->out; a.o_rs = d->o_rs; a.lse = d->lse;
+  DMT_CHECK_ARG(launch_fits(d), "dmt_kv_attn: the launch passes 2^31 workgroups");
   Split s;
   int nq;
   uint64_t ml_at;
   const uint64_t need = kv_ws(d, &s, &nq, &ml_at);
   DMT_CHECK_ARG(need == 0 || (d->ws && (uintptr_t)d->ws % 16 == 0 && d->ws_bytes >= need), "dmt_kv_attn: workspace of %llu bytes needed",
                 (unsigned long long)need);
-  DMT_CHECK_ARG((long long)d->n * d->Hkv * s.pieces * s.nqt < (1ll << 31), "dmt_kv_attn: the launch passes 2^31 workgroups");
+  DMT_CHECK_ARG((long long)d->n * d->Hkv * s.nqt * s.pieces < (1ll << 31), "dmt_kv_attn: the launch passes 2^31 workgroups");
+  DMT_CHECK_ARG(d->out != d->Q, "dmt_kv_attn: out must not be Q");
   float* po = (float*)d->ws;
   float2* ml = need ? (float2*)((char*)d->ws + ml_at) : nullptr;
   if (nq == 1) launch_kv_dh<1>(a, s, po, ml, (hipStream_t)stream);

@@ -85,6 +85,8 @@ def kv_plan(lens, new_lens, table, free, n_free, rows) -> KVPlan:
     dev = lens.device
     if not lens.is_cuda:
         raise RuntimeError("libdmt_hip kernels need device tensors (got a %s tensor); there is no CPU path" % dev)
+    if lens.dim() != 1 or table.dim() != 2:
+        raise ValueError("lens is [n] and table [n, width], got %s and %s" % (list(lens.shape), list(table.shape)))
     n, width, rows = lens.shape[0], table.shape[1], int(rows)
     _i32(lens, (n,), "lens", dev)
     _i32(new_lens, (n,), "new_lens", dev)
@@ -110,8 +112,13 @@ def kv_plan(lens, new_lens, table, free, n_free, rows) -> KVPlan:
 
 
 def kv_release(done, lens, table, free, n_free):
-    """Requests r with done[r] != 0 (int32 [n]) give their blocks back: pushed on `free`, n_free and lens are changed in place."""
+    """Requests r with done[r] != 0 (int32 [n]) give their blocks back: pushed on `free`, n_free and lens are changed in place.  A block that
+    two tables name is pushed once for each."""
     dev, n = lens.device, lens.shape[0]
+    if not lens.is_cuda:
+        raise RuntimeError("libdmt_hip kernels need device tensors (got a %s tensor); there is no CPU path" % dev)
+    if lens.dim() != 1 or table.dim() != 2:
+        raise ValueError("lens is [n] and table [n, width], got %s and %s" % (list(lens.shape), list(table.shape)))
     _i32(done, (n,), "done", dev)
     _i32(lens, (n,), "lens", dev)
     _i32(table, (n, table.shape[1]), "table", dev)
@@ -157,10 +164,13 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
             want_lse=False):
     """Attention of n requests' query rows over their cached tokens: q bf16 [rows, H * dh], request r owns rows row_off[r] .. row_off[r + 1]
     (int32 [n + 1]) and lens[r] tokens in the blocks table[r].  causal: its m rows stand at the positions lens - m .. lens - 1 (append
-    them first); otherwise every row stands behind the last token and sees all (candidates).  Scores as in ops.attn_var: scale, cap, slopes
+    them first; a request that the plan refused has nothing appended, so its rows stand over the last tokens that it held); otherwise
+    every row stands behind the last token and sees all (candidates).  Scores as in ops.attn_var: scale, cap, slopes
     (fp32 [H]).  max_q bounds the rows of a request, max_len the lengths (default: what the table can hold): they size the launch, so
     keep them fixed for a captured graph and tight for speed.  Rows past row_off[n] are not written; with `out` they stay as they were."""
     dev, n = cache.device, lens.shape[0]
+    if table.dim() != 2:
+        raise ValueError("table is [n, width], got %s" % list(table.shape))
     if H <= 0 or H % cache.Hkv:
         raise ValueError("H = %d query heads cannot share Hkv = %d key heads evenly" % (H, cache.Hkv))
     w = H * cache.dh
@@ -175,26 +185,29 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
         raise ValueError("scale must be positive and finite, cap 0 or positive and finite: got %r, %r" % (scale, cap))
     if max_q < 0 or (max_len is not None and max_len < 0):
         raise ValueError("max_q and max_len must not be negative")
+    max_q = min(int(max_q), q.shape[0])                                          # (no request has more rows than there are)
     given = out is not None
     if not given:
         out = q.new_empty((q.shape[0], w))
     elif out.shape != q.shape:
         raise ValueError("out must be %s" % list(q.shape))
+    elif out.data_ptr() == q.data_ptr() and q.shape[0]:
+        raise ValueError("out must not be q")
     o_rs = _rows(out, "out", w, dev) if given else w
     lse = torch.empty((q.shape[0], H), dtype=F32, device=dev) if want_lse else None
     most = table.shape[1] * BLOCK
     max_len = most if max_len is None else min(int(max_len), most)
-    key = (n, H, int(max_q), max_len)
+    key = (n, H, max_q, max_len)
     need = cache._ws_bytes.get(key)
     if need is None:                   # (a function of the sizes alone)
         if len(cache._ws_bytes) >= 4096:
             cache._ws_bytes.clear()
         d = L.KvAttnDesc()
-        d.n, d.Hq, d.Hkv, d.dh, d.max_q, d.max_len = n, H, cache.Hkv, cache.dh, int(max_q), max_len
+        d.n, d.Hq, d.Hkv, d.dh, d.max_q, d.max_len = n, H, cache.Hkv, cache.dh, max_q, max_len
         need = cache._ws_bytes[key] = int(L.load().dmt_kv_attn_ws_bytes(C.byref(d)))
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = cache._args
-    d = L.kv_attn_desc(n, H, a[0], a[1], a[2], int(max_q), max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
+    d = L.kv_attn_desc(n, H, a[0], a[1], a[2], max_q, max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
                        table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0,
                        0 if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, 0 if lse is None else lse.data_ptr(),
                        0 if ws is None else ws.data_ptr(), need)

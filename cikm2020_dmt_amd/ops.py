@@ -1298,8 +1298,8 @@ class AttnVarFn(torch.autograd.Function):
         rng = _var_doc_ranges(q_doc, q_lens.shape[0], cfg[5], cfg[6])
         desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg)
         L.call("dmt_attn_var_fwd", C.byref(desc), stream_ptr())
-        ctx.save_for_backward(q, k, v, slopes, out, lse, lo)
-        ctx.ints = (prefix, q_doc, k_doc, rng), lens
+        # (lengths and masks too: one that is changed in place before the backward is an error, not a wrong gradient)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, lo, prefix, q_doc, k_doc, rng, q_lens, q_off, k_lens, k_off)
         ctx.cfg, ctx.fill, ctx.need_sl, ctx.k_shared = cfg, fill, need_sl, k_shared
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -1307,10 +1307,12 @@ class AttnVarFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, _dlse):
-        q, k, v, slopes, out, lse, lo = ctx.saved_tensors
-        masks, lens = ctx.ints
+        q, k, v, slopes, out, lse, lo, *masks = ctx.saved_tensors
+        masks, lens = masks[:4], masks[4:]
         if dout is None:
             return (None,) * 14
+        if torch.is_grad_enabled():
+            raise RuntimeError("attn_var: its gradients have no gradient (create_graph=True)")
         if ctx.k_shared:
             raise RuntimeError("attn_var: examples that share key rows have no backward (their gradients would have to be summed)")
         dout = _aligned_rows(dout)

@@ -821,7 +821,7 @@ int dmt_q1mem_bwd(const dmt_q1mem_desc* d, void* stream);
  * A row that may see nothing gets out = 0, lse = -inf and no gradient.  What stands in a masked place -- NaN and infinities too -- does
  * not reach a row that may not see it.  Rows that belong to no example are neither read nor written.
  * Types: DMT_BF16 (dh a multiple of 8) and DMT_F32 (dh a multiple of 4), dh <= 128; sums, softmax statistics and gradients in fp32.
- * Every operand row 16-byte aligned (base and row stride).  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
+ * Every operand row 16-byte aligned (base and row stride); out is none of them.  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
  * caller's promise: it sizes the grid; longer examples are cut there).
  * Backward: dq, dk, dv for the rows of every example, and dslopes [Hq] (summed in a fixed order).
  * Bit-reproducible: no atomics.  ws: dmt_attn_var_ws_bytes(...) bytes, 16-byte aligned, no initialisation needed; one call at a time.
@@ -872,14 +872,13 @@ int dmt_attn_var_bwd(const dmt_attn_var_desc* d, void* stream);
  * ------------------------------------------------------------------------------------------------ */
 #define DMT_KV_BLOCK 64
 /* Block tables and slots from request lengths, on the device.  Request r has lens[r] tokens and gets new_lens[r] more, whose rows are
- * row_off[r] .. of the step's row matrices (row_off: exclusive sums of new_lens, [n + 1], cut at
- * 2^31 - 1).  Blocks come from the stack free_ids[0 .. n_free):
- * the last entry first, requests in order.  A request is refused (lens_out = lens, its slots -1) when new_lens < 0 (counted as 0 rows), when
- * lens + new would pass the table's width or its rows would pass `rows`, or when the requests up to and including it need more blocks than
- * are free.  Out: row_off, lens_out [n], table (the new blocks' entries), slots [rows] (-1: not stored), runs: run w = rows run_row[w] ..
- * + run_len[w] of one request in one block, in row order, then (-1, 0) up to max_runs = min(rows, rows / 64 + 2 n); free_cap: entries of
- * free_ids (n_free is cut there); state = {blocks left
- * free, requests refused}.  free_ids and n_free are read only: the caller keeps state[0] for its next step.
+ * row_off[r] .. of the step's row matrices (row_off: exclusive sums of new_lens, [n + 1], cut at 2^31 - 1).  Blocks come from the stack
+ * free_ids[0 .. n_free): the last entry first, requests in order.  A request is refused (lens_out = lens, its slots -1) when new_lens < 0
+ * (counted as 0 rows), when lens + new would pass the table's width or its rows would pass `rows`, or when the requests up to and
+ * including it need more blocks than are free.  Out: row_off, lens_out [n], table (the new blocks' entries), slots [rows] (-1: not stored),
+ * runs: run w = rows run_row[w] .. + run_len[w] of one request in one block, in row order, then (-1, 0) up to
+ * max_runs = min(rows, rows / 64 + 2 n); state = {blocks left free, requests refused}.  free_cap: entries of free_ids (n_free is cut
+ * there).  free_ids and n_free are read only: the caller keeps state[0] for its next step.  lens_out is not lens, state not n_free.
  * ws: dmt_kv_plan_ws_bytes(n) bytes, 16-byte aligned. */
 uint64_t dmt_kv_plan_ws_bytes(int32_t n);
 int dmt_kv_plan(int32_t n, int32_t rows, const int32_t* lens, const int32_t* new_lens, int32_t* table, int32_t width,
@@ -905,7 +904,7 @@ int dmt_kv_read(int32_t Hkv, int32_t dh, int32_t n_blocks, const uint8_t* k, con
  * slopes: |position - j|.  A row that sees nothing gets 0 and lse -inf.  max_len bounds the lengths (a promise that sizes the grid and the
  * split over the length; longer requests are cut there; lens past the table's width too).  Table entries outside the pool: masked.
  * One wavefront takes 64 tokens at a time; the length is split over workgroups by a rule on (n, Hkv, max_q, max_len) alone, and the pieces
- * are joined in their order: bit-reproducible.  ws: dmt_kv_attn_ws_bytes(d), 16-byte aligned, one call at a time. */
+ * are joined in their order: bit-reproducible.  out is not Q.  ws: dmt_kv_attn_ws_bytes(d), 16-byte aligned, one call at a time. */
 typedef struct {
   int32_t n, Hq, Hkv, dh, n_blocks;
   int32_t max_q, max_len, width;

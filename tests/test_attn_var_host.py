@@ -122,3 +122,29 @@ def test_kv_attn_refuses(kw, msg):
         for k, v in {**base, zero: 0}.items():
             setattr(d, k, v)
         assert lib.dmt_kv_attn(C.byref(d), None) == 0
+
+
+def test_outputs_in_place_of_inputs_are_refused():
+    lib = L.load()
+    for same in ("Q", "K", "V"):
+        d = _desc(Q=2048, K=4096, V=8192, out={"Q": 2048, "K": 4096, "V": 8192}[same])
+        assert lib.dmt_attn_var_fwd(C.byref(d), None) == -1 and b"operand" in lib.dmt_last_error()
+    assert lib.dmt_kv_plan(1, 4, 64, 68, 72, 4, 76, 4, 80, 84, 64, 88, 92, 96, 100, 128, 99, None) == -1 and b"lens_out" in lib.dmt_last_error()
+    assert lib.dmt_kv_plan(1, 4, 64, 68, 72, 4, 76, 4, 80, 84, 104, 88, 92, 96, 80, 128, 99, None) == -1 and b"state" in lib.dmt_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(max_q=2 ** 31 - 1, Hq=4), dict(n=65535, max_q=2 ** 24), dict(n=65535, Hq=65535, Hkv=65535)])
+def test_kv_attn_refuses_launches_that_do_not_fit(kw):
+    lib, d = L.load(), L.KvAttnDesc()
+    base = dict(n=1, Hq=2, Hkv=2, dh=32, n_blocks=8, max_q=1, max_len=2 ** 31 - 64, width=2 ** 24, rows=1, k=1024, v=1024, k_scale=64, v_scale=64, Q=1024,
+                q_rs=1 << 21, table=64, lens=64, row_off=64, scale=1.0, cap=0.0, causal=1, out=2048, o_rs=1 << 21, ws=1024, ws_bytes=1 << 62)
+    for k, v in {**base, **kw}.items():
+        setattr(d, k, v)
+    assert lib.dmt_kv_attn(C.byref(d), None) == -1 and b"2^31 workgroups" in lib.dmt_last_error()
+    assert lib.dmt_kv_attn_ws_bytes(C.byref(d)) == 0
+
+
+def test_release_needs_device_tensors():
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kv_cache.kv_release(i, i, i[:, None].contiguous(), i, i[:1])

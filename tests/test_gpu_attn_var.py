@@ -323,3 +323,57 @@ def test_slopes_without_queries_or_keys(cuda):
         assert (out == 0).all()
         for g, x in zip(torch.autograd.grad(out, lv, torch.ones_like(out)), lv):
             assert g.shape == x.shape and (g == 0).all()
+
+
+def test_gradients_of_gradients_and_changed_masks_are_refused(cuda):
+    q, k, v, do, _, _ = _make([9, 4], [9, 4], 2, 2, 32, F32, 3)
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+    seqs = ops.AttnSeqs([9, 4], device=cuda)
+    prefix = torch.tensor([2, 0], dtype=torch.int32, device=cuda)
+    out = ops.attn_var(*lv, seqs, 2, causal=True, prefix=prefix)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out, lv, do.to(cuda), create_graph=True)
+    out = ops.attn_var(*lv, seqs, 2, causal=True, prefix=prefix)
+    prefix[0] = 4
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, lv, do.to(cuda))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_padded_batch_is_a_packed_one(cuda, dtype):
+    """rows [B, T, d] with lengths: offsets b T, nothing copied; the padding of the results is zero and what stands in the operands' padding
+    (NaN here) reaches nothing.  Same kernels, same rows: bit-equal to the packed call"""
+    B, T, H, dh = 3, 70, 2, 32
+    ql = [70, 1, 33]
+    q, k, v, do, _, _ = (t.to(cuda) if isinstance(t, torch.Tensor) else t for t in _make(ql, ql, H, H, dh, dtype, 4))
+    at = torch.cat([b * T + torch.arange(n) for b, n in enumerate(ql)]).to(cuda)
+
+    def spread(t):
+        x = torch.full((B * T, H * dh), float("nan"), dtype=dtype, device=cuda)
+        x[at] = t
+        return x
+
+    packed = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = ops.attn_var(*packed, ops.AttnSeqs(ql, device=cuda), H, causal=True)
+    gw = torch.autograd.grad(want, packed, do)
+    dense = [spread(t).requires_grad_(True) for t in (q, k, v)]
+    got = ops.attn_var(*dense, ops.AttnSeqs(ql, q_off=[b * T for b in range(B)], device=cuda), H, causal=True)
+    gg = torch.autograd.grad(got, dense, spread(do))
+    pad = torch.ones(B * T, dtype=torch.bool, device=cuda)
+    pad[at] = False
+    for a, b in zip((want,) + gw, (got,) + gg):
+        assert torch.equal(a, b[at]) and (b[pad] == 0).all()
+
+
+def test_a_broadcast_gradient_and_parts_of_one_tensor(cuda):
+    """the gradient of a sum (a tensor without strides), and q, k, v as column slices of one projection"""
+    H, dh, ql = 2, 32, [40, 7]
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn((47, 3 * H * dh), generator=g).to(BF)
+    leaf = x.to(cuda).requires_grad_(True)
+    d = H * dh
+    out = ops.attn_var(leaf[:, :d], leaf[:, d:2 * d], leaf[:, 2 * d:], ops.AttnSeqs(ql, device=cuda), H, causal=True)
+    out.sum().backward()
+    ref = A.attn_var(x[:, :d], x[:, d:2 * d], x[:, 2 * d:], H, H, ql, ql, [0, 40], [0, 40], causal=True, dout=torch.ones((47, d), dtype=BF))
+    for n, c in (("dq", 0), ("dk", 1), ("dv", 2)):
+        A.close(leaf.grad[:, c * d:(c + 1) * d], ref[n], ref[n + "_tol"], n)

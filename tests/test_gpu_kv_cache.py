@@ -430,3 +430,79 @@ def test_another_stream(cuda):
         b = KV.kv_attn(cache, q, *args)
     side.synchronize()
     assert torch.equal(a, b)
+
+
+def test_two_graphs_two_streams_and_one_history_twice(cuda):
+    """split lengths: two captured calls and an eager one on a side stream do not share a workspace; two requests that name the same blocks
+    get the same rows"""
+    lens, H = [9000, 9000, 64], 4
+    cache, table, _ = _cache_of(cuda, lens, 2, 32, 8)
+    table[1] = table[0]
+    g = torch.Generator().manual_seed(3)
+    one = torch.randn((2, H * 32), generator=g).to(BF)
+    q1 = torch.cat([one, one, one]).to(cuda)
+    q2 = torch.randn((6, H * 32), generator=g).to(BF).to(cuda)
+    args = (table, _i(lens, cuda), _i([0, 2, 4, 6], cuda), H, 2)
+    w1, w2 = KV.kv_attn(cache, q1, *args), KV.kv_attn(cache, q2, *args)
+    assert torch.equal(w1[:2], w1[2:4])
+    torch.cuda.synchronize()
+    graphs = []
+    for q in (q1, q2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, KV.kv_attn(cache, q, *args)))
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        for _g, o in graphs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            e = KV.kv_attn(cache, q2, *args)
+            graphs[1][0].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(graphs[0][1], w1) and torch.equal(graphs[1][1], w2) and torch.equal(e, w2)
+
+
+def test_rows_of_a_refused_request(cuda):
+    """nothing is stored for them, the others are served, and their attention reads only what they held"""
+    cache = KV.KVCache.empty(2, 1, 32, cuda)
+    lens, table = _i([0, 0], cuda), torch.full((2, 2), -1, dtype=torch.int32, device=cuda)
+    free, n_free = _i([0, 1], cuda), _i([2], cuda)
+    x = torch.randn((100, 32), generator=torch.Generator().manual_seed(1)).to(BF).to(cuda)
+    plan = KV.kv_plan(lens, _i([30, 70], cuda), table, free, n_free, 100)        # one block for the first, two wanted by the second, one left
+    assert plan.refused.tolist() == [1] and plan.lens.tolist() == [30, 0] and plan.n_free.tolist() == [1] and (plan.slots[30:] == -1).all()
+    KV.kv_append(cache, x, x, plan)
+    out, lse = KV.kv_attn(cache, x, table, plan.lens, plan.row_off, 1, 70, want_lse=True)
+    assert (out[30:] == 0).all() and (lse[30:] == -np.inf).all() and (out[:30] != 0).any(-1).all()
+
+
+def test_refusals_of_device_arguments(cuda):
+    cache, table, _ = _cache_of(cuda, [70], 2, 32, 8)
+    q = torch.zeros((3, 128), dtype=BF, device=cuda)
+    lens, off = _i([70], cuda), _i([0, 3], cuda)
+    ok = dict(q=q, table=table, lens=lens, row_off=off, H=4, max_q=3)
+    for kw, msg in ((dict(H=3), "share"), (dict(q=q.float()), "bf16"), (dict(q=q[:, :64]), "bf16 rows"), (dict(table=table[0]), "table"),
+                    (dict(lens=lens.long()), "lens"), (dict(row_off=lens), "row_off"), (dict(max_q=-1), "negative"), (dict(scale=0.0), "scale"),
+                    (dict(cap=float("nan")), "scale"), (dict(out=q), "not be q"), (dict(out=q[:2].clone()), "out must be"),
+                    (dict(slopes=torch.zeros(3, device=cuda)), "slopes"), (dict(max_len=-1), "negative"), (dict(table=table.cpu()), "table")):
+        with pytest.raises(ValueError, match=msg):
+            KV.kv_attn(cache, **{**ok, **kw})
+    one = KV.kv_attn(cache, **ok)
+    assert torch.equal(one, KV.kv_attn(cache, **{**ok, "max_q": 2 ** 40, "max_len": 2 ** 40}))   # bounds that say nothing
+    n, i = _i([1], cuda), _i([3], cuda)
+    for a in ((lens, i, table[0], n, n, 3), (lens[None], i, table, n, n, 3), (lens, i, table, n, n, -1), (lens, i, table, n, n.cpu(), 3)):
+        with pytest.raises(ValueError):
+            KV.kv_plan(*a)
+    plan = KV.kv_plan(lens, i, table, n, n, 3)
+    x = torch.zeros((3, 64), dtype=BF, device=cuda)
+    for k, v in ((x[:2], x), (x, x[:, :32]), (x.float(), x), (x.cpu(), x)):
+        with pytest.raises(ValueError):
+            KV.kv_append(cache, k, v, plan)
+    with pytest.raises(ValueError):
+        KV.kv_read(cache, plan.slots.long())
+    c = cache
+    for a in ((c.k[:, :1], c.v, c.k_scale, c.v_scale), (c.k, c.v, c.k_scale[:1], c.v_scale), (c.k.view(torch.uint8), c.v, c.k_scale, c.v_scale),
+              (c.k, c.v, c.k_scale.double(), c.v_scale), (c.k.cpu(), c.v.cpu(), c.k_scale.cpu(), c.v_scale.cpu())):
+        with pytest.raises(ValueError):
+            KV.KVCache(*a)
