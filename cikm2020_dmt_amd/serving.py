@@ -65,9 +65,15 @@ class HistoryCache:
         self.lens, self.n_free = plan.lens, plan.n_free
         return plan
 
-    def attend(self, layer, q, row_off, num_heads, max_q, **kw):
-        """kv_attn of one layer: user r's query rows are row_off[r] .. row_off[r + 1] of q"""
-        return kv_attn(self.layers[layer], q, self.table, self.lens, row_off, num_heads, max_q, **kw)
+    def of(self, places):
+        """(table, lens) of the users in `places` (index tensor), in that order: what attend takes for a step that concerns these alone"""
+        return self.table.index_select(0, places), self.lens.index_select(0, places)
+
+    def attend(self, layer, q, row_off, num_heads, max_q, held=None, **kw):
+        """kv_attn of one layer: query rows row_off[r] .. row_off[r + 1] of q belong to user r, or to the r-th of held = of(places) (at most
+        65535 users a call)"""
+        table, lens = (self.table, self.lens) if held is None else held
+        return kv_attn(self.layers[layer], q, table, lens, row_off, num_heads, max_q, **kw)
 
     def drop(self, done):
         """done: int32 [n_users], non-zero: forget that user"""
@@ -223,18 +229,20 @@ class CandidateScorer:
         """(click_logit, order_logit) [B, 1] for candidate rows of remembered users: users[r] is the place of row r's user, in ascending
         order (rows of one user side by side).  The sequence columns of `batch` are not read by the attention."""
         eng, spec = self.engine, self.spec
-        users, n = self._places(users, batch.B)
+        users, _n = self._places(users, batch.B)
         if (np.diff(users) < 0).any():
             raise ValueError("the places must stand in ascending order")
         self._fresh_tables()
-        count = np.bincount(users, minlength=n)
+        asked, count = np.unique(users, return_counts=True)
         row_off = torch.as_tensor(np.concatenate([[0], np.cumsum(count)]).astype(np.int32)).to(eng.store.device)
+        asked = torch.as_tensor(asked).to(eng.store.device)
         saved_seed, eng.dropout_step_seed = eng.dropout_step_seed, None
         try:
             tar, zbuf = eng.gather_pooled(batch)
             us = []
             for i, h in enumerate(self.histories):
-                attend = lambda j, q, h=h: h.attend(j, q, row_off, spec["num_heads"], int(count.max()), causal=False)  # noqa: E731
+                held = h.of(asked)
+                attend = lambda j, q, h=h, held=held: h.attend(j, q, row_off, spec["num_heads"], int(count.max()), held, causal=False)  # noqa: E731
                 us.append(eng.decode_cached(eng.decoder_query(tar), i, attend))
             z = AssembleFn.apply(zbuf, eng.plan.interest_off, spec["d_model"], *eng.interest_blocks(us, [tar] * len(us)))
             tasks = eng.expert_gate(z, z_is_engine_buffer=True)

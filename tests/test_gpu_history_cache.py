@@ -16,6 +16,11 @@ pytestmark = pytest.mark.gpu
 ROWS = {"Sku": 3000, "Brand": 800, "Shopid": 900, "Cid3": 300, "Cid2": 50}
 
 
+def _slots(table_row, n):
+    pos = torch.arange(n, device=table_row.device)
+    return (table_row[pos // 64] * 64 + pos % 64).to(torch.int32)
+
+
 def _trainer(cuda, dtype=torch.bfloat16, **opt):
     sp = dict(S.scaled_spec(S.e64_spec(), ROWS), **opt)
     return sp, Trainer(sp, device=cuda, compute_dtype=dtype, init=True, dropout=False)
@@ -125,3 +130,31 @@ def test_no_room_and_refusals(cuda):
     x = torch.zeros((1, 64), dtype=torch.bfloat16, device=cuda)
     with pytest.raises(ValueError, match="2 layers"):
         h.append([(x, x)], torch.tensor([1, 0], dtype=torch.int32, device=cuda))
+
+
+def test_a_cache_of_many_users(cuda):
+    """attend for every place and for a few named ones (more places than one attention call takes): the same rows"""
+    n, H, dh = 70000, 2, 32
+    h = HistoryCache(n, 64, 100, H, dh, device=cuda)
+    g = torch.Generator().manual_seed(4)
+    new = torch.zeros(n, dtype=torch.int32)
+    places = [3, 1500, 69999]
+    new[places] = torch.tensor([100, 64, 1], dtype=torch.int32)
+    k, v = (torch.randn((165, H * dh), generator=g).to(torch.bfloat16).to(cuda) for _ in range(2))
+    assert int(h.append([(k, v)], new.to(cuda)).refused) == 0
+    at = torch.tensor(places, device=cuda)
+    table, lens = h.of(at)
+    assert lens.tolist() == [100, 64, 1] and (table[:, 0] >= 0).all() and h.max_len == 128
+    q = torch.randn((3, H * dh), generator=g).to(torch.bfloat16).to(cuda)
+    off = torch.arange(4, dtype=torch.int32, device=cuda)
+    got = h.attend(0, q, off, H, 1, (table, lens), causal=False)
+    for r, (a, b) in enumerate(((0, 100), (100, 164), (164, 165))):
+        kk, vv = (x.float().reshape(-1, H, dh).transpose(0, 1) for x in KV.kv_read(h.layers[0], _slots(table[r], b - a)))
+        p = torch.softmax((q[r].float().reshape(H, 1, dh) * kk).sum(-1) * dh ** -0.5, -1)
+        want = (p[..., None] * vv).sum(1).reshape(-1)
+        # weights and result are rounded once each: half a step of values of at most max |v|, twice
+        assert (got[r].float() - want).abs().max() <= 2 * 2.0 ** -8 * float(vv.abs().max())
+    with pytest.raises(Exception, match="65535"):
+        h.attend(0, q, torch.zeros(n + 1, dtype=torch.int32, device=cuda), H, 1)
+    h.drop((torch.arange(n) == 1500).to(torch.int32).to(cuda))
+    assert h.of(at)[1].tolist() == [100, 0, 1] and int(h.n_free) == 64 - 4 + 1
