@@ -342,6 +342,7 @@ __device__ __forceinline__ float other_half(float x) {
 __device__ __forceinline__ void settle(f32x16_t& a) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a)); }
 __device__ __forceinline__ void settle(f32x16_t& a, f32x16_t& b) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(a), "+v"(b)); }
 
+typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
 template <typename T, int DHP> struct Tile;
 template <int DHP> struct Tile<bf16_t, DHP> {
   typedef bf16x8_t Frag;
@@ -367,14 +368,17 @@ template <int DHP> struct Tile<bf16_t, DHP> {
   static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w
-  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int row0, const f32x16_t& w, int lane) {
+  // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w; sum += the lane's w as they were rounded
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int row0, const f32x16_t& w, int lane, float* sum = nullptr) {
     const int half = lane >> 5, i16 = lane & 15, grp = (lane >> 4) & 1, r = 4 * half + (i16 >> 2);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       union { bf16x8_t v; unsigned d[4]; } b;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b.d[i] = dmt_pack_bf16(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+      for (int i = 0; i < 4; ++i) {
+        b.d[i] = dmt_pack_bf16(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+        if (sum) *sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, b.d[i]), __builtin_bit_cast(bf2_t, 0x3f803f80u), *sum, false);
+      }
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
         const bf16_t* x = X + (row0 + 16 * u) * RS + at(r, 4 * dt + 2 * grp + ((i16 >> 1) & 1)) + 4 * (i16 & 1);
@@ -407,7 +411,7 @@ template <int DHP> struct Tile<float, DHP> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
-  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int row0, const f32x16_t& w, int lane) {
+  static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int row0, const f32x16_t& w, int lane, float* = nullptr) {
     const float* x = X + (row0 + 4 * (lane >> 5)) * RS + (lane & 31);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {

@@ -10,8 +10,8 @@ namespace {
 // and the next in registers.  S^T = K Q^T and O^T = V^T P^T: a lane owns a query, its statistics stay in the lane, and P packed is an operand.
 // One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
 // are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
-// What bounds it: the matrix pipe and, beside it, one power and about 4 other vector operations a score (2 x 4096 causal, 16 heads of 128: 162 us =
-// 846 TFLOP/s of the products that the mask leaves); for short histories the rows (256 of up to 200, 4 heads of 80: 38 us, 57 MB).
+// What bounds it: the matrix pipe and, beside it, one power and about 4 other vector operations a score (2 x 4096 causal, 16 heads of 128: 171 us =
+// 802 TFLOP/s of the products that the mask leaves); for short histories the rows (256 of up to 200, 4 heads of 80: 38 us, 57 MB).
 template <typename T, int DHP, int SHAPE, bool DOCS, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
@@ -74,7 +74,10 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
-  float m = -INFINITY, l = 0.f;
+  // l: the sum of the weights, for lse; lr: of the weights as the product with V has them.  The output is divided by lr: a row of few keys then keeps
+  // what the rounding of its large weight does out of rowsum(dout out), which the backward subtracts from nearly the same number (error of dQ
+  // and dK: 0.0025 of their norm instead of 0.0028 in capped sessions; 164 -> 171 us at 2 x 4096 causal, 16 heads of 128)
+  float m = -INFINITY, l = 0.f, lr = 0.f;
   if (t < nk) end(0);
   __syncthreads();
   while (t < nk) {
@@ -156,6 +159,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
         const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.f : exp2_hw(m - mn);
         m = mn;
         l *= f;
+        lr *= f;
 #pragma unroll
         for (int dt = 0; dt < TL::NDT; ++dt)
 #pragma unroll
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
           s[u][r] = exp2_hw(SHAPE ? s[u][r] - mu : __builtin_fmaf(s[u][r], c, -mu));
           l += s[u][r];
         }
-        TL::accumulate(o, Vl, 32 * u, s[u], lane);
+        TL::accumulate(o, Vl, 32 * u, s[u], lane, sizeof(T) == 2 ? &lr : nullptr);
       }
     }
     if (NB == 1) __syncthreads();
@@ -183,8 +187,9 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) settle(o[dt]);
   l += other_half(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  float bad = l * 0.f;
+  lr = sizeof(T) == 2 ? lr + other_half(lr) : l;
+  const float inv = lr == 0.f ? 0.f : 1.f / lr;
+  float bad = (l + lr) * 0.f;
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(o[dt], dt, half, a.dh);
   const long long row = e.q0 + i;
