@@ -422,7 +422,7 @@ template <int DHP> struct Tile<float, DHP> {
   }
 };
 
-// A buffer descriptor over `rows` rows of one head: what lies past the last row or past dim dh reads as zero, so that neither a ragged end
+// A buffer descriptor over `rows` rows (at most 64) of one head: what lies past the last row or past dim dh reads as zero, so that neither a ragged end
 // nor a padded head size needs a branch, and nothing outside the example is touched.
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 template <typename T> __device__ __forceinline__ rsrc_t rows_rsrc(const T* base, long long rs, int rows, int dh) {
@@ -432,11 +432,12 @@ template <typename T> __device__ __forceinline__ rsrc_t rows_rsrc(const T* base,
 constexpr int OUTSIDE = 0x7ffffff0;
 __device__ __forceinline__ u32x4_t load16(rsrc_t r, int off) { return __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); }
 
-// one lane's fragments of its own row (the B operands that stay in registers)
+// One lane's fragments of its own row (the B operands that stay in registers): row row0 + l31 of the example that starts at `base`.  The descriptor
+// starts at the wavefront's first row: its 32 rows of under 16 MB stay below 2^29 bytes, whatever the example's length times its stride.
 template <typename T, int DHP>
-__device__ __forceinline__ void own_row(typename Tile<T, DHP>::Frag* f, const T* base, long long rs, int rows, int dh, int row, int half) {
-  const rsrc_t r = rows_rsrc<T>(base, rs, rows, dh);
-  const int at = row * (int)(rs * (int)sizeof(T));
+__device__ __forceinline__ void own_row(typename Tile<T, DHP>::Frag* f, const T* base, long long rs, int rows, int dh, int row0, int l31, int half) {
+  const rsrc_t r = rows_rsrc<T>(base + row0 * rs, rs, min(rows - row0, 32), dh);
+  const int at = l31 * (int)(rs * (int)sizeof(T));
 #pragma unroll
   for (int s = 0; s < Tile<T, DHP>::NS; ++s) {
     const int c = Tile<T, DHP>::col(s, half);

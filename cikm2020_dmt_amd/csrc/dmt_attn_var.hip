@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
   int flags = 0, buf = 0, t = wk.next(0, flags);
   if (t < nk) begin(t, 0);                                 // (its latency and that of the row's own loads pass together)
   typename TL::Frag q[TL::NS];
-  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, iw, l31, half);
   f32x16_t o[TL::NDT];
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) o[dt] = zero16();
@@ -329,7 +329,8 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   DMT_CHECK_ARG(d->rows_q == 0 || (d->Q && d->out), "%s: NULL Q / out", what);
   DMT_CHECK_ARG(d->rows_k == 0 || (d->K && d->V), "%s: NULL K / V", what);
   DMT_CHECK_ARG(d->q_rs >= wq && d->k_rs >= wk && d->v_rs >= wk && (d->rows_q == 0 || d->o_rs >= wq), "%s: row stride shorter than a row", what);
-  DMT_CHECK_ARG(d->k_rs * es < (1ll << 24) && d->v_rs * es < (1ll << 24) && d->q_rs * es < (1ll << 24), "%s: row stride of 16 MB or more", what);
+  DMT_CHECK_ARG(d->k_rs * es < (1ll << 24) && d->v_rs * es < (1ll << 24) && d->q_rs * es < (1ll << 24) && d->o_rs * es < (1ll << 24),
+                "%s: row stride of 16 MB or more", what);
   DMT_CHECK_ARG(al16(d->Q, d->q_rs, es) && al16(d->K, d->k_rs, es) && al16(d->V, d->v_rs, es) && al16(d->out, d->o_rs, es),
                 "%s: operand rows must be 16-byte aligned", what);
   if (backward) {

@@ -89,20 +89,20 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
   int flags = 0, buf = 0, t = wk.next(0, flags);
   if (t < nk) begin(t, 0);                               // (its latency and that of the rows' own loads pass together)
   typename TL::Frag q[TL::NS], g[TL::NS];
-  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, i, half);
-  own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, i, half);
+  own_row<T, DHP>(q, (const T*)a.Q + e.q0 * a.q_rs + (long long)h * a.dh, a.q_rs, e.ql, a.dh, iw, l31, half);
+  own_row<T, DHP>(g, (const T*)a.dout + e.q0 * a.do_rs + (long long)h * a.dh, a.do_rs, e.ql, a.dh, iw, l31, half);
   const long long stat = (e.q0 + (in ? i : 0)) * a.Hq + h;
   // (a row that sees nothing: lse = -inf; its weights 2^(z - inf) are 0)
   const float lse = a.lse[stat], lse2 = in && lse != -INFINITY ? lse * LOG2E : INFINITY;
   float D = 0.f;                                         // rowsum(dout * out), for this kernel and the next
   {
     typename TL::Frag ov[TL::NS];
-    own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, i, half);
+    own_row<T, DHP>(ov, (const T*)a.out + e.q0 * a.o_rs + (long long)h * a.dh, a.o_rs, e.ql, a.dh, iw, l31, half);
 #pragma unroll
     for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
     if (sizeof(T) == 2 && a.out_lo) {
       const long long ls = (long long)a.Hq * a.dh;
-      own_row<T, DHP>(ov, (const T*)a.out_lo + e.q0 * ls + (long long)h * a.dh, ls, e.ql, a.dh, i, half);
+      own_row<T, DHP>(ov, (const T*)a.out_lo + e.q0 * ls + (long long)h * a.dh, ls, e.ql, a.dh, iw, l31, half);
 #pragma unroll
       for (int x = 0; x < TL::NS; ++x) D = TL::dot(g[x], ov[x], D);
     }
@@ -320,8 +320,8 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   const int first = t, first_flags = flags;
   if (g < ng) begin(0, t, 0);
   typename TL::Frag k[TL::NS], v[TL::NS];
-  own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, j, half);
-  if (WHAT & 1) own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, j, half);
+  own_row<T, DHP>(k, (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh, a.k_rs, e.kl, a.dh, jw, l31, half);
+  if (WHAT & 1) own_row<T, DHP>(v, (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh, a.v_rs, e.kl, a.dh, jw, l31, half);
   if (g < ng) end(0);
   __syncthreads();
   while (g < ng) {

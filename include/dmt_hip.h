@@ -821,7 +821,7 @@ int dmt_q1mem_bwd(const dmt_q1mem_desc* d, void* stream);
  * A row that may see nothing gets out = 0, lse = -inf and no gradient.  What stands in a masked place -- NaN and infinities too -- does
  * not reach a row that may not see it.  Rows that belong to no example are neither read nor written.
  * Types: DMT_BF16 (dh a multiple of 8) and DMT_F32 (dh a multiple of 4), dh <= 128; sums, softmax statistics and gradients in fp32.
- * Every operand row 16-byte aligned (base and row stride); out is none of them.  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
+ * Every operand row 16-byte aligned (base and row stride), row strides under 16 MB; out is none of them.  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
  * caller's promise: it sizes the grid; longer examples are cut there).
  * Backward: dq, dk, dv for the rows of every example, and dslopes [Hq] (summed in a fixed order).
  * Bit-reproducible: no atomics.  ws: dmt_attn_var_ws_bytes(...) bytes, 16-byte aligned, no initialisation needed; one call at a time.

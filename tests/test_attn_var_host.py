@@ -148,3 +148,10 @@ def test_release_needs_device_tensors():
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no CPU path"):
         kv_cache.kv_release(i, i, i[:, None].contiguous(), i, i[:1])
+
+
+@pytest.mark.parametrize("rs", ["q_rs", "k_rs", "v_rs", "o_rs", "do_rs"])
+def test_row_strides_that_32_rows_cannot_hold_are_refused(rs):
+    """rows are addressed by 32-bit offsets from the first row of a wavefront (or of a 64-row tile): 2^24 bytes a row at most, o_rs included"""
+    lib, d = L.load(), _desc(**{rs: 1 << 23})
+    assert lib.dmt_attn_var_bwd(C.byref(d), None) == -1 and b"stride" in lib.dmt_last_error()

@@ -377,3 +377,49 @@ def test_a_broadcast_gradient_and_parts_of_one_tensor(cuda):
     ref = A.attn_var(x[:, :d], x[:, d:2 * d], x[:, 2 * d:], H, H, ql, ql, [0, 40], [0, 40], causal=True, dout=torch.ones((47, d), dtype=BF))
     for n, c in (("dq", 0), ("dk", 1), ("dv", 2)):
         A.close(leaf.grad[:, c * d:(c + 1) * d], ref[n], ref[n + "_tol"], n)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_of_one_example_past_4_gib(cuda, dtype):
+    """300 rows of q, k, v and dout as columns of one matrix whose rows take nearly 16 MB: the example reaches past 2 and 4 GiB.  The head size is no
+    tile size, and what stands beside the columns (ones) belongs to no operand."""
+    L_, dh, es = 300, 96, torch.finfo(dtype).bits // 8
+    buf = torch.ones((L_, ((1 << 24) - 16) // es), dtype=dtype, device=cuda)
+    q, k, v, do, _, _ = _make([L_], [L_], 1, 1, dh, dtype, 11)
+    cols = []
+    for n, t in enumerate((q, k, v, do)):
+        buf[:, n * dh:n * dh + dh] = t.to(cuda)
+        cols.append(buf[:, n * dh:n * dh + dh])
+    ref = A.attn_var(q, k, v, 1, 1, [L_], [L_], [0], [0], causal=True, dout=do)
+    lv = [c.detach().requires_grad_(True) for c in cols[:3]]
+    out, lse = ops.attn_var(*lv, ops.AttnSeqs([L_], device=cuda), 1, causal=True, want_lse=True)
+    grads = torch.autograd.grad(out, lv, cols[3])
+    for t, n in zip((out, lse) + grads, ("out", "lse", "dq", "dk", "dv")):
+        A.close(t, ref[n], ref[n + "_tol"], n)
+
+
+def test_contiguous_rows_of_one_example_past_4_gib(cuda):
+    """360000 query rows of 64 heads of 96 (12 KB each) over 64 keys: q, out, dout and dq pass 4 GiB"""
+    g = torch.Generator(device=cuda).manual_seed(5)
+    n, kl, H, Hkv, dh = 360000, 64, 64, 2, 96
+    q, do = (torch.empty((n, H * dh), dtype=BF, device=cuda).normal_(generator=g) for _ in range(2))
+    k, v = (torch.empty((kl, Hkv * dh), dtype=BF, device=cuda).normal_(generator=g) for _ in range(2))
+    lv = [t.requires_grad_(True) for t in (q, k, v)]
+    out = ops.attn_var(*lv, ops.AttnSeqs([n], [kl], device=cuda), H, Hkv)
+    dq, dk, dv = torch.autograd.grad(out, lv, do)
+    two, four = 2 ** 31 // (H * dh * 2), 2 ** 32 // (H * dh * 2)
+    rows = torch.cat([torch.arange(a, b) for a, b in ((0, 130), (two - 70, two + 70), (four - 70, four + 70), (n - 130, n))]).to(cuda)
+    ok = torch.ones((n, kl), dtype=torch.bool, device=cuda)
+    dist = torch.zeros((1, 1), dtype=torch.int64, device=cuda)
+    u = torch.finfo(BF).eps / 2
+    sums = {x: torch.zeros((kl, Hkv * dh), dtype=torch.float64, device=cuda) for x in ("dk", "dv", "dk_tol", "dv_tol")}
+    with torch.no_grad():
+        for h in range(H):
+            c, ck = slice(h * dh, h * dh + dh), slice(h // 32 * dh, h // 32 * dh + dh)
+            r = A.head(q[:, c], k[:, ck], v[:, ck], ok, dist, dh ** -0.5, 0.0, None, BF, do[:, c])
+            for t, x in ((out, "out"), (dq, "dq")):
+                A.close(t[rows, c], r[x][rows].cpu(), r[x + "_tol"][rows].cpu(), "%s of head %d" % (x, h))
+            for x in sums:
+                sums[x][:, ck] += r[x]
+        for t, x in ((dk, "dk"), (dv, "dv")):
+            A.close(t, sums[x].cpu(), (sums[x + "_tol"] + u * sums[x].abs() + 1e-30).cpu(), x)
