@@ -190,9 +190,11 @@ class CandidateScorer:
 
     @torch.no_grad()
     def remember(self, users, batch: DeviceBatch):
-        """Encode row r of `batch` as the history of place users[r] (distinct places; what stood there is replaced).  Returns the number of
-        (user, sequence) histories that found no room: those are empty then, and attention over an empty history gives zeros.  A history
-        is as old as the weights that encoded it: after training steps, remember it again."""
+        """Encode row r of `batch` as the history of place users[r] (distinct places; what stood there is replaced).  A sequence without events
+        is kept as one row, the mean of its T padded rows (T: the column's width in this batch): the model's attention gives those the
+        same weight, in training and in logits().
+        Returns the number of (user, sequence) histories that found no room: nothing is kept of them, and the attention over them gives
+        zeros.  A history is as old as the weights that encoded it: after training steps, remember it again."""
         eng, spec = self.engine, self.spec
         users, n = self._places(users, batch.B)
         if len(np.unique(users)) != len(users):
@@ -210,13 +212,18 @@ class CandidateScorer:
             refused = 0
             for i, h in enumerate(self.histories):
                 lens, T = eng.seq_lens(dense, i), X[i].shape[1]
+                held = lens.cpu().numpy()
+                empty = torch.as_tensor(np.flatnonzero(held <= 0)).to(dev)
                 new = np.zeros(n, dtype=np.int32)
-                new[users] = np.minimum(lens.cpu().numpy(), T)
+                new[users] = np.clip(held, 1, T)
                 at = torch.as_tensor(np.concatenate([r * T + np.arange(new[users[r]]) for r in order])).to(dev)
                 mem = eng.encode_prepared(X[i], lens, i)
                 rows = []
                 for j in range(len(h.layers)):
-                    kv = eng.memory_kv(mem, i, j).reshape(-1, 2 * d)[at]
+                    kv = eng.memory_kv(mem, i, j)
+                    if len(empty):
+                        kv[empty, 0] = kv[empty].float().mean(1).to(kv.dtype)
+                    kv = kv.reshape(-1, 2 * d)[at]
                     rows.append((kv[:, :d], kv[:, d:]))
                 h.drop(torch.as_tensor(done).to(dev))
                 refused += int(h.append(rows, torch.as_tensor(new).to(dev)).refused)

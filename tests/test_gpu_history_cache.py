@@ -8,7 +8,7 @@ from cikm2020_dmt_amd import kv_cache as KV
 from cikm2020_dmt_amd import ops
 from cikm2020_dmt_amd import spec as S
 from cikm2020_dmt_amd.data_feed.synthetic import make_batch
-from cikm2020_dmt_amd.engine import AssembleFn, trans_prefix
+from cikm2020_dmt_amd.engine import AssembleFn, DeviceBatch, FeatureColumn, trans_prefix
 from cikm2020_dmt_amd.serving import CandidateScorer, HistoryCache
 from cikm2020_dmt_amd.train import Trainer
 
@@ -158,3 +158,74 @@ def test_a_cache_of_many_users(cuda):
         h.attend(0, q, torch.zeros(n + 1, dtype=torch.int32, device=cuda), H, 1)
     h.drop((torch.arange(n) == 1500).to(torch.int32).to(cuda))
     assert h.of(at)[1].tolist() == [100, 0, 1] and int(h.n_free) == 64 - 4 + 1
+
+
+def _emptied(batch, sp, rows):
+    """the batch with empty histories: rows[i] have no event in sequence i"""
+    for i, pairs in enumerate(sp["attention_embed_pairs"]):
+        for uf, _item in pairs:
+            c = batch.feats[uf]
+            c.lens[torch.as_tensor(rows[i], dtype=torch.long, device=c.lens.device)] = 0
+            c.lens_host[rows[i]] = 0
+    return batch
+
+
+def _row(batch, r, n):
+    """row r of the batch n times over"""
+    at = torch.full((n,), r, device=batch.dense.device)
+    return DeviceBatch(n, {f: FeatureColumn(c.idx[at], c.wts[at] if c.wts is not None else None, c.lens[at], c.T) for f, c in batch.feats.items()},
+                       batch.dense[at])
+
+
+def test_an_empty_sequence_is_the_mean_of_its_padded_rows(cuda):
+    """A user without events in a sequence: the model's attention gives every padded row the same weight, so what is kept is one row, the mean of
+    K and of V over them, within the roundings (fp32 mean of bf16 rows to bf16: 2^-8 of the value; half a step of e4m3: 2^-4 of it, 2^-10 of the
+    scale below the normal range)"""
+    sp, tr = _trainer(cuda, num_blocks_decode=2)
+    eng, d = tr.engine, sp["d_model"]
+    sc = CandidateScorer(eng)
+    sc.keep_histories(5, 12)
+    batch = _emptied(_one_user_rows(sp, tr, 5, 4), sp, {0: [1], 1: [0, 1, 3], 2: [0, 1, 2, 3]})
+    users = [4, 0, 1, 2]
+    assert sc.remember(users, batch) == 0
+    eng.packed_rows = False
+    with torch.no_grad():
+        X, _t, _z = eng.gather(batch)
+        for i, pairs in enumerate(sp["attention_embed_pairs"]):
+            lens = batch.feats[pairs[-1][0]].lens
+            mem, h = eng.encode_prepared(X[i], lens, i), sc.histories[i]
+            assert [int(h.lens[u]) for u in users] == [max(int(x), 1) for x in lens]
+            for j, cache in enumerate(h.layers):
+                mean = eng.memory_kv(mem, i, j).double().mean(1)
+                for r, u in enumerate(users):
+                    if int(lens[r]):
+                        continue
+                    slot = (h.table[u][:1] * 64).to(torch.int32)
+                    k, v = KV.kv_read(cache, slot)
+                    for got, want, scale in ((k, mean[r, :d], cache.k_scale), (v, mean[r, d:], cache.v_scale)):
+                        step = scale[int(slot) // 64].repeat_interleave(d // sp["num_heads"])
+                        assert ((got[0].double() - want).abs() <= (2.0 ** -4 + 2.0 ** -7) * want.abs() + 2.0 ** -10 * step).all()
+
+
+@pytest.mark.parametrize("opt", [dict(), dict(num_blocks_decode=2)])
+def test_logits_of_users_with_empty_sequences(cuda, opt):
+    """logits_of against logits, the request path that re-encodes the user: lengths of 0 in some sequences, in all, in none.  V is made the same
+    for every row (its kernel 0, its bias of values that 8 bits hold), so that the cache rounds nothing that counts and every non-empty or
+    empty attention gives that row: the tolerance is the bf16 one of the request path."""
+    sp, tr = _trainer(cuda, **opt)
+    state, rng = {}, np.random.default_rng(3)
+    for name, arr in tr.store.dense_state_dict().items():
+        if "vanilla_attention/dense_2/kernel" in name:
+            state[name] = np.zeros_like(arr)
+        elif "vanilla_attention/dense_2/bias" in name:
+            state[name] = rng.integers(-14, 15, arr.shape) / 8.0                 # (14 / 8 = 1.75: four significant bits at most)
+    tr.store.load_state(state)
+    sc = CandidateScorer(tr.engine)
+    sc.keep_histories(6, 24)
+    hist = _emptied(_one_user_rows(sp, tr, 6, 5), sp, {0: [0, 2], 1: [2, 3], 2: [2, 4]})
+    places = [0, 1, 3, 4, 5]
+    assert sc.remember(places, hist) == 0
+    for r, place in enumerate(places):
+        batch = _row(hist, r, 3)
+        for g, w in zip(sc.logits_of([place] * 3, batch), sc.logits(batch)):
+            assert torch.allclose(g.float(), w.float(), atol=4e-2, rtol=4e-2), (r, g.flatten().tolist(), w.flatten().tolist())
