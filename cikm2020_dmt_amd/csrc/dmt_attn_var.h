@@ -1,7 +1,6 @@
 // What the kernels of dmt_attn_var.hip (forward) and dmt_attn_var_bwd.hip share: the arguments, the scores and masks, and the row kernels.
 //
-// Scores are kept in log2 units (z2 = z log2 e), so that a weight is one v_exp_f32: p = 2^(z2 - m2).  tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e)):
-// exact at both ends (the power runs to infinity or zero), absolute error ~2^-23, which is what a score of magnitude `cap` has anyway.
+// Scores are kept in log2 units (z2 = z log2 e), so that a weight is one v_exp_f32: p = 2^(z2 - m2).
 #pragma once
 #include "dmt_common.h"
 
@@ -73,30 +72,19 @@ __device__ __forceinline__ Ex example(const Args& a, int b) {
   return e;
 }
 
-// constants of one head's scores: z2 = shaped ? ... : c1 s
+// constants of one head's scores: z2 = (capped ? cap(s) : cap.c1 s) - sl2 |distance|
 struct Shape {
-  float c1;        // scale log2e
-  float cap2;      // cap log2e
-  float ck;        // 2 log2e scale / cap
+  dmt_cap cap;
   float sl2;       // slope log2e
-  bool cap, slope;
+  bool capped, slope;
 };
-__device__ __forceinline__ Shape shape_of(const Args& a, int h) {
-  Shape s;
-  s.c1 = a.scale * LOG2E;
-  s.cap = a.cap > 0.f;
-  s.cap2 = a.cap * LOG2E;
-  s.ck = s.cap ? 2.f * LOG2E * a.scale / a.cap : 0.f;
-  s.slope = a.slopes != nullptr;
-  s.sl2 = s.slope ? a.slopes[h] * LOG2E : 0.f;
-  return s;
+template <typename T> __device__ __forceinline__ Shape shape_of(const Args& a, int h) {
+  const bool slope = a.slopes != nullptr;
+  return {dmt_cap(a.scale, a.cap, sizeof(T) == 2), slope ? a.slopes[h] * LOG2E : 0.f, a.cap > 0.f, slope};
 }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
-// 1 / (1 + 2^(ck s)) = (1 - tanh) / 2, from which tanh = 1 - 2 r and its derivative 1 - tanh^2 = 4 r (1 - r) follow
-__device__ __forceinline__ float cap_r(const Shape& s, float x) { return rcp_hw(1.f + exp2_hw(s.ck * x)); }
 __device__ __forceinline__ float z2_of(const Shape& s, float x, float dist) {
-  float y = s.cap ? __builtin_fmaf(-2.f * s.cap2, cap_r(s, x), s.cap2) : s.c1 * x;
+  float y = s.capped ? s.cap(x) : s.cap.c1 * x;
   if (s.slope) y = __builtin_fmaf(-s.sl2, fabsf(dist), y);
   return y;
 }
@@ -136,7 +124,7 @@ __device__ void row_fwd(const Args& a, const Ex& e, int h, int i, float* lds, in
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * dh;
   for (int c = lane; c < dh; c += 64) q[c] = ldf<T>(Q + c);
   lds_fence();
-  const Shape s = shape_of(a, h);
+  const Shape s = shape_of<T>(a, h);
   const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
   float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
   for (int j0 = 0; j0 < e.kl; j0 += 64) {
@@ -201,7 +189,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float D, float
     g[c] = ldf<T>((const T*)a.dout + row * a.do_rs + (long long)h * dh + c);
   }
   lds_fence();
-  const Shape s = shape_of(a, h);
+  const Shape s = shape_of<T>(a, h);
   const int qd = a.q_doc ? a.q_doc[e.q0 + i] : 0;
   const float lse2 = a.lse[row * a.Hq + h] * LOG2E;
   float o0 = 0.f, o1 = 0.f, s0 = 0.f, s1 = 0.f, s2 = 0.f, sp = 0.f;
@@ -221,10 +209,7 @@ __device__ float row_dq(const Args& a, const Ex& e, int h, int i, float D, float
       s1 = __builtin_fmaf(pd, fabsf(dist), s1);
       s2 = __builtin_fmaf(p, fabsf(dist), s2);
       dx = p * (dp - D);
-      if (s.cap) {
-        const float r = cap_r(s, x);
-        dx *= 4.f * r * (1.f - r);
-      }
+      if (s.capped) dx *= dmt_cap::derivative(s.cap.r(x));
     }
     xl[lane] = dx;
     lds_fence();
@@ -260,7 +245,7 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int i_lo, 
   lds_fence();
   float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
   for (int h = hk * a.G + part_head(a, part / a.qparts); h < hk * a.G + part_head(a, part / a.qparts + 1); ++h) {
-    const Shape s = shape_of(a, h);
+    const Shape s = shape_of<T>(a, h);
     const T* Q = (const T*)a.Q + e.q0 * a.q_rs + (long long)h * dh;
     const T* O = (const T*)a.dout + e.q0 * a.do_rs + (long long)h * dh;
     for (int i0 = i_lo; i0 < i_hi; i0 += 64) {
@@ -274,10 +259,7 @@ __device__ void row_dkv(const Args& a, const Ex& e, int hk, int part, int i_lo, 
         const float x = dot_rows<T>(k, Q + (long long)i * a.q_rs, dh);
         p = exp2_hw(z2_of(s, x, (float)(i + e.off - j)) - a.lse[qr] * LOG2E);
         dx = p * (dot_rows<T>(v, O + (long long)i * a.do_rs, dh) - a.D[qr]);
-        if (s.cap) {
-          const float r = cap_r(s, x);
-          dx *= 4.f * r * (1.f - r);
-        }
+        if (s.capped) dx *= dmt_cap::derivative(s.cap.r(x));
       }
       pl[lane] = p;
       xl[lane] = dx;

@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
   const bool active = iw < e.ql;
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
-  const Shape sh = shape_of(a, h);
+  const Shape sh = shape_of<T>(a, h);
   // what the workgroup, the wavefront and the lane's row may see
   const int last = (qt * ROWS + ROWS < e.ql ? qt * ROWS + ROWS : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
@@ -97,16 +97,21 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
       }
       settle(s[0], s[1]);
       if (SHAPE) {
-        if (SHAPE == 2) {
+        if (SHAPE == 2 && (sizeof(T) == 4 || sh.cap.near)) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = __builtin_fmaf(-2.f * sh.cap2, cap_r(sh, s[u][r]), sh.cap2);
+            for (int r = 0; r < 16; ++r) s[u][r] = sh.cap.less<true>(s[u][r], sh.cap.r(s[u][r]), 0.f);
+        } else if (SHAPE == 2) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = sh.cap.less<false>(s[u][r], sh.cap.r(s[u][r]), 0.f);
         } else {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] *= sh.c1;
+            for (int r = 0; r < 16; ++r) s[u][r] *= sh.cap.c1;
         }
         if (SHAPE == 1 || sh.slope) {
           const float d0 = (float)(i + e.off - k0 - 4 * half);
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
 #pragma unroll
       for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[1][r]));
       mx = fmaxf(mx, other_half(mx));
-      const float c = SHAPE ? 1.f : sh.c1;
+      const float c = SHAPE ? 1.f : sh.cap.c1;
       const float mt = mx * c;
       if (__any(mt > m + 8.f)) {
         const float mn = fmaxf(m, mt), f = m == -INFINITY ? 0.f : exp2_hw(m - mn);
@@ -316,8 +321,8 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   DMT_CHECK_ARG((int64_t)d->B * d->Hq * (cdiv64(d->max_q > d->max_k ? d->max_q : d->max_k, 64) + 1) < (1ll << 31), "%s: B * Hq * max length / 64 passes 2^31", what);
   DMT_CHECK_ARG(d->B <= 65535 && d->Hq <= 65535, "%s: B and Hq <= 65535", what);
   DMT_CHECK_ARG(d->rows_q < (1ll << 31) && d->rows_k < (1ll << 31), "%s: row numbers are int32", what);
-  DMT_CHECK_ARG(d->scale > 0.f && d->scale < 3.4e38f, "%s: scale must be positive and finite", what);
-  DMT_CHECK_ARG(d->cap >= 0.f && d->cap < 3.4e38f, "%s: cap must be 0 (none) or positive and finite", what);
+  DMT_CHECK_ARG(d->scale > 0.f && d->scale <= 1e38f, "%s: scale must be positive and at most 1e38", what);
+  DMT_CHECK_ARG(d->cap >= 0.f && d->cap <= 1e38f, "%s: cap must be 0 (none) or positive and at most 1e38", what);
   DMT_CHECK_ARG((d->q_doc == nullptr) == (d->k_doc == nullptr), "%s: q_doc and k_doc go together", what);
   if (d->B == 0 || d->max_q == 0 || d->rows_q == 0) {
     // no query row: the forward has nothing to do, the backward still owes dk = dv = 0 and dslopes = 0

@@ -9,21 +9,26 @@ using namespace attn_var;
 namespace {
 
 // The scores of one 32 x 32 tile, in place: z2 minus the row statistic (kept in rows or, stat[], in registers).  d0: distance of register row 0
-// and the lane's column; STEP: what a register row adds to it.  r2: what the cap's derivative needs.
-template <int SHAPE, int STEP, typename STAT>
-__device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& r2, const Shape& sh, float d0, STAT stat) {
+// and the lane's column; STEP: what a register row adds to it.  cr: what the cap's derivative needs.
+template <int SHAPE, int STEP, bool NEAR, typename STAT>
+__device__ __forceinline__ void weights_as(f32x16_t& s, f32x16_t& cr, const Shape& sh, float d0, STAT stat) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     float z;
     if (SHAPE == 2) {
-      r2[r] = cap_r(sh, s[r]);
-      z = __builtin_fmaf(-2.f * sh.cap2, r2[r], sh.cap2 - stat(r));
+      cr[r] = sh.cap.r(s[r]);
+      z = sh.cap.less<NEAR>(s[r], cr[r], stat(r));
     } else {
-      z = __builtin_fmaf(s[r], sh.c1, -stat(r));
+      z = __builtin_fmaf(s[r], sh.cap.c1, -stat(r));
     }
     if (SHAPE == 1 || (SHAPE == 2 && sh.slope)) z = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), z);
     s[r] = exp2_hw(z);
   }
+}
+template <typename T, int SHAPE, int STEP, typename STAT>
+__device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& cr, const Shape& sh, float d0, STAT stat) {
+  if (SHAPE == 2 && (sizeof(T) == 4 || sh.cap.near)) weights_as<SHAPE, STEP, true>(s, cr, sh, d0, stat);
+  else weights_as<SHAPE, STEP, false>(s, cr, sh, d0, stat);
 }
 
 // dQ (and D): one workgroup owns 128 or 64 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of
@@ -50,7 +55,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
   const bool active = iw < e.ql, in = i < e.ql;
   const T* K = (const T*)a.K + e.k0 * a.k_rs + (long long)hk * a.dh;
   const T* V = (const T*)a.V + e.k0 * a.v_rs + (long long)hk * a.dh;
-  const Shape sh = shape_of(a, h);
+  const Shape sh = shape_of<T>(a, h);
   const int last = (qt * ROWS + ROWS < e.ql ? qt * ROWS + ROWS : e.ql) - 1;
   const int lim_wg = a.causal ? max(e.pre, min(e.kl, last + e.off + 1)) : e.kl;
   const int lim_w = a.causal ? max(e.pre, min(e.kl, min(iw + 31, e.ql - 1) + e.off + 1)) : e.kl;
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
       const bool cut = k0 + KT > e.kl || (a.causal && k0 + KT > e.pre && k0 + KT - 1 > iw + e.off);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f32x16_t s = zero16(), dp = zero16(), r2;
+        f32x16_t s = zero16(), dp = zero16(), cr;
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) {
           s = TL::mma(TL::natural(Kl, u, l31, x, half), q[x], s);
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
         }
         const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
         settle(s, dp);
-        weights<SHAPE, -1>(s, r2, sh, d0, [&](int) { return lse2; });
+        weights<T, SHAPE, -1>(s, cr, sh, d0, [&](int) { return lse2; });
         if (docs_differ || cut) {
           // (a masked place gives weight and gradient 0 whatever stands there)
           const int pre = e.pre - k0 - 32 * u - 4 * half, lm = (docs_differ ? lim0 : lim) - k0 - 32 * u - 4 * half;
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] *= dp[r] - D;
-          if (SHAPE == 2) s[r] *= 4.f * r2[r] * (1.f - r2[r]);
+          if (SHAPE == 2) s[r] *= dmt_cap::derivative(cr[r]);
         }
         TL::accumulate(o, Kl, 32 * u, s, lane);
       }
@@ -335,13 +340,13 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
     if (gn < ng) begin(gn, tn, NB == 2 ? buf ^ 1 : 0);
     const T* Ql = lds + buf * 2 * QE;
     const T* Gl = Ql + QE;
-    const Shape sh = shape_of(a, hk * a.G + g0 + g);
+    const Shape sh = shape_of<T>(a, hk * a.G + g0 + g);
     const bool work = active && i0 + KT > lo_w && (flags & 1), docs_differ = DOCS && (flags & 2) && jw + 32 > e.pre;
     if (work) {
       const bool cut = jw + 32 > e.kl || (a.causal && jw + 32 > e.pre && i0 + e.off < jw + 31);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        f32x16_t s = zero16(), dp = zero16(), r2;
+        f32x16_t s = zero16(), dp = zero16(), cr;
 #pragma unroll
         for (int x = 0; x < TL::NS; ++x) {
           s = TL::mma(TL::natural(Ql, u, l31, x, half), k[x], s);
@@ -352,7 +357,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
         f32x4_t ls[4];
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg) ls[gg] = *reinterpret_cast<const f32x4_t*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
-        weights<SHAPE, 1>(s, r2, sh, (float)(i0 + 32 * u + 4 * half + e.off - j), [&](int r) { return ls[r >> 2][r & 3]; });
+        weights<T, SHAPE, 1>(s, cr, sh, (float)(i0 + 32 * u + 4 * half + e.off - j), [&](int r) { return ls[r >> 2][r & 3]; });
         if (docs_differ || cut) {
           const int lo = lo_l - i0 - 32 * u - 4 * half;
 #pragma unroll
@@ -377,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             s[4 * gg + c] *= dp[4 * gg + c] - D[c];
-            if (SHAPE == 2) s[4 * gg + c] *= 4.f * r2[4 * gg + c] * (1.f - r2[4 * gg + c]);
+            if (SHAPE == 2) s[4 * gg + c] *= dmt_cap::derivative(cr[4 * gg + c]);
           }
         }
         TL::accumulate(dk, Ql, 32 * u, s, lane);

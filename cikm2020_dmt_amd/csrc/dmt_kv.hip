@@ -409,11 +409,7 @@ __device__ __forceinline__ int sees(const KvArgs& a, const Req& q, int i) {
 }
 
 __device__ __forceinline__ float kv_z2(const KvArgs& a, float x, float slope2, float dist) {
-  float y = a.scale * LOG2E * x;
-  if (a.cap > 0.f) {
-    const float c2 = a.cap * LOG2E;
-    y = __builtin_fmaf(-2.f * c2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.f * LOG2E * a.scale / a.cap * x)), c2);
-  }
+  const float y = a.cap > 0.f ? dmt_cap(a.scale, a.cap, true)(x) : a.scale * LOG2E * x;
   return a.slopes ? __builtin_fmaf(-slope2, fabsf(dist), y) : y;
 }
 __device__ __forceinline__ void lds_fence() {
@@ -596,7 +592,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[x][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const float c1 = a.scale * LOG2E, cap2 = a.cap * LOG2E, ck = a.cap > 0.f ? 2.f * LOG2E * a.scale / a.cap : 0.f;
+  const dmt_cap cap(a.scale, a.cap, true);
+  const float c1 = cap.c1;
   const int* tb = a.table + (long long)r * a.width;
   int block = b0 + wave < b1 ? tb[b0 + wave] : 0;
   for (int t = b0 + wave; t < b1; t += 4) {
@@ -667,15 +664,23 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
       const int lx = lim[x] - j0 - 4 * grp;
       const float d0 = (float)(pos[x] - j0 - 4 * grp);
       float mx = -INFINITY;
+      if (SHAPED) {
+        const auto each = [&](auto score) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[x][u][e] = score(s[x][u][e]);
+        };
+        if (!(a.cap > 0.f)) each([&](float z) { return c1 * z; });
+        else if (cap.near) each([&](float z) { return cap.less<true>(z, cap.r(z), 0.f); });
+        else each([&](float z) { return cap.less<false>(z, cap.r(z), 0.f); });
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float z = s[x][u][e];
-          if (SHAPED) {
-            z = a.cap > 0.f ? __builtin_fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(ck * z)), cap2) : c1 * z;
-            z = __builtin_fmaf(-sl2[x], fabsf(d0 - (float)(16 * u + e)), z);
-          }
+          if (SHAPED) z = __builtin_fmaf(-sl2[x], fabsf(d0 - (float)(16 * u + e)), z);
           z = 16 * u + e < lx ? z : -INFINITY;
           s[x][u][e] = z;
           mx = fmaxf(mx, z);
@@ -996,7 +1001,8 @@ extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
   DMT_CHECK_ARG(d->Hq > 0 && d->Hq <= 65535 && d->Hq % d->Hkv == 0, "dmt_kv_attn: Hq %d is not a multiple of Hkv %d", d->Hq, d->Hkv);
   DMT_CHECK_ARG(d->n >= 0 && d->n <= 65535 && d->max_q >= 0 && d->max_len >= 0 && d->width >= 0 && d->rows >= 0 && d->rows < (1ll << 31),
                 "dmt_kv_attn: n %d (at most 65535), max_q %d, max_len %d, width %d", d->n, d->max_q, d->max_len, d->width);
-  DMT_CHECK_ARG(d->scale > 0.f && d->scale < 3.4e38f && d->cap >= 0.f && d->cap < 3.4e38f, "dmt_kv_attn: scale must be positive, cap 0 or positive");
+  DMT_CHECK_ARG(d->scale > 0.f && d->scale <= 1e38f && d->cap >= 0.f && d->cap <= 1e38f,
+                "dmt_kv_attn: scale must be positive, cap 0 or positive, both at most 1e38");
   if (d->n == 0 || d->max_q == 0 || d->rows == 0) return DMT_OK;
   DMT_CHECK_ARG(d->Q && d->out && d->lens && d->row_off && (d->table || d->width == 0), "dmt_kv_attn: NULL pointer");
   const int64_t wq = (int64_t)d->Hq * d->dh;

@@ -181,8 +181,8 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
     if slopes is not None and (slopes.dtype != F32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous() or slopes.device != dev):
         raise ValueError("slopes must be a contiguous fp32 tensor [%d] on %s" % (H, dev))
     scale = 1.0 / float(cache.dh) ** 0.5 if scale is None else float(scale)
-    if not (0.0 < scale < 3e38) or not (0.0 <= cap < 3e38):
-        raise ValueError("scale must be positive and finite, cap 0 or positive and finite: got %r, %r" % (scale, cap))
+    if not (0.0 < scale <= 1e38) or not (0.0 <= cap <= 1e38):
+        raise ValueError("scale must be positive, cap 0 or positive, both at most 1e38: got %r, %r" % (scale, cap))
     if max_q < 0 or (max_len is not None and max_len < 0):
         raise ValueError("max_q and max_len must not be negative")
     max_q = min(int(max_q), q.shape[0])                                          # (no request has more rows than there are)

@@ -1361,8 +1361,8 @@ def attn_var(q, k, v, seqs: AttnSeqs, H, Hkv=None, *, scale=None, cap=0.0, slope
     if slopes is not None and (slopes.dtype != F32 or tuple(slopes.shape) != (H,) or not slopes.is_contiguous() or slopes.device != q.device):
         raise ValueError("slopes must be a contiguous fp32 tensor [%d] on %s" % (H, q.device))
     scale = 1.0 / float(dh) ** 0.5 if scale is None else float(scale)
-    if not (0.0 < scale < 3e38) or not (0.0 <= cap < 3e38):
-        raise ValueError("scale must be positive and finite, cap 0 or positive and finite: got %r, %r" % (scale, cap))
+    if not (0.0 < scale <= 1e38) or not (0.0 <= cap <= 1e38):
+        raise ValueError("scale must be positive, cap 0 or positive, both at most 1e38: got %r, %r" % (scale, cap))
     prefix = _ids(prefix, seqs.B, "prefix", q.device)
     q_doc, k_doc = (None, None) if docs is None else (_ids(docs[0], q.shape[0], "docs[0]", q.device), _ids(docs[1], k.shape[0], "docs[1]", q.device))
     fill = (seqs.zero_fill, seqs.zero_fill) if seqs.zero_fill is not None else (seqs.total_q != q.shape[0], seqs.total_k != k.shape[0] or seqs.k_shared)

@@ -821,6 +821,7 @@ int dmt_q1mem_bwd(const dmt_q1mem_desc* d, void* stream);
  * A row that may see nothing gets out = 0, lse = -inf and no gradient.  What stands in a masked place -- NaN and infinities too -- does
  * not reach a row that may not see it.  Rows that belong to no example are neither read nor written.
  * Types: DMT_BF16 (dh a multiple of 8) and DMT_F32 (dh a multiple of 4), dh <= 128; sums, softmax statistics and gradients in fp32.
+ * A capped score is within 2^-20 of its value for fp32 operands and for caps over 64; for bf16 operands with smaller caps within 2^-21 cap besides.
  * Every operand row 16-byte aligned (base and row stride), row strides under 16 MB; out is none of them.  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
  * caller's promise: it sizes the grid; longer examples are cut there).
  * Backward: dq, dk, dv for the rows of every example, and dslopes [Hq] (summed in a fixed order).
@@ -836,8 +837,8 @@ typedef struct {
   const void* V; int64_t v_rs;
   const int32_t* q_off; const int32_t* q_lens;
   const int32_t* k_off; const int32_t* k_lens;
-  float scale;                             /* > 0                                                      */
-  float cap;                               /* 0: none                                                  */
+  float scale;                             /* > 0, at most 1e38                                        */
+  float cap;                               /* 0: none; at most 1e38                                    */
   int32_t causal;
   const float* slopes;                     /* [Hq] or NULL                                             */
   const int32_t* prefix;                   /* [B] or NULL                                              */

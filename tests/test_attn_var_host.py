@@ -155,3 +155,16 @@ def test_row_strides_that_32_rows_cannot_hold_are_refused(rs):
     """rows are addressed by 32-bit offsets from the first row of a wavefront (or of a 64-row tile): 2^24 bytes a row at most, o_rs included"""
     lib, d = L.load(), _desc(**{rs: 1 << 23})
     assert lib.dmt_attn_var_bwd(C.byref(d), None) == -1 and b"stride" in lib.dmt_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(cap=1.1e38), dict(scale=1.1e38), dict(cap=3e38)])
+def test_caps_and_scales_whose_log2_form_overflows_are_refused(kw):
+    """(2 cap log2 e has to be finite: past 1e38 it was not, and the scores came out NaN)"""
+    lib, d = L.load(), _desc(**kw)
+    assert lib.dmt_attn_var_fwd(C.byref(d), None) == -1 and b"1e38" in lib.dmt_last_error()
+    k = L.KvAttnDesc()
+    base = dict(n=1, Hq=2, Hkv=2, dh=32, n_blocks=8, max_q=1, max_len=64, width=1, rows=1, k=1024, v=1024, k_scale=64, v_scale=64, Q=1024, q_rs=64,
+                table=64, lens=64, row_off=64, scale=1.0, cap=0.0, causal=1, out=1024, o_rs=64, ws=1024, ws_bytes=1 << 30)
+    for n, v in {**base, **kw}.items():
+        setattr(k, n, v)
+    assert lib.dmt_kv_attn(C.byref(k), None) == -1 and b"1e38" in lib.dmt_last_error()

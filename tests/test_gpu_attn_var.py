@@ -423,3 +423,37 @@ def test_contiguous_rows_of_one_example_past_4_gib(cuda):
                 sums[x][:, ck] += r[x]
         for t, x in ((dk, "dk"), (dv, "dv")):
             A.close(t, sums[x].cpu(), (sums[x + "_tol"] + u * sums[x].abs() + 1e-30).cpu(), x)
+
+
+@pytest.mark.parametrize("cap", [0.01, 1.0, 30.0, 50.0, 1e3, 1e6, 1e30, 9e37])
+def test_capped_scores_keep_their_bits(cuda, cap):
+    """One visible key: lse is the score.  x is exact in fp32 (one product, a scale of 1), so what is off is the cap alone: the tanh form (under
+    2^-20 of the value: a polynomial below x = 0.35 cap, 1 - 2 / (1 + e^2x) above, with v_rcp_f32 and v_exp_f32 of 1 ulp) and three
+    products that turn it to log2 units and back (2^-24 each).  Nothing may grow with the cap."""
+    mags = torch.logspace(-6, 4, 401, dtype=torch.float64).to(F32)
+    if cap < 1e4:
+        mags = torch.cat([mags, torch.linspace(0.01, 4, 400, dtype=torch.float64).to(F32) * cap])
+    x = torch.cat([mags, -mags, torch.zeros(1)])
+    q = torch.zeros((len(x), 16), dtype=F32)
+    q[:, 3] = x
+    k = torch.zeros((1, 16), dtype=F32)
+    k[0, 3] = 1.0
+    out, lse = ops.attn_var(q.to(cuda), k.to(cuda), k.to(cuda), ops.AttnSeqs([len(x)], [1], device=cuda), 1, scale=1.0, cap=cap, want_lse=True)
+    want = cap * torch.tanh(x.double() / cap)
+    assert ((lse[:, 0].cpu().double() - want).abs() <= 2.0 ** -19 * want.abs()).all()
+    assert torch.equal(out.cpu(), k.expand(len(x), 16))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e30])
+def test_caps_far_over_the_scores_change_nothing(cuda, cap, dtype):
+    """Scores of about 8 under a cap of 1e4 and more: y = x (1 - (x / cap)^2 / 3 ...) is x to 1e-6 of it.  The bounds are those of scores without a
+    cap (which do not grow with it), plus that difference in the scores' own bound (FP32 = 2^-17 holds it)."""
+    ql, kl, H, Hkv, dh = [100, 37], [100, 90], 4, 2, 64
+    q, k, v, do, qo, ko = _make(ql, kl, H, Hkv, dh, dtype, 12, 1.5)
+    sl = torch.tensor([0.1, 0.0, 1.0, 0.01])
+    ref = A.attn_var(q, k, v, H, Hkv, ql, kl, qo, ko, causal=True, slopes=sl, dout=do)
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v, sl)]
+    out, lse = ops.attn_var(*lv[:3], ops.AttnSeqs(ql, kl, device=cuda), H, Hkv, slopes=lv[3], causal=True, cap=cap, want_lse=True)
+    for t, n in zip((out, lse) + torch.autograd.grad(out, lv, do.to(cuda)), ("out", "lse", "dq", "dk", "dv", "dslope")):
+        A.close(t, ref[n], ref[n + "_tol"], n)

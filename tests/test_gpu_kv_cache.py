@@ -506,3 +506,41 @@ def test_refusals_of_device_arguments(cuda):
               (c.k, c.v, c.k_scale.double(), c.v_scale), (c.k.cpu(), c.v.cpu(), c.k_scale.cpu(), c.v_scale.cpu())):
         with pytest.raises(ValueError):
             KV.KVCache(*a)
+
+
+@pytest.mark.parametrize("m", [1, 30])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e30])
+def test_caps_far_over_the_scores(cuda, cap, m):
+    """the bounds of scores without a cap hold: a cap of 1e4 and more changes scores of about 8 by less than 1e-6 of them"""
+    lens, H, Hkv, dh = [200, 65], 4, 2, 80
+    cache, table, dense = _cache_of(cuda, lens, Hkv, dh, 23)
+    q = torch.randn((2 * m, H * dh), generator=torch.Generator().manual_seed(24)).to(BF)
+    got, lse = KV.kv_attn(cache, q.to(cuda), table, _i(lens, cuda), _i([0, m, 2 * m], cuda), H, m, causal=False, cap=cap, want_lse=True)
+    for r, L in enumerate(lens):
+        ok, dist = torch.ones((m, L), dtype=torch.bool), torch.zeros((m, L), dtype=torch.int64)
+        for h in range(H):
+            c, hk = slice(h * dh, h * dh + dh), h // (H // Hkv)
+            ref = A.head(q[r * m:r * m + m, c], dense[r][0][hk], dense[r][1][hk], ok, dist, dh ** -0.5, 0.0, None, BF)
+            A.close(got[r * m:r * m + m, c], ref["out"], ref["out_tol"], "out")
+            A.close(lse[r * m:r * m + m, h], ref["lse"], ref["lse_tol"], "lse")
+
+
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e3, 1e6, 9e37])
+def test_capped_scores_keep_their_bits(cuda, cap):
+    """One cached token: lse is the score, whose dot product is exact; what is off is the tanh form and three roundings.  Caps of at most 64 take
+    cap (1 - 2 r): r, at most 1, comes from a sum (2^-24), v_rcp_f32 (2^-23) and a power (v_exp_f32 and its argument, 2^-23 each of r (1 - r) <= 1/4
+    where |a| is small and less where the argument is long): under 2^-22.4, doubled and rounded: 2^-21 of the cap.  Larger ones: 2^-20 of the value."""
+    cache = KV.KVCache.empty(1, 1, 16, cuda)
+    one = torch.zeros((1, 16), dtype=BF, device=cuda)
+    one[0, 3] = 1.0
+    plan = KV.kv_plan(_i([0], cuda), _i([1], cuda), _i([[-1]], cuda), _i([0], cuda), _i([1], cuda), 1)
+    KV.kv_append(cache, one, one, plan)
+    mags = torch.logspace(-6, 3, 301, dtype=F64).to(BF)
+    if cap < 1e4:
+        mags = torch.cat([mags, (torch.linspace(0.01, 4, 400, dtype=F64) * cap).to(BF)])
+    x = torch.cat([mags, -mags])
+    q = torch.zeros((len(x), 16), dtype=BF)
+    q[:, 3] = x
+    _, lse = KV.kv_attn(cache, q.to(cuda), _i([[0]], cuda), plan.lens, _i([0, len(x)], cuda), 1, len(x), causal=False, scale=1.0, cap=cap, want_lse=True)
+    want = cap * torch.tanh(x.double() / cap)
+    assert ((lse[:, 0].cpu().double() - want).abs() <= 2.0 ** -19 * want.abs() + (2.0 ** -21 * cap if cap <= 64 else 0.0)).all()
