@@ -387,25 +387,29 @@ struct KvArgs {
   float* lse;
 };
 
-struct Req { int m, L; long long row0; };
+// A request's rows and tokens as far as they are computed (m, L: cut at max_q, max_len, the table's width and the matrix), and `at`, the position
+// of its first row (causal) or of all of them, from the lengths as they stand: what is cut off moves nothing that stays.
+struct Req { int m, L, at; long long row0; };
 __device__ __forceinline__ Req request(const KvArgs& a, int r) {
   Req q;
-  const long long lo = a.row_off[r], hi = a.row_off[r + 1];
+  const long long lo = a.row_off[r], hi = a.row_off[r + 1], held = a.lens[r];
   q.row0 = lo < 0 ? 0 : (lo > a.rows ? a.rows : lo);
   long long m = (hi > a.rows ? a.rows : hi) - q.row0;
   q.m = m < 0 ? 0 : (int)(m > a.max_q ? a.max_q : m);
   const long long most = (long long)a.width * BS;
-  long long L = a.lens[r];
+  long long L = held;
   if (L > a.max_len) L = a.max_len;
   if (L > most) L = most;
   q.L = L < 0 ? 0 : (int)L;
+  const long long at = a.causal ? held - (hi - q.row0) : held;
+  q.at = (int)(at < -0x7fffffffll ? -0x7fffffffll : at);       // (held < 2^31 and hi >= row0 where there is a row)
   return q;
 }
 // position of row i, and the number of tokens that it sees
-__device__ __forceinline__ int position(const KvArgs& a, const Req& q, int i) { return a.causal ? q.L - q.m + i : q.L; }
+__device__ __forceinline__ int position(const KvArgs& a, const Req& q, int i) { return a.causal ? q.at + i : q.at; }
 __device__ __forceinline__ int sees(const KvArgs& a, const Req& q, int i) {
-  const int s = a.causal ? q.L - q.m + i + 1 : q.L;
-  return s < 0 ? 0 : s;
+  const int s = a.causal ? q.at + i + 1 : q.L;
+  return s < 0 ? 0 : (s < q.L ? s : q.L);
 }
 
 __device__ __forceinline__ float kv_z2(const KvArgs& a, float x, float slope2, float dist) {

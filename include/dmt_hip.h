@@ -903,7 +903,8 @@ int dmt_kv_read(int32_t Hkv, int32_t dh, int32_t n_blocks, const uint8_t* k, con
  * (at most max_q of them are computed), lens[r] cached tokens.  causal: row i of m stands at position lens - m + i and sees the tokens up
  * to itself (the step's own tokens were appended before); otherwise every row stands at position lens and sees them all.  Distance of the
  * slopes: |position - j|.  A row that sees nothing gets 0 and lse -inf.  max_len bounds the lengths (a promise that sizes the grid and the
- * split over the length; longer requests are cut there; lens past the table's width too).  Table entries outside the pool: masked.
+ * split over the length; tokens past it are not seen, nor those past the table's width, and rows past max_q not computed; lens, m and the
+ * positions are those of the whole request all the same).  Table entries outside the pool: masked.
  * One wavefront takes 64 tokens at a time; the length is split over workgroups by a rule on (n, Hkv, max_q, max_len) alone, and the pieces
  * are joined in their order: bit-reproducible.  out is not Q.  ws: dmt_kv_attn_ws_bytes(d), 16-byte aligned, one call at a time. */
 typedef struct {

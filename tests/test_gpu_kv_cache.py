@@ -544,3 +544,26 @@ def test_capped_scores_keep_their_bits(cuda, cap):
     _, lse = KV.kv_attn(cache, q.to(cuda), _i([[0]], cuda), plan.lens, _i([0, len(x)], cuda), 1, len(x), causal=False, scale=1.0, cap=cap, want_lse=True)
     want = cap * torch.tanh(x.double() / cap)
     assert ((lse[:, 0].cpu().double() - want).abs() <= 2.0 ** -19 * want.abs() + (2.0 ** -21 * cap if cap <= 64 else 0.0)).all()
+
+
+@pytest.mark.parametrize("m,max_q,L,max_len,causal", [(40, 16, 200, None, True), (40, 33, 200, None, True), (5, 1, 70, None, True), (3, 3, 300, 128, True),
+                                                      (64, 10, 300, 256, True), (3, 2, 300, 100, False), (9, 4, 5, None, True)])
+def test_rows_and_tokens_past_the_bounds_are_cut_where_they_stand(cuda, m, max_q, L, max_len, causal):
+    """A replayed graph's requests may outgrow max_q / max_len: rows and tokens past them are cut, and row i still stands at lens - m + i, so it sees
+    no token of the rows behind it, and its distances are those of the whole request"""
+    H, Hkv, dh = 4, 2, 32
+    cache, table, dense = _cache_of(cuda, [L], Hkv, dh, 21)
+    q = torch.randn((m, H * dh), generator=torch.Generator().manual_seed(22)).to(BF)
+    sl = torch.tensor([0.05, 0.0, 0.2, 0.01])
+    out = torch.full_like(q, 7.0).to(cuda)
+    got, lse = KV.kv_attn(cache, q.to(cuda), table, _i([L], cuda), _i([0, m], cuda), H, max_q, max_len, causal=causal, slopes=sl.to(cuda), out=out, want_lse=True)
+    n, most = min(m, max_q), L if max_len is None else min(L, max_len)
+    pos = L - m + torch.arange(n) if causal else torch.full((n,), L)
+    dist = pos[:, None] - torch.arange(most)[None]
+    ok = dist >= 0 if causal else torch.ones((n, most), dtype=torch.bool)
+    for h in range(H):
+        c, hk = slice(h * dh, h * dh + dh), h // (H // Hkv)
+        ref = A.head(q[:n, c], dense[0][0][hk][:most], dense[0][1][hk][:most], ok, dist, dh ** -0.5, 0.0, sl[h].double(), BF)
+        A.close(got[:n, c], ref["out"], ref["out_tol"], "out of head %d" % h)
+        A.close(lse[:n, h], ref["lse"], ref["lse_tol"], "lse of head %d" % h)
+    assert (got[n:] == 7.0).all()
