@@ -48,7 +48,7 @@ __device__ __forceinline__ const Args* args_again() {
   return (const Args*)p;
 }
 
-// one example's lengths and what its queries may see
+// one example's lengths (as far as they are computed), the distance of its last key and last query, and what its queries may see
 struct Ex {
   int ql, kl, off, pre;
   long long q0, k0;
@@ -66,7 +66,10 @@ __device__ __forceinline__ Ex example(const Args& a, int b) {
   e.k0 = a.k_off[b];
   e.ql = clip_len(a.q_lens[b], a.max_q, (int)e.q0, a.rows_q);
   e.kl = clip_len(a.k_lens[b], a.max_k, (int)e.k0, a.rows_k);
-  e.off = e.kl - e.ql;
+  // positions are those of the lengths as they stand: what is cut off moves nothing that stays (the last 4096 numbers below 2^31 are kept free for the
+  // rows and keys that a tile has beyond its example)
+  const auto whole = [](int n) { return n < 0 ? 0 : (n < 0x7fffefff ? n : 0x7fffefff); };
+  e.off = whole(a.k_lens[b]) - whole(a.q_lens[b]);
   const int p = a.prefix ? a.prefix[b] : 0;
   e.pre = p < 0 ? 0 : (p > e.kl ? e.kl : p);
   return e;

@@ -823,7 +823,7 @@ int dmt_q1mem_bwd(const dmt_q1mem_desc* d, void* stream);
  * Types: DMT_BF16 (dh a multiple of 8) and DMT_F32 (dh a multiple of 4), dh <= 128; sums, softmax statistics and gradients in fp32.
  * A capped score is within 2^-20 of its value for fp32 operands and for caps over 64; for bf16 operands with smaller caps within 2^-21 cap besides.
  * Every operand row 16-byte aligned (base and row stride), row strides under 16 MB; out is none of them.  No length limit but int32 row numbers; max_q / max_k bound the lengths (the
- * caller's promise: it sizes the grid; longer examples are cut there).
+ * caller's promise: it sizes the grid; rows and keys past them are left out, off_b stays that of the lengths as they stand).
  * Backward: dq, dk, dv for the rows of every example, and dslopes [Hq] (summed in a fixed order).
  * Bit-reproducible: no atomics.  ws: dmt_attn_var_ws_bytes(...) bytes, 16-byte aligned, no initialisation needed; one call at a time.
  * ------------------------------------------------------------------------------------------------ */

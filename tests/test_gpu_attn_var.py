@@ -457,3 +457,33 @@ def test_caps_far_over_the_scores_change_nothing(cuda, cap, dtype):
     out, lse = ops.attn_var(*lv[:3], ops.AttnSeqs(ql, kl, device=cuda), H, Hkv, slopes=lv[3], causal=True, cap=cap, want_lse=True)
     for t, n in zip((out, lse) + torch.autograd.grad(out, lv, do.to(cuda)), ("out", "lse", "dq", "dk", "dv", "dslope")):
         A.close(t, ref[n], ref[n + "_tol"], n)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_lengths_past_the_bounds_are_cut_where_they_stand(cuda, causal):
+    """A replayed graph's lengths may outgrow max_q / max_k: the rows past them are cut, and those before keep their positions (i + Lk - Lq of the
+    stated lengths): nothing sees a key that it would not see in the whole history"""
+    for mq, mk, ql, kl in ((40, 90, 70, 90), (70, 50, 70, 90), (33, 65, 150, 170), (40, 200, 100, 30)):
+        q, k, v, do, _, _ = _make([ql], [kl], 2, 1, 32, F32, 13)
+        seqs = ops.AttnSeqs([min(ql, mq)], [min(kl, mk)], device=cuda, max_q=mq, max_k=mk, zero_fill=True)
+        seqs.q_lens.fill_(ql)
+        seqs.k_lens.fill_(kl)
+        nq, nk = min(ql, mq), min(kl, mk)
+        sl = torch.tensor([0.2, 0.05])
+        lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v, sl)]
+        out, lse = ops.attn_var(*lv[:3], seqs, 2, 1, slopes=lv[3], causal=causal, want_lse=True)
+        grads = torch.autograd.grad(out, lv, do.to(cuda))
+        dist = torch.arange(nq)[:, None] + kl - ql - torch.arange(nk)[None]
+        ok = dist >= 0 if causal else torch.ones((nq, nk), dtype=torch.bool)
+        dk, dv, tk, tv = (torch.zeros((nk, 32), dtype=torch.float64) for _ in range(4))
+        for h in range(2):
+            c = slice(32 * h, 32 * h + 32)
+            r = A.head(q[:nq, c], k[:nk], v[:nk], ok, dist, 32 ** -0.5, 0.0, sl[h].double(), F32, do[:nq, c])
+            A.close(out[:nq, c], r["out"], r["out_tol"], "out")
+            A.close(lse[:nq, h], r["lse"], r["lse_tol"], "lse")
+            A.close(grads[0][:nq, c], r["dq"], r["dq_tol"], "dq")
+            A.close(grads[3][h:h + 1], r["dslope"][None], r["dslope_tol"][None], "dslope")
+            dk, dv, tk, tv = dk + r["dk"], dv + r["dv"], tk + r["dk_tol"], tv + r["dv_tol"]
+        A.close(grads[1][:nk], dk, tk + 2.0 ** -24 * dk.abs() + 1e-30, "dk")
+        A.close(grads[2][:nk], dv, tv + 2.0 ** -24 * dv.abs() + 1e-30, "dv")
+        assert (out[nq:] == 0).all() and (grads[0][nq:] == 0).all() and (grads[1][nk:] == 0).all() and (grads[2][nk:] == 0).all()
