@@ -324,9 +324,16 @@ int dmt_attn_var_args(const dmt_attn_var_desc* d, Args* a, bool backward, const 
   DMT_CHECK_ARG(d->scale > 0.f && d->scale <= 1e38f, "%s: scale must be positive and at most 1e38", what);
   DMT_CHECK_ARG(d->cap >= 0.f && d->cap <= 1e38f, "%s: cap must be 0 (none) or positive and at most 1e38", what);
   DMT_CHECK_ARG((d->q_doc == nullptr) == (d->k_doc == nullptr), "%s: q_doc and k_doc go together", what);
-  if (d->B == 0 || d->max_q == 0 || d->rows_q == 0) {
+  if (d->B == 0) {                       // no example: only a slopes' gradient is owed, and nothing is read
+    if (!backward || !d->dslopes) return 1;
+    *a = Args{};
+    a->Hq = d->Hq;
+    a->dslopes = d->dslopes;
+    return DMT_OK;
+  }
+  if (d->max_q == 0 || d->rows_q == 0) {
     // no query row: the forward has nothing to do, the backward still owes dk = dv = 0 and dslopes = 0
-    if (!backward || ((d->B == 0 || d->max_k == 0 || d->rows_k == 0) && !d->dslopes)) return 1;
+    if (!backward || ((d->max_k == 0 || d->rows_k == 0) && !d->dslopes)) return 1;
   }
   DMT_CHECK_ARG(d->q_off && d->q_lens && d->k_off && d->k_lens, "%s: NULL offsets or lengths", what);
   const int es = d->dtype == DMT_F32 ? 4 : 2;

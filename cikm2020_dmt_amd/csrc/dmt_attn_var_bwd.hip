@@ -491,7 +491,7 @@ int launch_bwd(Args a, hipStream_t st) {
     else launch_dq<T, 128>(a, st);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(dq)");
   }
-  if (a.dslopes && (!nkt || !a.rows_q || !nqt)) {      // (no dK / dV kernel to finish them, or no query at all: n = 0)
+  if (a.dslopes && (!nkt || !a.rows_q || !nqt)) {      // (no dK / dV kernel to finish them, or no query or example at all: n = 0)
     slopes_kernel<<<a.Hq, 256, 0, st>>>(a, a.rows_q && nqt ? (long long)a.B * nqt : 0);
     DMT_CHECK_LAUNCH("dmt_attn_var_bwd(slopes)");
     a.slope_part = nullptr;

@@ -487,3 +487,16 @@ def test_lengths_past_the_bounds_are_cut_where_they_stand(cuda, causal):
         A.close(grads[1][:nk], dk, tk + 2.0 ** -24 * dk.abs() + 1e-30, "dk")
         A.close(grads[2][:nk], dv, tv + 2.0 ** -24 * dv.abs() + 1e-30, "dv")
         assert (out[nq:] == 0).all() and (grads[0][nq:] == 0).all() and (grads[1][nk:] == 0).all() and (grads[2][nk:] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [0, 3])
+@pytest.mark.parametrize("most", [None, 4])
+def test_an_empty_batch_has_gradients(cuda, rows, most):
+    """no example at all, with and without rows of no example: everything is zero, the slopes' gradient too"""
+    lv = [torch.randn((rows, 64), device=cuda).to(BF).requires_grad_(True) for _ in range(3)] + [torch.tensor([0.3, 0.1], device=cuda, requires_grad=True)]
+    keep = torch.full((2,), 7.0, device=cuda)
+    del keep                                                                     # (the allocator hands this memory out again: nothing may be left unwritten)
+    out = ops.attn_var(*lv[:3], ops.AttnSeqs([], device=cuda, max_q=most, max_k=most), 2, slopes=lv[3])
+    assert out.shape == (rows, 64) and (out == 0).all()
+    for g, x in zip(torch.autograd.grad(out, lv, torch.ones_like(out)), lv):
+        assert g.shape == x.shape and (g == 0).all()
