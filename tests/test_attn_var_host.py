@@ -1,5 +1,8 @@
 """What attn_var and the K / V cache refuse, and the host side of AttnSeqs: no GPU needed."""
 import ctypes as C
+import glob
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -168,3 +171,11 @@ def test_caps_and_scales_whose_log2_form_overflows_are_refused(kw):
     for n, v in {**base, **kw}.items():
         setattr(k, n, v)
     assert lib.dmt_kv_attn(C.byref(k), None) == -1 and b"1e38" in lib.dmt_last_error()
+
+
+def test_other_flags_build_every_object_again():
+    """the flags stand in the Makefile, and some of them are needed for right results: objects of an earlier Makefile are not linked"""
+    csrc = os.path.join(os.path.dirname(L.__file__), "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc], check=True, capture_output=True, text=True).stdout
+    for f in glob.glob(os.path.join(csrc, "*.hip")):
+        assert "-c " + os.path.basename(f) in plan, f
