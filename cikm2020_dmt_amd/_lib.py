@@ -18,7 +18,7 @@ DMT_MAX_FEATURES, DMT_MAX_SEQS, DMT_MAX_TABLES = 32, 4, 32
 DMT_SEQ_TARGET = 100
 DMT_KV_BLOCK = 64
 DMT_ERR_UNSUPPORTED = -3
-DMT_ABI_VERSION = 7        # include/dmt_hip.h: the revision this binding was written against (checked by load())
+DMT_ABI_VERSION = 8        # include/dmt_hip.h: the revision this binding was written against (checked by load())
 
 c_i32, c_i64, c_f32, c_vp = C.c_int32, C.c_int64, C.c_float, C.c_void_p
 
@@ -150,8 +150,8 @@ class AttnVarDesc(C.Structure):
 class KvAttnDesc(C.Structure):
     _fields_ = [("n", c_i32), ("Hq", c_i32), ("Hkv", c_i32), ("dh", c_i32), ("n_blocks", c_i32), ("max_q", c_i32), ("max_len", c_i32),
                 ("width", c_i32), ("rows", c_i64), ("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("Q", c_vp), ("q_rs", c_i64),
-                ("table", c_vp), ("lens", c_vp), ("row_off", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32), ("slopes", c_vp),
-                ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
+                ("table", c_vp), ("lens", c_vp), ("row_off", c_vp), ("scale", c_f32), ("cap", c_f32), ("causal", c_i32), ("rest", c_i32),
+                ("slopes", c_vp), ("out", c_vp), ("o_rs", c_i64), ("lse", c_vp), ("ws", c_vp), ("ws_bytes", C.c_uint64)]
 
 
 def _packer(desc):

@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256) void read_kernel(const Cache c, int n, const i
 // ================================================================================================================ attention
 struct KvArgs {
   Cache c;
-  int n, Hq, G, max_q, max_len, width, causal;
+  int n, Hq, G, max_q, max_len, width, causal, rest;
   long long rows;
   const bf16_t* Q; long long q_rs;
   const int* table; const int* lens; const int* row_off;
@@ -420,6 +420,31 @@ __device__ __forceinline__ void lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// rows r0 .. r1 - 1 of the heads h0 .. h0 + heads - 1 that no request's row is: zeros in out, -inf in lse, as a.rest asks
+__device__ __forceinline__ void rest_rows(const KvArgs& a, long long r0, long long r1, int h0, int heads) {
+  const int c8 = heads * a.c.dh / 8;
+  if (a.rest & 1)
+    for (long long x = threadIdx.x; x < (r1 - r0) * c8; x += blockDim.x)
+      *reinterpret_cast<uint4*>(a.out + (r0 + x / c8) * a.o_rs + (long long)h0 * a.c.dh + x % c8 * 8) = make_uint4(0u, 0u, 0u, 0u);
+  if ((a.rest & 2) && a.lse)
+    for (long long x = threadIdx.x; x < (r1 - r0) * heads; x += blockDim.x) a.lse[(r0 + x / heads) * a.Hq + h0 + x % heads] = -INFINITY;
+}
+// ... as workgroup `part` of `parts` of key head hk finds them: what of request r (part `first` of its own) lies past max_q, the rows before the first
+// request's, and its share of those behind the last one's
+__device__ __forceinline__ void rest_of(const KvArgs& a, const Req& rq, int r, int hk, bool first, long long part, long long parts) {
+  const long long hi = a.row_off[r + 1], end = hi < a.rows ? hi : a.rows, last = a.row_off[a.n], tail = last < 0 ? 0 : (last < a.rows ? last : a.rows);
+  if (first && r == 0 && rq.row0 > 0) rest_rows(a, 0, rq.row0, hk * a.G, a.G);
+  if (first && rq.row0 + rq.m < end) rest_rows(a, rq.row0 + rq.m, end, hk * a.G, a.G);
+  if (tail < a.rows) {
+    const long long each = (a.rows - tail + parts - 1) / parts, r0 = tail + part * each;
+    if (r0 < a.rows) rest_rows(a, r0, r0 + each < a.rows ? r0 + each : a.rows, hk * a.G, a.G);
+  }
+}
+// ... of a call without requests
+__global__ __launch_bounds__(256) void kv_rest_kernel(const KvArgs a) {
+  rest_rows(a, a.rows * blockIdx.x / gridDim.x, a.rows * (blockIdx.x + 1ll) / gridDim.x, 0, a.Hq);
 }
 
 // One wavefront, one (row, head), plain arithmetic: a lane per token for the scores, a lane per dim for the sums.
@@ -554,6 +579,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
   const int piece = item % sp.pieces, pair = item / sp.pieces, hk = pair % a.c.Hkv, r = pair / a.c.Hkv;
   const Req rq = request(a, r);
   const int cols = rq.m * a.G, nb = (rq.L + BS - 1) / BS;
+  if (a.rest) rest_of(a, rq, r, hk, qt == 0 && piece == 0, ((long long)r * sp.pieces + piece) * sp.nqt + qt, (long long)a.n * sp.pieces * sp.nqt);
   if (qt * NC >= cols || (piece > 0 && piece * sp.chunk >= nb)) return;
   int lim[NQ], pos[NQ], lim_wg = 0;
   float sl2[NQ];
@@ -1007,16 +1033,23 @@ extern "C" int dmt_kv_attn(const dmt_kv_attn_desc* d, void* stream) {
                 "dmt_kv_attn: n %d (at most 65535), max_q %d, max_len %d, width %d", d->n, d->max_q, d->max_len, d->width);
   DMT_CHECK_ARG(d->scale > 0.f && d->scale <= 1e38f && d->cap >= 0.f && d->cap <= 1e38f,
                 "dmt_kv_attn: scale must be positive, cap 0 or positive, both at most 1e38");
-  if (d->n == 0 || d->max_q == 0 || d->rows == 0) return DMT_OK;
-  DMT_CHECK_ARG(d->Q && d->out && d->lens && d->row_off && (d->table || d->width == 0), "dmt_kv_attn: NULL pointer");
+  const bool none = d->n == 0 || d->max_q == 0;
+  if (d->rows == 0 || (none && !d->rest)) return DMT_OK;
+  DMT_CHECK_ARG(d->Q && d->out && (none || (d->lens && d->row_off && (d->table || d->width == 0))), "dmt_kv_attn: NULL pointer");
   const int64_t wq = (int64_t)d->Hq * d->dh;
   DMT_CHECK_ARG(d->q_rs >= wq && d->o_rs >= wq && d->q_rs % 8 == 0 && d->o_rs % 8 == 0 && (uintptr_t)d->Q % 16 == 0 && (uintptr_t)d->out % 16 == 0,
                 "dmt_kv_attn: rows of at least Hq * dh, 16-byte aligned");
   KvArgs a;
   a.c = {d->Hkv, d->dh, d->n_blocks, (uint8_t*)d->k, (uint8_t*)d->v, (float*)d->k_scale, (float*)d->v_scale};
   a.n = d->n; a.Hq = d->Hq; a.G = d->Hq / d->Hkv; a.max_q = d->max_q; a.max_len = d->max_len; a.width = d->width; a.causal = d->causal != 0;
+  a.rest = d->rest;
   a.rows = d->rows; a.Q = (const bf16_t*)d->Q; a.q_rs = d->q_rs; a.table = d->table; a.lens = d->lens; a.row_off = d->row_off;
   a.scale = d->scale; a.cap = d->cap; a.slopes = d->slopes; a.out = (bf16_t*)d->out; a.o_rs = d->o_rs; a.lse = d->lse;
+  if (none) {
+    kv_rest_kernel<<<(unsigned)(d->rows < 4096 ? d->rows : 4096), 256, 0, (hipStream_t)stream>>>(a);
+    DMT_CHECK_LAUNCH("dmt_kv_attn(no request)");
+    return DMT_OK;
+  }
   DMT_CHECK_ARG(launch_fits(d), "dmt_kv_attn: the launch passes 2^31 workgroups");
   Split s;
   int nq;

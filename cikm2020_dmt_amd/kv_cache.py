@@ -167,7 +167,8 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
     them first; a request that the plan refused has nothing appended, so its rows stand over the last tokens that it held); otherwise
     every row stands behind the last token and sees all (candidates).  Scores as in ops.attn_var: scale, cap, slopes
     (fp32 [H]).  max_q bounds the rows of a request, max_len the lengths (default: what the table can hold): they size the launch, so
-    keep them fixed for a captured graph and tight for speed.  Rows past row_off[n] are not written; with `out` they stay as they were."""
+    keep them fixed for a captured graph and tight for speed.  Rows of no request (before row_off[0], past a request's max_q, past
+    row_off[n]) are zeros, with `out` they stay as they were there; their lse is -inf."""
     dev, n = cache.device, lens.shape[0]
     if table.dim() != 2:
         raise ValueError("table is [n, width], got %s" % list(table.shape))
@@ -208,7 +209,7 @@ def kv_attn(cache: KVCache, q, table, lens, row_off, H, max_q, max_len=None, *, 
     ws = q.new_empty(need, dtype=torch.uint8) if need else None
     a = cache._args
     d = L.kv_attn_desc(n, H, a[0], a[1], a[2], max_q, max_len, table.shape[1], q.shape[0], a[3], a[4], a[5], a[6], q.data_ptr(), q_rs,
-                       table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0,
+                       table.data_ptr(), lens.data_ptr(), row_off.data_ptr(), scale, cap, 1 if causal else 0, 2 if given else 3,
                        0 if slopes is None else slopes.data_ptr(), out.data_ptr(), o_rs, 0 if lse is None else lse.data_ptr(),
                        0 if ws is None else ws.data_ptr(), need)
     _call(dev, "dmt_kv_attn", C.byref(d))

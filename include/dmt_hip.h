@@ -48,6 +48,7 @@ extern "C" {
  *   6  round 6: dmt_mhsa_block_bwd + dmt_mhsa_bwd_image_* added; dmt_sort_pairs / dmt_segment_heads are the library's own kernels (vals_in may be NULL; 16-byte aligned workspace; the
  *   workspace sizes changed), dmt_embgrad_keys takes vals == NULL.
  *   7  dmt_attn_var_* (attention over packed rows of any length with shaped scores and masks) and dmt_kv_* (8-bit K / V cache) added.
+ *   8  dmt_kv_attn_desc: rest, in the place of padding.
  *
  * PACKED ROWS.  A behaviour sequence of a batch may be stored WITHOUT its padding: example b's rows t = 0 .. len[b] - 1 are rows
  * row_off[b] + t of an [R, d] matrix, R = sum_b len[b] (row_off: int32 [B], any order of the examples -- the engine groups examples of
@@ -55,7 +56,7 @@ extern "C" {
  * know about examples take row_off (NULL = the dense [B, T, d] layout, row b * T + t).  Rows t >= len[b] do not exist: in the dense
  * layout they hold finite values nothing reads (the reference masks them as keys, and their gradients are zero), so the
  * two layouts agree on every row that exists.  Dropout counters keep the DENSE element index, so a packed and a dense run draw the same mask. */
-#define DMT_ABI_VERSION 7
+#define DMT_ABI_VERSION 8
 const char* dmt_last_error(void);
 int dmt_version(void);
 /* gfx arch string the device code was built for ("gfx950"). */
@@ -917,6 +918,8 @@ typedef struct {
   const int32_t* table; const int32_t* lens; const int32_t* row_off;
   float scale, cap;
   int32_t causal;
+  int32_t rest;                              /* rows that are computed for no request (before row_off[0], past max_q, past row_off[n]): + 1: zeros in
+                                              * out, + 2: -inf in lse; else they stay as they were (row_off must not fall)              */
   const float* slopes;
   void* out; int64_t o_rs;
   float* lse;                                /* [rows, Hq] or NULL */

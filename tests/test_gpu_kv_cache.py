@@ -567,3 +567,43 @@ def test_rows_and_tokens_past_the_bounds_are_cut_where_they_stand(cuda, m, max_q
         A.close(got[:n, c], ref["out"], ref["out_tol"], "out of head %d" % h)
         A.close(lse[:n, h], ref["lse"], ref["lse_tol"], "lse of head %d" % h)
     assert (got[n:] == 7.0).all()
+
+
+def test_rows_of_nobody_are_zero(cuda):
+    """without `out`, rows that belong to no request, rows past max_q and whole calls without requests give zeros (lse -inf), not what the memory
+    held; with `out` they stay as they were"""
+    H, Hkv, dh, rows = 4, 2, 32, 50
+    lens, m = [100, 30, 70], [7, 0, 12]
+    cache, table, dense = _cache_of(cuda, lens, Hkv, dh, 25)
+    q = torch.randn((rows, H * dh), generator=torch.Generator().manual_seed(26)).to(BF).to(cuda)
+    lens, off = _i(lens, cuda), _i([3, 10, 10, 22], cuda)                         # rows 0 .. 2 and 22 .. 49 are nobody's
+
+    def poison():
+        for shape, dt in (((rows, H * dh), BF), ((rows, H), torch.float32)):
+            bad = torch.full(shape, float("nan"), dtype=dt, device=cuda)
+            del bad                                                              # (the allocator hands the same memory out again)
+
+    poison()
+    want, wl = KV.kv_attn(cache, q, table, lens, off, H, 12, out=torch.full_like(q, 7.0), want_lse=True)
+    assert (want[:3] == 7.0).all() and (want[22:] == 7.0).all() and (wl[:3] == -np.inf).all() and (wl[22:] == -np.inf).all()
+    for max_q in (12, 5, 40):
+        poison()
+        got, lse = KV.kv_attn(cache, q, table, lens, off, H, max_q, want_lse=True)
+        held = torch.zeros(rows, dtype=torch.bool, device=cuda)
+        for a, b in ((3, 10), (10, 22)):
+            held[a:min(b, a + max_q)] = True
+        assert torch.equal(got[held], want[held]) and torch.equal(lse[held], wl[held])
+        assert (got[~held] == 0).all() and (lse[~held] == -np.inf).all()
+    for kw in (dict(max_q=0), dict(max_q=12, table=table[:0], lens=lens[:0], row_off=off[:1])):
+        poison()
+        a = {**dict(table=table, lens=lens, row_off=off, max_q=12), **kw}
+        got, lse = KV.kv_attn(cache, q, a["table"], a["lens"], a["row_off"], H, a["max_q"], want_lse=True)
+        assert (got == 0).all() and (lse == -np.inf).all()
+    big, tb, _d = _cache_of(cuda, [5000, 1], Hkv, dh, 27)                         # the length split over workgroups and joined
+    for max_q in (3, 2):
+        poison()
+        got, lse = KV.kv_attn(big, q, tb, _i([5000, 1], cuda), _i([1, 4, 6], cuda), H, max_q, want_lse=True)
+        held = torch.zeros(rows, dtype=torch.bool, device=cuda)
+        held[1:1 + max_q] = True
+        held[4:6] = True
+        assert (got[held] != 0).any(-1)[:max_q].all() and (got[~held] == 0).all() and (lse[~held] == -np.inf).all()
