@@ -1287,14 +1287,14 @@ class AttnVarFn(torch.autograd.Function):
     every call: two captured graphs never share one)."""
 
     @staticmethod
-    def forward(ctx, q, k, v, slopes, prefix, q_doc, k_doc, q_lens, q_off, k_lens, k_off, cfg, fill, k_shared):
+    def forward(ctx, q, k, v, slopes, prefix, q_doc, k_doc, q_lens, q_off, k_lens, k_off, cfg, fill, k_shared, train):
         H, Hkv = cfg[:2]
         rows, d = q.shape
         out = q.new_zeros((rows, d)) if fill[0] else q.new_empty((rows, d))
         lse = torch.full((rows, H), -float("inf"), device=q.device) if fill[0] else q.new_empty((rows, H), dtype=F32)
         need_sl = slopes is not None and ctx.needs_input_grad[3]
         lens = (q_lens, q_off, k_lens, k_off)
-        lo = torch.empty_like(out) if q.dtype != F32 and any(ctx.needs_input_grad[:4]) else None
+        lo = torch.empty_like(out) if q.dtype != F32 and train else None
         rng = _var_doc_ranges(q_doc, q_lens.shape[0], cfg[5], cfg[6])
         desc = _attn_var_desc(q, k, v, slopes, prefix, q_doc, k_doc, rng, lens, out, lse, lo, cfg)
         L.call("dmt_attn_var_fwd", C.byref(desc), stream_ptr())
@@ -1310,7 +1310,7 @@ class AttnVarFn(torch.autograd.Function):
         q, k, v, slopes, out, lse, lo, *masks = ctx.saved_tensors
         masks, lens = masks[:4], masks[4:]
         if dout is None:
-            return (None,) * 14
+            return (None,) * 15
         if torch.is_grad_enabled():
             raise RuntimeError("attn_var: its gradients have no gradient (create_graph=True)")
         if ctx.k_shared:
@@ -1324,7 +1324,7 @@ class AttnVarFn(torch.autograd.Function):
         ws = q.new_empty(need, dtype=torch.uint8)
         desc.ws, desc.ws_bytes = ws.data_ptr(), need
         L.call("dmt_attn_var_bwd", C.byref(desc), stream_ptr())
-        return (dq, dk, dv, dsl) + (None,) * 10
+        return (dq, dk, dv, dsl) + (None,) * 11
 
 
 def _ids(t, n, what, device):
@@ -1367,8 +1367,10 @@ def attn_var(q, k, v, seqs: AttnSeqs, H, Hkv=None, *, scale=None, cap=0.0, slope
     q_doc, k_doc = (None, None) if docs is None else (_ids(docs[0], q.shape[0], "docs[0]", q.device), _ids(docs[1], k.shape[0], "docs[1]", q.device))
     fill = (seqs.zero_fill, seqs.zero_fill) if seqs.zero_fill is not None else (seqs.total_q != q.shape[0], seqs.total_k != k.shape[0] or seqs.k_shared)
     cfg = (H, Hkv, scale, float(cap), bool(causal), seqs.max_q, seqs.max_k)
+    # (in a Function's forward the grad mode is off, and requires_grad of the operands says nothing about it)
+    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, slopes))
     args = (_aligned_rows(q), _aligned_rows(k), _aligned_rows(v), slopes, prefix, q_doc, k_doc, seqs.q_lens, seqs.q_off, seqs.k_lens, seqs.k_off, cfg,
-            fill, seqs.k_shared)
+            fill, seqs.k_shared, train)
     if _cur_device() == q.device.index:
         out, lse = AttnVarFn.apply(*args)
     else:

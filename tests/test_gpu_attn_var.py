@@ -500,3 +500,17 @@ def test_an_empty_batch_has_gradients(cuda, rows, most):
     assert out.shape == (rows, 64) and (out == 0).all()
     for g, x in zip(torch.autograd.grad(out, lv, torch.ones_like(out)), lv):
         assert g.shape == x.shape and (g == 0).all()
+
+
+def test_nothing_is_kept_for_a_backward_that_will_not_run(cuda, monkeypatch):
+    """under no_grad the part of the output that rounding took away is neither allocated nor written, whatever the operands require"""
+    seen, orig = [], ops._attn_var_desc
+    monkeypatch.setattr(ops, "_attn_var_desc", lambda *a, **kw: seen.append(a[11]) or orig(*a, **kw))
+    lv = [torch.randn((9, 64), device=cuda).to(BF).requires_grad_(True) for _ in range(3)]
+    seqs = ops.AttnSeqs([9], device=cuda)
+    with torch.no_grad():
+        a = ops.attn_var(*lv, seqs, 2)
+    b = ops.attn_var(*lv, seqs, 2)
+    ops.attn_var(*(t.detach() for t in lv), seqs, 2)
+    assert seen[0] is None and seen[1] is not None and seen[2] is None
+    assert torch.equal(a, b)
