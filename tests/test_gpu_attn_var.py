@@ -514,3 +514,33 @@ def test_nothing_is_kept_for_a_backward_that_will_not_run(cuda, monkeypatch):
     ops.attn_var(*(t.detach() for t in lv), seqs, 2)
     assert seen[0] is None and seen[1] is not None and seen[2] is None
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dh,dtype", [(20, F32), (64, F32), (80, F32), (128, F32), (64, BF), (80, BF), (128, BF)])
+def test_fp32_results_have_fp32_bits(cuda, dh, dtype):
+    """Held to the bound of fp32 arithmetic (out in fp32, lse in both types), under what rounding the operands or the weights to a shorter type would
+    leave in rows of few keys (2^-12 for fp16, 2^-9 for bf16).  q and k are multiples of 1/8 up to 1: every partial sum of q . k is a multiple of
+    1/64 under 2^7, exact in any order.  z = x / 16, |z| <= 8; in log2 units its two products and the subtraction of the maximum round by 2^-24 of up
+    to 23 each: 2^-18 in the exponent, as much in the weight; v_exp_f32: 1 ulp, 2^-23.  The sums of weights and of weights times v over at most 300
+    keys: 300 2^-24 = 2^-15.8 of the absolute sum in the worst order, each.  Together under 2^-14.5 of sum p |v|, and of the sum for lse."""
+    g = torch.Generator().manual_seed(dh)
+    ql, kl = [300, 70], [300, 200]
+    n = lambda r: (torch.randint(-8, 9, (r, 2 * dh), generator=g) / 8.0)  # noqa: E731
+    q, k, v = n(370), n(500), n(500)
+    scale = 1.0 / 16
+    out, lse = ops.attn_var(*(t.to(dtype).to(cuda) for t in (q, k, v)), ops.AttnSeqs(ql, kl, device=cuda), 2, scale=scale, causal=True, want_lse=True)
+    qo, ko = [0, 300], [0, 300]
+    for b in range(2):
+        for h in range(2):
+            c = slice(h * dh, h * dh + dh)
+            qq, kk, vv = q[qo[b]:qo[b] + ql[b], c].double(), k[ko[b]:ko[b] + kl[b], c].double(), v[ko[b]:ko[b] + kl[b], c].double()
+            z = qq @ kk.T * scale
+            see = torch.arange(kl[b])[None] <= torch.arange(ql[b])[:, None] + kl[b] - ql[b]
+            z = z.masked_fill(~see, -np.inf)
+            assert float(z[see].abs().max()) <= 8
+            p = torch.softmax(z, -1)
+            # lse: the sum's relative error and 2^-22 of the value (two products, v_log_f32)
+            want = torch.logsumexp(z, -1)
+            assert ((lse[qo[b]:qo[b] + ql[b], h].cpu().double() - want).abs() <= 2.0 ** -14.5 + 2.0 ** -22 * want.abs()).all()
+            if dtype is F32:
+                assert ((out[qo[b]:qo[b] + ql[b], c].cpu().double() - p @ vv).abs() <= 2.0 ** -14.5 * (p @ vv.abs()) + 1e-30).all()
