@@ -443,8 +443,12 @@ __device__ __forceinline__ u32x4_t rsrc_words(const void* base, unsigned bytes) 
   r[3] = 0x00027000u;
   return r;
 }
+// m0, the LDS address of the load, is a reserved register that an asm statement may not leave changed: it is put back behind the load, which has read
+// it by then.  (No output register: nothing that a load in flight could write.)
 __device__ __forceinline__ void load16_lds(const u32x4_t& rsrc, int off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+  unsigned kept;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(kept) : "s"(lds), "v"(off), "s"(rsrc) : "memory");
 }
 template <int DHP, int NW> struct Stage<bf16_t, DHP, NW> {
   typedef Tile<bf16_t, DHP> TL;
