@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
   l += other_half(l);
   lr = sizeof(T) == 2 ? lr + other_half(lr) : l;
   const float inv = lr == 0.f ? 0.f : 1.f / lr;
-  float bad = (l + lr) * 0.f;
+  float bad = 0.f;
 #pragma unroll
   for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(o[dt], dt, half, a.dh);
   const long long row = e.q0 + i;
@@ -217,10 +217,14 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
     }
     if (a.lse && half == 0) a.lse[row * a.Hq + h] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2;
   }
-  unsigned long long again = __ballot(in && !(bad == 0.f));
+  // (a sum that is NaN: so is a score that the row sees, and the whole row)
+  unsigned long long again = __ballot(in && !(bad == 0.f) && l == l);
   again |= again >> 32;
+  if (!again) return;
+  const unsigned long long dims = not_finite_bits<TL::NDT>(o, half, a.dh);
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_fwd<T>(*args_again(), e, h, iw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1)
+      row_fwd<T>(*args_again(), e, h, iw + r, dim_of_row(dims, r, 0, lane), dim_of_row(dims, r, 1, lane), (float*)lds + wave * ROW_LDS, lane);
 }
 
 // (least, largest) document id of every 64 rows, of the queries (blockIdx.z = 0) and of the keys: tiles that share no id are skipped, tiles of

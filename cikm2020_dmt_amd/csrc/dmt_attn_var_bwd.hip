@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
       sp += other_half(sp);
       sl = in ? slope_part(s0, s1, s2, sp) : 0.f;
     }
-    float bad = sl * 0.f;
+    float bad = 0.f;                                     // (sl holds: what is masked was zeroed in both of its factors)
 #pragma unroll
     for (int dt = 0; dt < TL::NDT; ++dt) bad += not_finite(o[dt], dt, half, a.dh);
     if (in) {
@@ -201,13 +201,17 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
 #pragma unroll
       for (int dt = 0; dt < TL::NDT; ++dt) store_dims<T>(o[dt], a.scale, O, dt, half, a.dh);
     }
-    unsigned long long again = __ballot(in && !(bad == 0.f));
+    // (a row that sees something, and whose lse or D is NaN, is NaN)
+    unsigned long long again = __ballot(in && !(bad == 0.f) && (lse == -INFINITY || (lse == lse && D == D)));
     again |= again >> 32;
-    if ((again >> l31) & 1) sl = 0.f;
     if (half) sl = 0.f;                                  // (both halves hold the row's)
     sl = wave_sum(sl);
-    for (int r = 0; r < 32; ++r)
-      if ((again >> r) & 1) sl += row_dq<T>(*args_again(), e, h, iw + r, __shfl(D, r), (float*)lds + wave * ROW_LDS, lane);
+    if (again) {
+      const unsigned long long dims = not_finite_bits<TL::NDT>(o, half, a.dh);
+      for (int r = 0; r < 32; ++r)
+        if ((again >> r) & 1)
+          row_dq<T>(*args_again(), e, h, iw + r, __shfl(D, r), dim_of_row(dims, r, 0, lane), dim_of_row(dims, r, 1, lane), (float*)lds + wave * ROW_LDS, lane);
+    }
   }
   if (a.slope_part) {
     if (lane == 0) part[wave] = sl;
@@ -427,8 +431,14 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
   }
   unsigned long long again = __ballot(in && !(bad == 0.f));
   again |= again >> 32;
+  if (!again) return;
+  unsigned long long bk = 0, bv = 0;
+  if (WHAT & 1) bk = not_finite_bits<TL::NDT>(dk, half, a.dh);
+  if (WHAT & 2) bv = not_finite_bits<TL::NDT>(dv, half, a.dh);
   for (int r = 0; r < 32; ++r)
-    if ((again >> r) & 1) row_dkv<T>(*args_again(), e, hk, part, t0 * KT, min(e.ql, t1 * KT), jw + r, (float*)lds + wave * ROW_LDS, lane);
+    if ((again >> r) & 1)
+      row_dkv<T>(*args_again(), e, hk, part, t0 * KT, min(e.ql, t1 * KT), jw + r, dim_of_row(bk, r, 0, lane), dim_of_row(bk, r, 1, lane),
+                 dim_of_row(bv, r, 0, lane), dim_of_row(bv, r, 1, lane), (float*)lds + wave * ROW_LDS, lane);
 }
 
 // dK = scale (sum of its parts), dV = sum of its parts, in their order: 16 key rows of one example a workgroup.  Bound by the parts' bytes (4 x 2 x 4096

@@ -447,8 +447,9 @@ __global__ __launch_bounds__(256) void kv_rest_kernel(const KvArgs a) {
   rest_rows(a, a.rows * blockIdx.x / gridDim.x, a.rows * (blockIdx.x + 1ll) / gridDim.x, 0, a.Hq);
 }
 
-// One wavefront, one (row, head), plain arithmetic: a lane per token for the scores, a lane per dim for the sums.
-__device__ void kv_row(const KvArgs& a, const Req& rq, int r, int h, int i, float* lds, int lane) {
+// One wavefront, one (row, head), plain arithmetic: a lane per token for the scores, a lane per dim for the sums -- of the dims that the tiles left
+// not finite (s0, s1: of the lane's two), until all of them are NaN, which nothing after them changes.
+__device__ void kv_row(const KvArgs& a, const Req& rq, int r, int h, int i, bool s0, bool s1, float* lds, int lane) {
   float* q = lds;
   float* pl = lds + MAX_DH;
   const int dh = a.c.dh, hk = h / a.G;
@@ -491,12 +492,19 @@ __device__ void kv_row(const KvArgs& a, const Req& rq, int r, int h, int i, floa
       if (lane + 64 < dh) o1 = __builtin_fmaf(pt, f8_to_f32(vb[(long long)(lane + 64) * BS + pc]), o1);
     }
     lds_fence();
+    if (!__any((s0 && o0 == o0) || (s1 && o1 == o1))) break;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   bf16_t* O = a.out + row * a.o_rs + (long long)h * dh;
-  if (lane < dh) O[lane] = f2bf(o0 * inv);
-  if (lane + 64 < dh) O[lane + 64] = f2bf(o1 * inv);
-  if (a.lse && lane == 0) a.lse[row * a.Hq + h] = (m == -INFINITY && l == 0.f) ? -INFINITY : (m + __log2f(l)) * LN2;
+  if (s0) O[lane] = f2bf(o0 * inv);
+  if (s1) O[lane + 64] = f2bf(o1 * inv);
+}
+// which of 8 values are not finite
+__device__ __forceinline__ unsigned not_finite8(const float* x) {
+  unsigned m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m |= x[e] * 0.f == 0.f ? 0u : 1u << e;
+  return m;
 }
 
 // Tiles.  A wavefront takes a block of 64 tokens at a time and the columns of a tile -- 16 NQ (row, head of the group) pairs: heads that share a
@@ -564,6 +572,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
   constexpr int NC = 16 * NQ, NDT = DH / 16, LO = DH + 4;
   __shared__ __attribute__((aligned(16))) float lo[4][NC * LO];
   __shared__ float lm[4][NC], ll[4][NC];
+  __shared__ unsigned char dims[NC][16];       // a bit for each dim of a column that came out not finite
   static_assert(sizeof(lo[0]) >= (MAX_DH + 64) * sizeof(float), "the row form works in a wavefront's part");
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = lane >> 4, l15 = lane & 15;
   const int pairs = a.n * a.c.Hkv, items = pairs * sp.pieces, id = blockIdx.x;
@@ -793,10 +802,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
         make_uint4(dmt_pack_bf16(acc[0] * inv, acc[1] * inv), dmt_pack_bf16(acc[2] * inv, acc[3] * inv), dmt_pack_bf16(acc[4] * inv, acc[5] * inv),
                    dmt_pack_bf16(acc[6] * inv, acc[7] * inv));
     if (a.lse && d8 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
-    float bad = Ls * 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) bad += acc[e] * 0.f;
-    if (!(bad == 0.f)) again |= 1ull << cl;
+    // (a sum that is NaN: so is a score that the row sees, and the whole row)
+    const unsigned bad = Ls == Ls ? not_finite8(acc) : 0u;
+    dims[cl][d8 / 8] = (unsigned char)bad;
+    if (bad) again |= 1ull << cl;
   }
   if (sp.pieces > 1) return;
   // columns that came out not finite once more, by what they may see alone
@@ -809,7 +818,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
     for (int cl = wave; cl < NC; cl += 4)
       if ((redo >> cl) & 1) {
         const int c = qt * NC + cl, i = c / a.G;
-        kv_row(a, rq, r, hk * a.G + c - i * a.G, i, lo[wave], lane);
+        kv_row(a, rq, r, hk * a.G + c - i * a.G, i, lane < DH && ((dims[cl][lane / 8] >> (lane % 8)) & 1),
+               lane + 64 < DH && ((dims[cl][8 + lane / 8] >> (lane % 8)) & 1), lo[wave], lane);
       }
 }
 
@@ -871,19 +881,18 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const KvArgs a, const Spli
   const bool mine = in && g0 == 0;
   const float inv = Ls == 0.f ? 0.f : 1.f / Ls;
   const long long row = rq.row0 + i;
-  float bad = Ls * 0.f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) bad += acc[e] * 0.f;
+  const unsigned bad = mine && Ls == Ls && l15 * 8 < dh ? not_finite8(acc) : 0u;       // (as above)
   if (mine && l15 * 8 < dh)
     *reinterpret_cast<uint4*>(a.out + row * a.o_rs + (long long)h * dh + l15 * 8) =
         make_uint4(dmt_pack_bf16(acc[0] * inv, acc[1] * inv), dmt_pack_bf16(acc[2] * inv, acc[3] * inv), dmt_pack_bf16(acc[4] * inv, acc[5] * inv),
                    dmt_pack_bf16(acc[6] * inv, acc[7] * inv));
   if (mine && a.lse && l15 == 0) a.lse[row * a.Hq + h] = Ls == 0.f ? -INFINITY : (M + __log2f(Ls)) * LN2;
-  const unsigned long long again = __ballot(mine && !(bad == 0.f));
+  const unsigned long long again = __ballot(bad != 0u);
   for (int g = 0; g < 4; ++g)
     if ((again >> (16 * g)) & 0xffff) {
       const int cc = blockIdx.x * per + (wave * 4 + g) / gpc, ii = cc / a.G;
-      kv_row(a, rq, r, hk * a.G + cc - ii * a.G, ii, lo[wave * 4], lane);
+      const unsigned b0 = __shfl(bad, 16 * g + lane / 8), b1 = __shfl(bad, 16 * g + 8 + lane / 8);
+      kv_row(a, rq, r, hk * a.G + cc - ii * a.G, ii, (b0 >> (lane % 8)) & 1, (b1 >> (lane % 8)) & 1, lo[wave * 4], lane);
     }
 }
 

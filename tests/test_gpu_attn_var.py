@@ -544,3 +544,86 @@ def test_fp32_results_have_fp32_bits(cuda, dh, dtype):
             assert ((lse[qo[b]:qo[b] + ql[b], h].cpu().double() - want).abs() <= 2.0 ** -14.5 + 2.0 ** -22 * want.abs()).all()
             if dtype is F32:
                 assert ((out[qo[b]:qo[b] + ql[b], c].cpu().double() - p @ vv).abs() <= 2.0 ** -14.5 * (p @ vv.abs()) + 1e-30).all()
+
+
+def _masked_reference(q, k, v, do, ok, dist, scale, slope):
+    """one head in 64 bits, with sums over the visible places alone: what stands in a masked one does not enter even as 0 * NaN"""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    z = torch.where(ok, (q[:, None] * k[None]).sum(-1) * scale - slope * dist.abs(), torch.full(ok.shape, -np.inf, dtype=torch.float64))
+    p = torch.where(ok, torch.softmax(z, -1), torch.zeros_like(z))
+    over = lambda w, x, dim: torch.where(ok[..., None], w[..., None] * x, torch.zeros((), dtype=torch.float64)).sum(dim)  # noqa: E731
+    out = over(p, v[None], 1)
+    D = (do * out).sum(-1, keepdim=True)
+    dx = torch.where(ok, p * ((do[:, None] * v[None]).sum(-1) - D), torch.zeros_like(z))
+    return dict(out=out, dq=over(dx, k[None], 1) * scale, dk=over(dx, q[:, None], 0) * scale, dv=over(p, do[:, None], 0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("where", ["q", "k", "v", "v dims", "do", "all v"])
+@pytest.mark.parametrize("dh", [32, 80, 128])
+def test_nan_reaches_what_sees_it_and_nothing_else(cuda, dh, where, dtype):
+    """NaN in some places of a causal history with slopes: the same places of every result are NaN as by the definition, with sums over the visible
+    places alone, and the others hold the bounds of the history without it"""
+    n, H = 150, 2
+    q, k, v, do, _, _ = _make([n], [n], H, 1, dh, dtype, 31)
+    clean = [t.clone() for t in (q, k, v, do)]
+    if where == "q":
+        q[70, 5] = np.nan
+    elif where == "k":
+        k[[100, 149], 3] = np.nan
+    elif where == "v":
+        v[[64, 140]] = np.nan
+    elif where == "v dims":
+        v[130, [0, dh - 1]], v[20, 17] = np.nan, np.nan
+    elif where == "do":
+        do[90, dh + 1] = np.nan
+    else:
+        v[:, 9] = np.nan
+    sl = torch.tensor([0.1, 0.02])
+    ref = A.attn_var(*clean[:3], H, 1, [n], [n], [0], [0], causal=True, slopes=sl, dout=clean[3])
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+    out = ops.attn_var(*lv, ops.AttnSeqs([n], device=cuda), H, 1, slopes=sl.to(cuda), causal=True)
+    grads = torch.autograd.grad(out, lv, do.to(cuda))
+    dist = (torch.arange(n)[:, None] - torch.arange(n)[None]).double()
+    want = dict(out=torch.zeros(q.shape, dtype=torch.float64), dq=torch.zeros(q.shape, dtype=torch.float64), dk=0, dv=0)
+    for h in range(H):
+        c = slice(h * dh, h * dh + dh)
+        r = _masked_reference(q[:, c], k, v, do[:, c], dist >= 0, dist, dh ** -0.5, float(sl[h]))
+        want["out"][:, c], want["dq"][:, c] = r["out"], r["dq"]
+        want["dk"], want["dv"] = want["dk"] + r["dk"], want["dv"] + r["dv"]
+    for t, x in zip((out,) + grads, ("out", "dq", "dk", "dv")):
+        assert want[x].isnan().any() or (where == "do" and x == "out") or (where in ("v", "v dims", "all v") and x == "dv")
+        A.close(t, torch.where(want[x].isnan(), want[x], ref[x]), ref[x + "_tol"], x)
+
+
+@pytest.mark.parametrize("where", ["q", "v"])
+def test_nan_in_every_row_is_not_a_matter_of_minutes(cuda, where):
+    """a step whose operands hold NaN everywhere (one NaN weight is enough): the rows that are looked at again stop where NaN has settled them.  Walking
+    them to the end took several hundred times the step; a clean one here takes some 0.2 ms"""
+    n, H, dh = 2048, 8, 64
+    g = torch.Generator(device=cuda).manual_seed(3)
+    q, k, v, do = (torch.empty((2 * n, H * dh), dtype=BF, device=cuda).normal_(generator=g) for _ in range(4))
+    seqs = ops.AttnSeqs([n, n], device=cuda)
+
+    def step(*ops_):
+        lv = [t.detach().requires_grad_(True) for t in ops_]
+        torch.cuda.synchronize()
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        out = ops.attn_var(*lv, seqs, H, causal=True)
+        grads = torch.autograd.grad(out, lv, do)
+        b.record()
+        torch.cuda.synchronize()
+        return a.elapsed_time(b), out, grads
+
+    fine = min(step(q, k, v)[0] for _ in range(4))
+    bad = [t.clone() for t in (q, k, v)]
+    if where == "q":
+        bad[0][:, ::dh] = np.nan
+    else:
+        bad[2][:, ::dh] = np.nan
+    took, out, grads = min((step(*bad) for _ in range(3)), key=lambda r: r[0])
+    cols = torch.arange(H * dh, device=cuda) % dh == 0
+    assert out.isnan().all() if where == "q" else (out[:, cols].isnan().all() and not out[:, ~cols].isnan().any())
+    assert grads[0].isnan().all() and grads[1].isnan().all()
+    assert took < 60 * max(fine, 0.1), "%.2f ms, %.2f ms without NaN" % (took, fine)

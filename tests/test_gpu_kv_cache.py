@@ -607,3 +607,23 @@ def test_rows_of_nobody_are_zero(cuda):
         held[1:1 + max_q] = True
         held[4:6] = True
         assert (got[held] != 0).any(-1)[:max_q].all() and (got[~held] == 0).all() and (lse[~held] == -np.inf).all()
+
+
+@pytest.mark.parametrize("m,L", [(1, 200), (20, 200), (40, 150), (2, 9000), (30, 9000)])
+def test_stored_nan_of_single_dims(cuda, m, L):
+    """NaN stored in single dims of V, of a token that all rows see and of the last one, which only the last row sees (also where the length is split
+    and joined): those dims are NaN where they are seen, every other value holds its bound"""
+    H, Hkv, dh = 4, 2, 80
+    cache, table, dense = _cache_of(cuda, [L], Hkv, dh, 33)
+    for pos, hk, dim in ((5, 0, 3), (5, 1, 79), (L - 1, 0, 64), (L - 1, 1, 0)):
+        cache.v.view(torch.uint8)[int(table[0, pos // BS]), hk, dim, _place(pos % BS)] = 0x7F
+    q = torch.randn((m, H * dh), generator=torch.Generator().manual_seed(34)).to(BF)
+    got = KV.kv_attn(cache, q.to(cuda), table, _i([L], cuda), _i([0, m], cuda), H, m)
+    dist = (L - m + torch.arange(m))[:, None] - torch.arange(L)[None]
+    for h in range(H):
+        hk, c = h // (H // Hkv), slice(h * dh, h * dh + dh)
+        ref = A.head(q[:, c], dense[0][0][hk], dense[0][1][hk], dist >= 0, dist, dh ** -0.5, 0.0, None, BF)
+        want = ref["out"].clone()
+        want[:, 3 if hk == 0 else 79] = np.nan
+        want[-1, 64 if hk == 0 else 0] = np.nan
+        A.close(got[:, c], want, ref["out_tol"], "out of head %d" % h)
