@@ -213,7 +213,9 @@ class CandidateScorer:
             for i, h in enumerate(self.histories):
                 lens, T = eng.seq_lens(dense, i), X[i].shape[1]
                 held = lens.cpu().numpy()
-                empty = torch.as_tensor(np.flatnonzero(held <= 0)).to(dev)
+                empty = np.flatnonzero(held <= 0)
+                if len(empty):
+                    empty = torch.as_tensor(empty).to(dev)
                 new = np.zeros(n, dtype=np.int32)
                 new[users] = np.clip(held, 1, T)
                 at = torch.as_tensor(np.concatenate([r * T + np.arange(new[users[r]]) for r in order])).to(dev)
