@@ -357,15 +357,17 @@ template <int DHP> struct Tile<bf16_t, DHP> {
   static __device__ __forceinline__ f32x16_t mma(const Frag& a, const Frag& b, const f32x16_t& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
-  // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w; sum += the lane's w as they were rounded
+  // acc[dt] += X[row0 .. row0 + 31][dims dt]^T w; sum += the lane's w as they were rounded.  LO: what the rounding took away is multiplied too
+  template <bool LO = false>
   static __device__ __forceinline__ void accumulate(f32x16_t* acc, const bf16_t* X, int row0, const f32x16_t& w, int lane, float* sum = nullptr) {
     const int half = lane >> 5, i16 = lane & 15, grp = (lane >> 4) & 1, r = 4 * half + (i16 >> 2);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      union { bf16x8_t v; unsigned d[4]; } b;
+      union { bf16x8_t v; unsigned d[4]; } b, l;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         b.d[i] = dmt_pack_bf16(w[8 * u + 2 * i], w[8 * u + 2 * i + 1]);
+        if (LO) l.d[i] = dmt_pack_bf16(w[8 * u + 2 * i] - __uint_as_float(b.d[i] << 16), w[8 * u + 2 * i + 1] - __uint_as_float(b.d[i] & 0xffff0000u));
         if (sum) *sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2_t, b.d[i]), __builtin_bit_cast(bf2_t, 0x3f803f80u), *sum, false);
       }
 #pragma unroll
@@ -373,7 +375,9 @@ template <int DHP> struct Tile<bf16_t, DHP> {
         const bf16_t* x = X + (row0 + 16 * u) * RS + at(r, 4 * dt + 2 * grp + ((i16 >> 1) & 1)) + 4 * (i16 & 1);
         const bf16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x));
         const bf16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p4)(x + 8 * RS));
-        acc[dt] = mma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b.v, acc[dt]);
+        const bf16x8_t f = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[dt] = mma(f, b.v, acc[dt]);
+        if (LO) acc[dt] = mma(f, l.v, acc[dt]);
       }
     }
   }
@@ -400,6 +404,7 @@ template <int DHP> struct Tile<float, DHP> {
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
     return c;
   }
+  template <bool LO = false>
   static __device__ __forceinline__ void accumulate(f32x16_t* acc, const float* X, int row0, const f32x16_t& w, int lane, float* = nullptr) {
     const float* x = X + (row0 + 4 * (lane >> 5)) * RS + (lane & 31);
 #pragma unroll

@@ -1,7 +1,9 @@
 // Attention over packed rows of any length: backward.  Two kernels recompute the weights from the saved row sums -- one owns query rows (dQ and
 // the slopes' gradient), one owns key rows (dK, dV, over all query heads of the group) -- so that nothing is added by atomics.
 // P and dX are rounded to bf16 as operands of the matrix instructions: measured error of dQ and dK 0.0024 of their norm, 0.0017 of it the rounding of
-// the result itself; a second product with what the rounding took away would cost a third of the matrix time for that difference.
+// the result itself; a second product with what the rounding took away would cost a third of the matrix time for that difference.  With documents,
+// where few keys share a row and D (from the rounded weights of the output) adds to it, 0.0025 in capped sessions, it is done for dX: 0.0017 (4
+// histories of 2048 in sessions, forward and backward: 166 instead of 161 us; the chain of a walk bounds them, not the matrix pipe).
 #include "dmt_attn_var.h"
 
 using namespace attn_var;
@@ -32,7 +34,7 @@ __device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& cr, const Shape& 
 }
 
 // dQ (and D): one workgroup owns 128 or 64 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of
-// dQ^T += K^T dX.  Bound by the matrix pipe: 2 x 4096 causal, 16 heads of 128: 209 us = 984 TFLOP/s; 256 histories of up to 200, 4 heads of 80: 48 us.
+// dQ^T += K^T dX.  Bound by the matrix pipe: 2 x 4096 causal, 16 heads of 128: 210 us = 977 TFLOP/s; 256 histories of up to 200, 4 heads of 80: 46 us.
 template <typename T, int DHP, int SHAPE, bool DOCS, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
@@ -172,7 +174,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
           s[r] *= dp[r] - D;
           if (SHAPE == 2) s[r] *= dmt_cap::derivative(cr[r]);
         }
-        TL::accumulate(o, Kl, 32 * u, s, lane);
+        TL::template accumulate<DOCS>(o, Kl, 32 * u, s, lane);
       }
     }
     if (NB == 1) __syncthreads();
@@ -241,8 +243,8 @@ __global__ __launch_bounds__(256) void slopes_kernel(const Args a, long long n) 
 // dK, dV: one workgroup owns 128 keys (a wavefront 32, their K and V rows in registers) and walks over the queries of every head of the group in
 // tiles of 64: S and dP with lane = key, P and dX packed are the B operands of dV^T += dO^T P and dK^T += Q^T dX.  Nothing crosses wavefronts.
 // WHAT: 1 = dK, 2 = dV, 3 = both.  Both accumulators and both operands' rows fit the 256 registers of two wavefronts a SIMD up to 80 dims (64 in
-// fp32); wider heads take a kernel each -- one more product of scores, but at 4096 causal keys, 16 heads of 128 dims 225 + 164 us against 443 us
-// for one kernel with one wavefront a SIMD (accumulators moved between register files) and 1033 us with spills.  (915 and 837 TFLOP/s; up to 80 dims
+// fp32); wider heads take a kernel each -- one more product of scores, but at 4096 causal keys, 16 heads of 128 dims 221 + 164 us against 443 us
+// for one kernel with one wavefront a SIMD (accumulators moved between register files) and 1033 us with spills.  (930 and 835 TFLOP/s; up to 80 dims
 // two kernels would lose: 4 histories of 2048 in sessions 77 to 92 us against 71 to 84 for one.)  256 histories of up to 200, 4 heads of 80: 49 us.
 template <typename T, int DHP, int SHAPE, bool DOCS, int WHAT>
 __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, int nqt) {
@@ -389,7 +391,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
             if (SHAPE == 2) s[4 * gg + c] *= dmt_cap::derivative(cr[4 * gg + c]);
           }
         }
-        TL::accumulate(dk, Ql, 32 * u, s, lane);
+        TL::template accumulate<DOCS>(dk, Ql, 32 * u, s, lane);
       }
     }
     if (NB == 1) __syncthreads();
@@ -442,7 +444,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
 }
 
 // dK = scale (sum of its parts), dV = sum of its parts, in their order: 16 key rows of one example a workgroup.  Bound by the parts' bytes (4 x 2 x 4096
-// rows of 512: 26 us; 4 histories of 2048: 12 us).
+// rows of 512, 134 MB of K and V: 35 us; 4 histories of 2048: 12 us).
 template <typename T>
 __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
   const Ex e = example(a, blockIdx.y);
