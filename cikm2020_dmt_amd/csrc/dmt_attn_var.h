@@ -625,19 +625,23 @@ inline int rows_of(const attn_var::Args& a, int dhp) {
   return dhp <= 80 && (long long)a.B * a.Hq * cdiv64(a.max_q, 128) <= 512 ? 64 : 128;
 }
 
-// the kernels' variants: scores as they are (0), with slopes alone (1), capped and perhaps with slopes (2); documents or none
+// The kernels' variants: scores as they are (0), with slopes alone (1), capped and perhaps with slopes (2; 3: near, see dmt_cap); documents or none.
+// (One kernel with a branch between 2 and 3 takes the registers of both: 128 dims causal with a cap of 20 took 669 instead of 542 us.)
 template <int V> struct Const { static constexpr int value = V; };
-template <typename F> void with_shape(const attn_var::Args& a, F f) {
-  const int shape = a.cap > 0.f ? 2 : (a.slopes ? 1 : 0);
-  if (a.q_doc) {
-    if (shape == 0) f(Const<0>(), Const<1>());
-    else if (shape == 1) f(Const<1>(), Const<1>());
-    else f(Const<2>(), Const<1>());
-  } else {
-    if (shape == 0) f(Const<0>(), Const<0>());
-    else if (shape == 1) f(Const<1>(), Const<0>());
-    else f(Const<2>(), Const<0>());
+template <typename T, typename DOCS, typename F> void with_score(const attn_var::Args& a, DOCS docs, F f) {
+  if (!(a.cap > 0.f)) {
+    if (a.slopes) f(Const<1>(), docs);
+    else f(Const<0>(), docs);
+    return;
   }
+  if constexpr (sizeof(T) == 2) {
+    if (!dmt_cap(a.scale, a.cap, true).near) return f(Const<2>(), docs);
+  }
+  f(Const<3>(), docs);
+}
+template <typename T, typename F> void with_shape(const attn_var::Args& a, F f) {
+  if (a.q_doc) with_score<T>(a, Const<1>(), f);
+  else with_score<T>(a, Const<0>(), f);
 }
 
 int dmt_attn_var_args(const dmt_attn_var_desc* d, attn_var::Args* a, bool backward, const char* what);

@@ -11,7 +11,9 @@ namespace {
 // One pass: the running maximum m moves only when a row's scores pass it by more than 2^8 (the weights
 // are then at most 256, exact in fp32 sums and without loss in bf16), so the output is rescaled a few times a row instead of every tile.
 // What bounds it: the matrix pipe and, beside it, one power and about 4 other vector operations a score (2 x 4096 causal, 16 heads of 128: 171 us =
-// 802 TFLOP/s of the products that the mask leaves); for short histories the rows (256 of up to 200, 4 heads of 80: 38 us, 57 MB).
+// 802 TFLOP/s of the products that the mask leaves); for short histories the rows (256 of up to 200, 4 heads of 80: 37 us, 57 MB).
+// fp32 takes 32x32x2 products; past 64 dims its operands and sums do not fit the registers and part of them goes to scratch (64 histories of up to
+// 200 with slopes, 4 heads of 20 / 80 / 128: 27 / 74 / 86 us, dQ 37 / 128 / 142, dK and dV 41 / 134 / 229).
 template <typename T, int DHP, int SHAPE, bool DOCS, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int nt) {
   typedef Tile<T, DHP> TL;
@@ -97,16 +99,11 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_fwd_kernel(const Args a, int 
       }
       settle(s[0], s[1]);
       if (SHAPE) {
-        if (SHAPE == 2 && (sizeof(T) == 4 || sh.cap.near)) {
+        if (SHAPE >= 2) {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = sh.cap.less<true>(s[u][r], sh.cap.r(s[u][r]), 0.f);
-        } else if (SHAPE == 2) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[u][r] = sh.cap.less<false>(s[u][r], sh.cap.r(s[u][r]), 0.f);
+            for (int r = 0; r < 16; ++r) s[u][r] = sh.cap.less<SHAPE == 3>(s[u][r], sh.cap.r(s[u][r]), 0.f);
         } else {
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -247,7 +244,7 @@ __global__ __launch_bounds__(256) void doc_ranges_kernel(const Args a) {
 template <typename T, int DHP, int NW> void launch_tile_as(const Args& a, hipStream_t st) {
   const int nt = (int)cdiv64(a.max_q, 32 * NW);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  with_shape(a, [&](auto shape, auto docs) { tile_fwd_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
+  with_shape<T>(a, [&](auto shape, auto docs) { tile_fwd_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
 }
 template <typename T, int DHP> void launch_tile(const Args& a, hipStream_t st) {
   if constexpr (DHP <= 80) {

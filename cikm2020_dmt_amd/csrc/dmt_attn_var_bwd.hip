@@ -12,25 +12,20 @@ namespace {
 
 // The scores of one 32 x 32 tile, in place: z2 minus the row statistic (kept in rows or, stat[], in registers).  d0: distance of register row 0
 // and the lane's column; STEP: what a register row adds to it.  cr: what the cap's derivative needs.
-template <int SHAPE, int STEP, bool NEAR, typename STAT>
-__device__ __forceinline__ void weights_as(f32x16_t& s, f32x16_t& cr, const Shape& sh, float d0, STAT stat) {
+template <int SHAPE, int STEP, typename STAT>
+__device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& cr, const Shape& sh, float d0, STAT stat) {
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     float z;
-    if (SHAPE == 2) {
+    if (SHAPE >= 2) {
       cr[r] = sh.cap.r(s[r]);
-      z = sh.cap.less<NEAR>(s[r], cr[r], stat(r));
+      z = sh.cap.less<SHAPE == 3>(s[r], cr[r], stat(r));
     } else {
       z = __builtin_fmaf(s[r], sh.cap.c1, -stat(r));
     }
-    if (SHAPE == 1 || (SHAPE == 2 && sh.slope)) z = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), z);
+    if (SHAPE == 1 || (SHAPE >= 2 && sh.slope)) z = __builtin_fmaf(-sh.sl2, fabsf(d0 + (float)(STEP * reg_row(r, 0))), z);
     s[r] = exp2_hw(z);
   }
-}
-template <typename T, int SHAPE, int STEP, typename STAT>
-__device__ __forceinline__ void weights(f32x16_t& s, f32x16_t& cr, const Shape& sh, float d0, STAT stat) {
-  if (SHAPE == 2 && (sizeof(T) == 4 || sh.cap.near)) weights_as<SHAPE, STEP, true>(s, cr, sh, d0, stat);
-  else weights_as<SHAPE, STEP, false>(s, cr, sh, d0, stat);
 }
 
 // dQ (and D): one workgroup owns 128 or 64 queries of a head, as in the forward: S^T and dP^T with lane = query, dX packed is the B operand of
@@ -141,7 +136,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
         }
         const float d0 = (float)(i + e.off - k0 - 32 * u - 4 * half);
         settle(s, dp);
-        weights<T, SHAPE, -1>(s, cr, sh, d0, [&](int) { return lse2; });
+        weights<SHAPE, -1>(s, cr, sh, d0, [&](int) { return lse2; });
         if (docs_differ || cut) {
           // (a masked place gives weight and gradient 0 whatever stands there)
           const int pre = e.pre - k0 - 32 * u - 4 * half, lm = (docs_differ ? lim0 : lim) - k0 - 32 * u - 4 * half;
@@ -172,7 +167,7 @@ __global__ __launch_bounds__(64 * NW, 2) void tile_dq_kernel(const Args a, int n
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           s[r] *= dp[r] - D;
-          if (SHAPE == 2) s[r] *= dmt_cap::derivative(cr[r]);
+          if (SHAPE >= 2) s[r] *= dmt_cap::derivative(cr[r]);
         }
         TL::template accumulate<DOCS>(o, Kl, 32 * u, s, lane);
       }
@@ -363,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
         f32x4_t ls[4];
 #pragma unroll
         for (int gg = 0; gg < 4; ++gg) ls[gg] = *reinterpret_cast<const f32x4_t*>(&stats[buf][0][32 * u + 8 * gg + 4 * half]);
-        weights<T, SHAPE, 1>(s, cr, sh, (float)(i0 + 32 * u + 4 * half + e.off - j), [&](int r) { return ls[r >> 2][r & 3]; });
+        weights<SHAPE, 1>(s, cr, sh, (float)(i0 + 32 * u + 4 * half + e.off - j), [&](int r) { return ls[r >> 2][r & 3]; });
         if (docs_differ || cut) {
           const int lo = lo_l - i0 - 32 * u - 4 * half;
 #pragma unroll
@@ -388,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void tile_dkv_kernel(const Args a, int nt, 
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             s[4 * gg + c] *= dp[4 * gg + c] - D[c];
-            if (SHAPE == 2) s[4 * gg + c] *= dmt_cap::derivative(cr[4 * gg + c]);
+            if (SHAPE >= 2) s[4 * gg + c] *= dmt_cap::derivative(cr[4 * gg + c]);
           }
         }
         TL::template accumulate<DOCS>(dk, Ql, 32 * u, s, lane);
@@ -470,7 +465,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(const Args a) {
 template <typename T, int DHP, int NW> void launch_dq_as(const Args& a, hipStream_t st) {
   const int nt = (int)cdiv64(a.max_q, 32 * NW);
   const unsigned grid = (unsigned)((long long)nt * a.Hq * a.B);
-  with_shape(a, [&](auto shape, auto docs) { tile_dq_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
+  with_shape<T>(a, [&](auto shape, auto docs) { tile_dq_kernel<T, DHP, decltype(shape)::value, decltype(docs)::value, NW><<<grid, 64 * NW, 0, st>>>(a, nt); });
 }
 template <typename T, int DHP> void launch_dq(const Args& a, hipStream_t st) {
   if constexpr (DHP <= 80) {
@@ -480,7 +475,7 @@ template <typename T, int DHP> void launch_dq(const Args& a, hipStream_t st) {
 }
 template <typename T, int DHP> void launch_dkv(const Args& a, int nt, int nqt, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)nt * a.Hkv * a.B * a.parts), more = a.slope_part ? a.Hq : 0;
-  with_shape(a, [&](auto shape, auto docs) {
+  with_shape<T>(a, [&](auto shape, auto docs) {
     constexpr int S = decltype(shape)::value;
     constexpr bool D = decltype(docs)::value;
     if constexpr (DHP > (sizeof(T) == 2 ? 80 : 64)) {

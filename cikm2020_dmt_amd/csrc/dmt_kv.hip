@@ -35,8 +35,8 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((unsigned)
 // ================================================================================================================ plan
 // The sums run over the requests in chunks of one workgroup (1024): rows, blocks wanted, runs.  What a row needs -- its request, position,
 // block -- it then finds by itself (a binary search over row_off), so the second part is as wide as there are rows; with few rows and
-// requests the first workgroup does it too and there is one launch.  Latency bounds it: 64 requests of one event 4.7 us; 2000 requests with 600000
-// rows 6.2 + 5.9 us.
+// requests the first workgroup does it too and there is one launch.  Latency bounds it: 64 requests of one event 4.8 us; 2000 requests with 270000
+// rows 5.7 + 7.1 us.
 constexpr int PLAN_NT = 1024;
 constexpr int PLAN_SMALL_ROWS = 4096;
 
@@ -212,7 +212,7 @@ struct Cache {
 
 // One workgroup owns a (run, head): its rows are held in registers between the maximum and the rounding.  What bounds it is the rows' bytes; the
 // bytes of V pass through LDS because they lie across the tokens (68 bytes a dim there: the 16 chunks of a row would meet in one bank at 64).
-// 256 requests of one event, 8 heads of 128: 10 us; 40000 rows of them: 35 us.  (A thread with 4 side-by-side tokens, whole words of V instead of
+// 256 requests of one event, 8 heads of 128: 11 us; 16 fills of up to 2500 rows: 36 us.  (A thread with 4 side-by-side tokens, whole words of V instead of
 // bytes: 33 us for the rows, but 12 to 15 for the events; bytes of V straight to memory for short runs did not help.)
 constexpr int VLD = BS + 4;
 __global__ __launch_bounds__(256) void append_kernel(const Cache c, int rows, const bf16_t* kr, long long k_rs, const bf16_t* vr, long long v_rs,
@@ -515,9 +515,9 @@ __device__ __forceinline__ unsigned not_finite8(const float* x) {
 //                 row are two steps of 8 -- and Q is laid out the same way; a remainder of 16 dims is a step whose upper half is zero
 //                 (a 16x16x16 product that adds to the result of a 16x16x32 one just before it came out wrong here).
 //   O^T = V^T P^T (dims x columns): the weights of S^T, packed, are the B operand; the places of V are in that order.
-// What bounds it: the cache's bytes for few columns (64 ragged requests of up to 8192 tokens, 32 heads on 8 of 128, one row each: 117 us, 4.7 TB/s);
-// with many columns the walk of a wavefront over its blocks, load after load (16 requests of up to 1000 tokens, 300 rows, 4 heads of 80: 23 us;
-// requesting the next block ahead takes the registers of a third workgroup: 30; 48 columns a tile: 34); for a single short request the launch (4.6 us).
+// What bounds it: the cache's bytes for few columns (64 ragged requests of up to 8192 tokens, 32 heads on 8 of 128, one row each: 117 to 121 us, 4.6 TB/s);
+// with many columns the walk of a wavefront over its blocks, load after load (16 requests of up to 1000 tokens, 300 rows, 4 heads of 80: 24 us;
+// requesting the next block ahead takes the registers of a third workgroup: 30; 48 columns a tile: 34); for a single short request the launch (4.8 us).
 typedef __attribute__((ext_vector_type(8))) short bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) short bf16x4_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
@@ -566,7 +566,8 @@ template <int DH> struct Dims {
   static constexpr int KW = 4 * N64 + 2 * N32 + N16;                                       // dwords of a lane
 };
 
-template <int DH, int NQ, bool SHAPED>
+// SHAPE: 0 the scores as they are, 1 with a cap and / or slopes, 2 with a cap that takes the longer form (dmt_cap: near)
+template <int DH, int NQ, int SHAPE>
 __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const Split sp, float* __restrict__ part_o, float2* __restrict__ part_ml) {
   typedef Dims<DH> DM;
   constexpr int NC = 16 * NQ, NDT = DH / 16, LO = DH + 4;
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
     const int i = in ? c / a.G : 0, g = in ? c - i * a.G : 0, h = hk * a.G + g;
     lim[x] = in ? sees(a, rq, i) : 0;
     pos[x] = position(a, rq, i);
-    sl2[x] = SHAPED && a.slopes ? a.slopes[h] * LOG2E : 0.f;
+    sl2[x] = SHAPE && a.slopes ? a.slopes[h] * LOG2E : 0.f;
     const bf16_t* Q = a.Q + (rq.row0 + i) * a.q_rs + (long long)h * DH;
     const bf16x8_t z8 = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
@@ -703,28 +704,27 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
       const int lx = lim[x] - j0 - 4 * grp;
       const float d0 = (float)(pos[x] - j0 - 4 * grp);
       float mx = -INFINITY;
-      if (SHAPED) {
+      if (SHAPE) {
         const auto each = [&](auto score) {
 #pragma unroll
           for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[x][u][e] = score(s[x][u][e]);
         };
-        if (!(a.cap > 0.f)) each([&](float z) { return c1 * z; });
-        else if (cap.near) each([&](float z) { return cap.less<true>(z, cap.r(z), 0.f); });
-        else each([&](float z) { return cap.less<false>(z, cap.r(z), 0.f); });
+        if (SHAPE == 1 && !(a.cap > 0.f)) each([&](float z) { return c1 * z; });
+        else each([&](float z) { return cap.less<SHAPE == 2>(z, cap.r(z), 0.f); });
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float z = s[x][u][e];
-          if (SHAPED) z = __builtin_fmaf(-sl2[x], fabsf(d0 - (float)(16 * u + e)), z);
+          if (SHAPE) z = __builtin_fmaf(-sl2[x], fabsf(d0 - (float)(16 * u + e)), z);
           z = 16 * u + e < lx ? z : -INFINITY;
           s[x][u][e] = z;
           mx = fmaxf(mx, z);
         }
-      mx = col_max(mx) * (SHAPED ? 1.f : c1);
+      mx = col_max(mx) * (SHAPE ? 1.f : c1);
       if (__any(mx > m[x] + 8.f)) {               // (as in the tile kernels of attn_var: weights up to 2^8 before the output is rescaled)
         const float mn = fmaxf(m[x], mx), f = m[x] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[x] - mn);
         m[x] = mn;
@@ -739,7 +739,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(const KvArgs a, const S
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[x][u][e] = __builtin_amdgcn_exp2f(SHAPED ? s[x][u][e] - mu : __builtin_fmaf(s[x][u][e], c1, -mu));
+          s[x][u][e] = __builtin_amdgcn_exp2f(SHAPE ? s[x][u][e] - mu : __builtin_fmaf(s[x][u][e], c1, -mu));
           l[x] += s[x][u][e];
         }
 #pragma unroll
@@ -919,8 +919,9 @@ Split split_of(int n, int Hkv, int G, int max_q, int max_len, int& nq) {
 
 template <int DH, int NQ> void launch_kv(const KvArgs& a, const Split& s, float* po, float2* ml, hipStream_t st) {
   const unsigned grid = (unsigned)((long long)a.n * a.c.Hkv * s.pieces * s.nqt);
-  if (a.cap > 0.f || a.slopes) kv_tile_kernel<DH, NQ, true><<<grid, 256, 0, st>>>(a, s, po, ml);
-  else kv_tile_kernel<DH, NQ, false><<<grid, 256, 0, st>>>(a, s, po, ml);
+  if (a.cap > 0.f && dmt_cap(a.scale, a.cap, true).near) kv_tile_kernel<DH, NQ, 2><<<grid, 256, 0, st>>>(a, s, po, ml);
+  else if (a.cap > 0.f || a.slopes) kv_tile_kernel<DH, NQ, 1><<<grid, 256, 0, st>>>(a, s, po, ml);
+  else kv_tile_kernel<DH, NQ, 0><<<grid, 256, 0, st>>>(a, s, po, ml);
 }
 template <int NQ> void launch_kv_dh(const KvArgs& a, const Split& s, float* po, float2* ml, hipStream_t st) {
   switch (a.c.dh) {
