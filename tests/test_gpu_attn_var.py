@@ -646,3 +646,41 @@ def test_gradients_with_documents_are_as_exact_as_their_rounding(cuda, cap, Hkv)
     for t, x in zip(torch.autograd.grad(out, lv, do.to(cuda))[:2], ("dq", "dk")):
         alone = (ref[x].to(BF).double() - ref[x]).norm()
         assert (t.cpu().double() - ref[x]).norm() <= 1.2 * alone, x
+
+
+@pytest.mark.parametrize("dh", [32, 64, 80, 128])
+@pytest.mark.parametrize("cap", [64.0, 65.0, 400.0])
+def test_caps_on_both_sides_of_the_short_form(cuda, cap, dh):
+    """bf16 takes the short form of a cap up to 64, kernels of their own beyond; few and many rows a workgroup, with and without documents, scores that
+    reach the cap"""
+    docs = (np.arange(200) * 5 // 200, np.arange(200) * 5 // 200)
+    _check(cuda, [130, 70], [130, 70], 4, 2, dh, std=8.0, cap=cap, causal=True, slopes=[0.1, 0.0, 1.0, 0.01], scale=0.5)
+    _check(cuda, [130, 70], [130, 70], 2, 2, dh, std=2.0, cap=cap, docs=tuple(torch.as_tensor(d) for d in docs), prefix=[3, 0])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("where", ["q", "v", "v dims", "do"])
+def test_nan_stays_in_its_document(cuda, where, dtype):
+    """NaN in one session of a causal history behind a prefix: what sees that session, and nothing else"""
+    n, H, dh, prefix = 160, 2, 64, 5
+    q, k, v, do, _, _ = _make([n], [n], H, 1, dh, dtype, 51)
+    clean = [t.clone() for t in (q, k, v, do)]
+    t, at = {"q": (q, (90,)), "v": (v, (100,)), "v dims": (v, (85, [0, 63])), "do": (do, (95, slice(0, dh)))}[where]
+    t[at] = np.nan
+    doc = torch.as_tensor(np.arange(n) // 40, dtype=torch.int32)
+    ref = A.attn_var(*clean[:3], H, 1, [n], [n], [0], [0], causal=True, prefix=[prefix], docs=(doc, doc), dout=clean[3])
+    lv = [t.to(cuda).requires_grad_(True) for t in (q, k, v)]
+    d = doc.to(cuda)
+    out = ops.attn_var(*lv, ops.AttnSeqs([n], device=cuda), H, 1, causal=True, docs=(d, d), prefix=torch.tensor([prefix], dtype=torch.int32, device=cuda))
+    grads = torch.autograd.grad(out, lv, do.to(cuda))
+    ok, dist = A.visible(n, n, True, prefix, doc, doc), (torch.arange(n)[:, None] - torch.arange(n)[None]).double()
+    want = dict(out=torch.zeros(q.shape, dtype=torch.float64), dq=torch.zeros(q.shape, dtype=torch.float64), dk=0, dv=0)
+    for h in range(H):
+        c = slice(h * dh, h * dh + dh)
+        r = _masked_reference(q[:, c], k, v, do[:, c], ok, dist, dh ** -0.5, 0.0)
+        want["out"][:, c], want["dq"][:, c] = r["out"], r["dq"]
+        want["dk"], want["dv"] = want["dk"] + r["dk"], want["dv"] + r["dv"]
+    for t, x in zip((out,) + grads, ("out", "dq", "dk", "dv")):
+        nan = want[x].isnan()
+        assert not nan[:80].all() and not nan[120:].any()
+        A.close(t, torch.where(nan, want[x], ref[x]), ref[x + "_tol"], x)

@@ -627,3 +627,41 @@ def test_stored_nan_of_single_dims(cuda, m, L):
         want[:, 3 if hk == 0 else 79] = np.nan
         want[-1, 64 if hk == 0 else 0] = np.nan
         A.close(got[:, c], want, ref["out_tol"], "out of head %d" % h)
+
+
+@pytest.mark.parametrize("dh", [16, 80, 128])
+@pytest.mark.parametrize("cap", [64.0, 65.0, 400.0])
+def test_caps_on_both_sides_of_the_short_form(cuda, cap, dh):
+    """caps up to 64 take the short form, kernels of their own beyond: few rows and many, a length in pieces, scores that reach the cap"""
+    _attn_check(cuda, [200, 65], [1, 4], 4, 2, dh, cap=cap, scale=4.0, slopes=[0.1, 0.0, 1.0, 0.01])
+    _attn_check(cuda, [200, 65], [30, 64], 4, 2, dh, cap=cap, scale=4.0)
+    _attn_check(cuda, [9000], [2], 2, 1, dh, cap=cap, causal=False)
+
+
+def test_a_replay_with_other_rows_leaves_zeros_where_nobody_is(cuda):
+    """one captured step, replayed with more, fewer and no rows of each request, and with other lengths: every replay as the eager call, the rest zero"""
+    H, Hkv, dh, rows = 4, 2, 64, 24
+    cache, table, _ = _cache_of(cuda, [300, 70, 129], Hkv, dh, 61)
+    q = torch.randn((rows, H * dh), generator=torch.Generator().manual_seed(62)).to(BF).to(cuda)
+    lens, off = _i([300, 70, 129], cuda), _i([0, 4, 8, 12], cuda)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        KV.kv_attn(cache, q, table, lens, off, H, 8, want_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = KV.kv_attn(cache, q, table, lens, off, H, 8, want_lse=True)
+    for L, o in (([300, 70, 129], [0, 8, 16, 24]), ([10, 70, 64], [2, 2, 7, 9]), ([300, 1, 0], [0, 0, 0, 0]), ([299, 69, 100], [5, 6, 7, 20])):
+        lens.copy_(_i(L, cuda))
+        off.copy_(_i(o, cuda))
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        graph.replay()
+        want, wl = KV.kv_attn(cache, q, table, lens, off, H, 8, want_lse=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+        held = torch.zeros(rows, dtype=torch.bool, device=cuda)
+        for a, b in zip(o, o[1:]):
+            held[a:min(b, a + 8)] = True
+        assert (out[~held] == 0).all() and (lse[~held] == -np.inf).all()
